@@ -270,6 +270,43 @@ int bdh_rank_barrier(const long long* flag_ptrs, int rank, int world, unsigned e
 int bdh_wait_timeout_probe(const unsigned* flag, unsigned value, unsigned long long limit_ns, int* status,
                            cudaStream_t s);
 
+// ---- parts of a state-space layer (rows of fp32 / fp16 / bf16 elements; channels are adjacent) ----------------
+enum { BDH_F32 = 0, BDH_F16 = 1, BDH_BF16 = 2 };
+
+// Causal depthwise convolution, s = [state | x]: y_t = act(bias + sum_j w[:, j] s_{t+j}), state' = the last k - 1
+// rows of s before the sequence's length (causal_conv.cu). x, state, state_out, dy: strides in elements of the batch
+// and of a row; y, dx, dstate, dstate_out: contiguous. w [C, k] and bias [C] fp32. lengths: int32 / int64 [B] or null
+// (values are clamped to [0, T]); rows behind a length give y = 0 and take no part in any gradient.
+typedef struct {
+  const void* x;
+  long long x_sb, x_st;
+  const float* w;
+  const float* bias;          // or null
+  const void* state;          // [B, k - 1, C], or null: zeros
+  long long state_sb, state_sr;
+  const void* lengths;
+  int lengths64;
+  int B, T, C, k;             // k <= 8
+  int dtype, silu;
+  void* y;                    // [B, T, C]
+  void* state_out;            // [B, k - 1, C], or null
+  long long state_out_sb, state_out_sr;
+  const void* dy;             // backward only, from here on
+  long long dy_sb, dy_st;
+  const void* dstate_out;     // gradient of state_out, or null
+  void* dx;
+  void* dstate;               // or null
+} BdhConvDesc;
+
+int bdh_causal_conv_fwd(const BdhConvDesc* d, cudaStream_t s);
+// fp32 scratch that the backward pass needs for dw and db
+long long bdh_causal_conv_partials(const BdhConvDesc* d);
+// dw [C, k], db [C] (either may be null) are written, not added to
+int bdh_causal_conv_bwd(const BdhConvDesc* d, float* dw, float* db, float* partial, cudaStream_t s);
+// One row per sequence (T = 1): y [B, C]; state_out may be the state itself. active (bytes, or null): a stream whose
+// byte is 0 gives y = 0 and keeps its state.
+int bdh_causal_conv_step(const BdhConvDesc* d, const unsigned char* active, cudaStream_t s);
+
 // Checked build (-DBDH_DEBUG_BOUNDS; csrc/debug_bounds.cuh): the first data-dependent index that was
 // out of range in the kernels of rowwise.cu / graph.cu. out5 = {checked build?, site, index, extent, where}.
 int bdh_bounds_record_rowwise(long long* out5, int clear);

@@ -1,0 +1,175 @@
+// torch.ops.bdh.* of the parts of a state-space layer (causal convolution, per-head norm + rotation, selective
+// scan). As in bindings.cpp the caller allocates every output and all scratch; shapes that the kernels rely on are
+// checked here once more, so that a direct call cannot make them read or write out of range.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+
+#include "bdh_kernels.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+void check_rc(int rc, const char* what) { TORCH_CHECK(rc == BDH_OK, "bdh kernel '", what, "' failed with code ", rc); }
+
+cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+int elem_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return BDH_F32;
+    case at::kHalf: return BDH_F16;
+    case at::kBFloat16: return BDH_BF16;
+    default: TORCH_CHECK(false, name, ": expected fp32, fp16 or bf16");
+  }
+}
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// `t` on the device of `on`, of type `type` and the given sizes, the last dimension adjacent
+void check_rows(const Tensor& t, const Tensor& on, at::ScalarType type, at::IntArrayRef sizes, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == on.device(), name, ": expected a tensor on ", on.device());
+  TORCH_CHECK(t.scalar_type() == type, name, ": expected ", type, ", got ", t.scalar_type());
+  TORCH_CHECK(t.sizes() == sizes, name, ": expected sizes ", sizes, ", got ", t.sizes());
+  TORCH_CHECK(t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1, name, ": expected a last dimension of stride 1");
+}
+
+void check_dense(const Tensor& t, const Tensor& on, at::ScalarType type, at::IntArrayRef sizes, const char* name) {
+  check_rows(t, on, type, sizes, name);
+  TORCH_CHECK(t.is_contiguous(), name, ": expected a contiguous tensor");
+}
+
+void check_f32(const OptTensor& t, const Tensor& on, at::IntArrayRef sizes, const char* name) {
+  if (given(t)) check_dense(*t, on, at::kFloat, sizes, name);
+}
+
+const float* f32_ptr(const OptTensor& t) { return given(t) ? t->const_data_ptr<float>() : nullptr; }
+float* f32_out(const OptTensor& t) { return given(t) ? t->data_ptr<float>() : nullptr; }
+
+void set_lengths(const OptTensor& t, const Tensor& on, int64_t B, const void*& ptr, int& is64) {
+  ptr = nullptr;
+  is64 = 0;
+  if (!given(t)) return;
+  TORCH_CHECK(t->is_cuda() && t->device() == on.device() && t->dim() == 1 && t->size(0) == B && t->is_contiguous() &&
+              (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong), "lengths: expected int32 or int64 [", B, "] on ",
+              on.device());
+  ptr = t->const_data_ptr();
+  is64 = t->scalar_type() == at::kLong;
+}
+
+const unsigned char* active_ptr(const OptTensor& t, const Tensor& on, int64_t B) {
+  if (!given(t)) return nullptr;
+  check_dense(*t, on, at::kBool, {B}, "active");
+  return reinterpret_cast<const unsigned char*>(t->const_data_ptr());
+}
+
+int to_int(int64_t v, const char* name) {
+  TORCH_CHECK(v >= 0 && v <= 0x7fffffff - 4096, name, ": too large");
+  return static_cast<int>(v);
+}
+
+// ---- causal convolution ------------------------------------------------------------------------------
+BdhConvDesc conv_desc(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
+                      bool silu) {
+  const int64_t B = x.size(0), T = x.size(1), C = x.size(2), k = w.size(1);
+  BdhConvDesc d{};
+  d.dtype = elem_type(x, "x");
+  check_rows(x, x, x.scalar_type(), {B, T, C}, "x");
+  check_dense(w, x, at::kFloat, {C, k}, "w");
+  check_f32(bias, x, {C}, "bias");
+  d.x = x.const_data_ptr(); d.x_sb = x.stride(0); d.x_st = x.stride(1);
+  d.w = w.const_data_ptr<float>(); d.bias = f32_ptr(bias);
+  if (given(state)) {
+    check_rows(*state, x, x.scalar_type(), {B, k - 1, C}, "state");
+    d.state = state->const_data_ptr(); d.state_sb = state->stride(0); d.state_sr = state->stride(1);
+  }
+  set_lengths(lengths, x, B, d.lengths, d.lengths64);
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.C = to_int(C, "C"); d.k = to_int(k, "k");
+  d.silu = silu;
+  return d;
+}
+
+void set_state_out(BdhConvDesc& d, const Tensor& x, const Tensor& out) {
+  check_rows(out, x, x.scalar_type(), {x.size(0), d.k - 1, x.size(2)}, "state_out");
+  d.state_out = out.data_ptr(); d.state_out_sb = out.stride(0); d.state_out_sr = out.stride(1);
+}
+
+void causal_conv_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
+                     bool silu, Tensor& y, Tensor& state_out) {
+  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.dim() == 3 && w.dim() == 2, "x: [B, T, C], w: [C, k]");
+  BdhConvDesc d = conv_desc(x, w, bias, state, lengths, silu);
+  check_dense(y, x, x.scalar_type(), x.sizes(), "y");
+  d.y = y.data_ptr();
+  set_state_out(d, x, state_out);
+  check_rc(bdh_causal_conv_fwd(&d, cur_stream()), "causal_conv_fwd");
+}
+
+int64_t causal_conv_partials(int64_t B, int64_t T, int64_t C, int64_t k) {
+  BdhConvDesc d{};
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.C = to_int(C, "C"); d.k = to_int(k, "k");
+  return bdh_causal_conv_partials(&d);
+}
+
+void causal_conv_bwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
+                     bool silu, const Tensor& dy, const OptTensor& dstate_out, Tensor& dx, const OptTensor& dstate,
+                     const OptTensor& dw, const OptTensor& db, const OptTensor& partial) {
+  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.dim() == 3 && w.dim() == 2, "x: [B, T, C], w: [C, k]");
+  BdhConvDesc d = conv_desc(x, w, bias, state, lengths, silu);
+  const int64_t B = x.size(0), C = x.size(2);
+  check_rows(dy, x, x.scalar_type(), x.sizes(), "dy");
+  d.dy = dy.const_data_ptr(); d.dy_sb = dy.stride(0); d.dy_st = dy.stride(1);
+  check_dense(dx, x, x.scalar_type(), x.sizes(), "dx");
+  d.dx = dx.data_ptr();
+  if (given(dstate_out)) {
+    check_dense(*dstate_out, x, x.scalar_type(), {B, d.k - 1, C}, "dstate_out");
+    d.dstate_out = dstate_out->const_data_ptr();
+  }
+  if (given(dstate)) {
+    check_dense(*dstate, x, x.scalar_type(), {B, d.k - 1, C}, "dstate");
+    d.dstate = dstate->data_ptr();
+  }
+  check_f32(dw, x, {C, d.k}, "dw");
+  check_f32(db, x, {C}, "db");
+  if (given(dw) || given(db)) {
+    TORCH_CHECK(given(partial), "partial: needed for dw and db");
+    check_f32(partial, x, {partial->size(0)}, "partial");
+    TORCH_CHECK(partial->size(0) >= bdh_causal_conv_partials(&d), "partial: too small");
+  }
+  check_rc(bdh_causal_conv_bwd(&d, f32_out(dw), f32_out(db), f32_out(partial), cur_stream()), "causal_conv_bwd");
+}
+
+void causal_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, const OptTensor& bias, const OptTensor& active, bool silu,
+                      Tensor& y, Tensor& state_out) {
+  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [B, C], w: [C, k]");
+  BdhConvDesc d = conv_desc(x.unsqueeze(1), w, bias, state, c10::nullopt, silu);
+  check_dense(y, x, x.scalar_type(), x.sizes(), "y");
+  d.y = y.data_ptr();
+  set_state_out(d, x.unsqueeze(1), state_out);
+  check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(bdh, m) {
+  m.def("causal_conv_fwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor(a!) y, "
+        "Tensor(b!) state_out) -> ()");
+  m.def("causal_conv_partials(int B, int T, int C, int k) -> int");
+  m.def("causal_conv_bwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor dy, "
+        "Tensor? dstate_out, Tensor(a!) dx, Tensor(b!)? dstate, Tensor(c!)? dw, Tensor(d!)? db, Tensor(e!)? partial) -> ()");
+  m.def("causal_conv_step(Tensor x, Tensor state, Tensor w, Tensor? bias, Tensor? active, bool silu, Tensor(a!) y, "
+        "Tensor(b!) state_out) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
+  m.impl("causal_conv_fwd", &causal_conv_fwd);
+  m.impl("causal_conv_bwd", &causal_conv_bwd);
+  m.impl("causal_conv_step", &causal_conv_step);
+}
+TORCH_LIBRARY_IMPL(bdh, CompositeExplicitAutograd, m) {
+  m.impl("causal_conv_partials", &causal_conv_partials);
+}

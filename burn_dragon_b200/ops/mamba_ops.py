@@ -2,15 +2,20 @@
 gated RMSNorm behind. On a GPU both run as one fp32 kernel per direction (`csrc/mamba_ops.cu`) with their
 backward passes written out; elsewhere the torch statement of the same function runs under autograd.
 The reference has no Mamba path; these serve the Mamba-2 model family of this package (models/mamba.py).
+
+`causal_conv` / `causal_conv_step` are the convolution in its general form: fp32, fp16 or bf16 rows, which may be a
+view into a wider projection; a carried state in and out; padded batches; and a form for single tokens
+(`csrc/causal_conv.cu`).
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 
 from . import native
+from . import seqargs as A
 
 
 def _on_kernels(*ts) -> bool:
@@ -52,6 +57,124 @@ def conv1d_silu(seq: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor]
     if _on_kernels(seq, w, bias) and w.shape[1] <= 8:
         return _ConvSilu.apply(seq, w, bias)
     return conv1d_silu_reference(seq, w, bias)
+
+
+# ---- causal convolution with a carried state -----------------------------------------------------------
+def causal_conv_reference(x, w, bias=None, state=None, lengths=None, activation: Optional[str] = "silu"):
+    """Torch statement of `causal_conv` (any device and floating type, differentiable)."""
+    B, T, C = x.shape
+    k = w.shape[1]
+    ct = torch.promote_types(x.dtype, torch.float32)
+    keep = A.valid_rows(lengths, B, T, x.device)
+    xs = x.to(ct) if keep is None else torch.where(keep[..., None], x.to(ct), 0.0)
+    head = state.to(ct) if state is not None else xs.new_zeros(B, k - 1, C)
+    seq = torch.cat((head, xs), dim=1)                                         # [B, T + k - 1, C]
+    pre = sum(seq[:, j:j + T] * w[:, j].to(ct) for j in range(k))
+    if bias is not None:
+        pre = pre + bias.to(ct)
+    y = F.silu(pre) if activation == "silu" else pre
+    if keep is None:
+        return y.to(x.dtype), seq[:, T:].to(x.dtype)
+    rows = lengths.clamp(0, T).long()[:, None] + torch.arange(k - 1, device=x.device)
+    tail = torch.gather(seq, 1, rows[..., None].expand(-1, -1, C))
+    return torch.where(keep[..., None], y, 0.0).to(x.dtype), tail.to(x.dtype)
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, state, lengths, silu):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, w, bias, state, lengths)
+        ctx.silu = silu
+        return _causal_conv_fwd(x, w, bias, state, lengths, silu)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dtail):
+        x, w, bias, state, lengths = ctx.saved_tensors
+        if dy is None and dtail is None:
+            return (None,) * 6
+        B, T, C = x.shape
+        k = w.shape[1]
+        dy = A.adjacent(dy) if dy is not None else torch.zeros_like(x)
+        dtail = dtail.contiguous() if dtail is not None else None
+        need = ctx.needs_input_grad
+        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
+        dw = torch.empty_like(w) if need[1] else None
+        db = torch.empty_like(bias) if bias is not None and need[2] else None
+        dstate = torch.empty(B, k - 1, C, device=x.device, dtype=x.dtype) if state is not None and need[3] else None
+        if B * T == 0:                                                         # no rows: the state went through unchanged
+            zero = lambda t: t.zero_() if t is not None else None
+            return dx, zero(dw), zero(db), dtail if dstate is not None and dtail is not None else zero(dstate), None, None
+        part = None
+        if dw is not None or db is not None:
+            part = torch.empty(native.ops.causal_conv_partials(B, T, C, k), device=x.device, dtype=torch.float32)
+        native.ops.causal_conv_bwd(x, w, bias, state, lengths, ctx.silu, dy, dtail, dx, dstate, dw, db, part)
+        return dx, dw, db, dstate, None, None
+
+
+def _causal_conv_fwd(x, w, bias, state, lengths, silu):
+    B, T, C = x.shape
+    y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
+    tail = torch.empty(B, w.shape[1] - 1, C, device=x.device, dtype=x.dtype)
+    native.ops.causal_conv_fwd(x, w, bias, state, lengths, silu, y, tail)
+    return y, tail
+
+
+def _check_conv(x, w, bias, activation, dims: int) -> bool:
+    A.require(x.dim() == dims and x.is_floating_point(), f"x: expected a floating tensor of {dims} dimensions, got {x.dtype} {tuple(x.shape)}")
+    C = x.shape[-1]
+    A.require(w.dim() == 2 and w.shape[0] == C and 1 <= w.shape[1] <= 8,
+              f"w: expected [{C}, k] with k in 1..8, got {tuple(w.shape)}")
+    A.require(C >= 1, "x: expected at least one channel")
+    A.check_like(w, x, w.shape, "w")
+    A.check_like(bias, x, (C,), "bias")
+    A.require(activation in (None, "silu"), f"activation: expected None or 'silu', got {activation!r}")
+    return activation == "silu"
+
+
+def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, state: Optional[torch.Tensor] = None,
+                lengths: Optional[torch.Tensor] = None, activation: Optional[str] = "silu") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Causal depthwise convolution of x [B, T, C] with w [C, k] (k <= 8), bias [C]: with s = [state | x],
+    y_t = act(bias + sum_j w[:, j] s_{t+j}). Returns (y [B, T, C], state' [B, k-1, C]): the last k - 1 rows of s, to be
+    passed as `state` with the sequence's next rows (None: zeros). Rows are fp32, fp16 or bf16 (y and the states are of
+    their type), sums fp32; x and the state may be views whose channels are adjacent. `lengths` [B]: the rows of each sequence that
+    count; y is 0 behind them, the state ends there, and whatever x holds there is not read. Differentiable in x, w,
+    bias and both states; the sums over rows are made in a fixed order."""
+    silu = _check_conv(x, w, bias, activation, 3)
+    B, T, C = x.shape
+    A.check_like(state, x, (B, w.shape[1] - 1, C), "state", x.dtype)
+    lengths = A.check_lengths(lengths, x, B)
+    if not A.on_kernels(x):
+        return causal_conv_reference(x, w, bias, state, lengths, activation)
+    args = (A.adjacent(x), A.dense_f32(w), A.dense_f32(bias), A.adjacent(state), lengths, silu)
+    return _CausalConv.apply(*args) if A.wants_grad(x, w, bias, state) else _causal_conv_fwd(*args)
+
+
+def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                     activation: Optional[str] = "silu", active: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`causal_conv` for one row of every stream: x [B, C], state [B, k-1, C] -> (y [B, C], state'). The state is left
+    as it was unless `out=state` asks for the update in place (`out`: where state' goes). `active` [B] (bool): a stream
+    marked false gives y = 0 and keeps its state. No gradients (a decoding form)."""
+    silu = _check_conv(x, w, bias, activation, 2)
+    B, C = x.shape
+    k = w.shape[1]
+    A.check_like(state, x, (B, k - 1, C), "state", x.dtype)
+    active = A.check_active(active, x, B)
+    A.check_out(out, state, "out")
+    A.require(not A.wants_grad(x, state, w, bias), "causal_conv_step has no gradient: call it under torch.no_grad(), or use causal_conv")
+    if not A.on_kernels(x):
+        y, new = causal_conv_reference(x.unsqueeze(1), w, bias, state, None, activation)
+        y = y[:, 0]
+        if active is not None:
+            y, new = torch.where(active[:, None], y, 0.0), torch.where(active[:, None, None], new, state)
+        return y, (new if out is None else out.copy_(new))
+    A.require(out is None or C == 1 or out.stride(-1) == 1, "out: its channels must be adjacent")
+    y = torch.empty(B, C, device=x.device, dtype=x.dtype)
+    new = torch.empty(B, k - 1, C, device=x.device, dtype=x.dtype) if out is None else out
+    native.ops.causal_conv_step(A.adjacent(x), A.adjacent(state), A.dense_f32(w), A.dense_f32(bias), active, silu, y, new)
+    return y, new
 
 
 # ---- gated RMSNorm -----------------------------------------------------------------------------------

@@ -1,0 +1,90 @@
+"""Argument checks shared by the operators over padded sequences (`mamba_ops.causal_conv`, `norm_rotate`, `selective_scan`)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import native
+
+KERNEL_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def on_kernels(t: torch.Tensor) -> bool:
+    """Do calls with this tensor run on the CUDA kernels? (float64 and CPU tensors take the torch statement.)"""
+    return t.is_cuda and t.dtype in KERNEL_TYPES and native.load()
+
+
+def check_like(t: Optional[torch.Tensor], ref: torch.Tensor, shape: tuple, name: str, dtype: Optional[torch.dtype] = None) -> None:
+    """`t` (or None) has this shape, is on the device of `ref`, and is of `dtype` (None: any floating type)."""
+    if t is None:
+        return
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
+    if t.dtype != dtype if dtype is not None else not t.is_floating_point():
+        raise ValueError(f"{name}: expected {dtype if dtype is not None else 'a floating type'}, got {t.dtype}")
+
+
+def check_lengths(lengths: Optional[torch.Tensor], ref: torch.Tensor, B: int) -> Optional[torch.Tensor]:
+    """int32 / int64 [B] on the device of `ref`, contiguous. Values are not read here (that would wait for the device);
+    every path takes a value outside [0, T] as the nearer of the two."""
+    if lengths is None:
+        return None
+    if lengths.shape != (B,):
+        raise ValueError(f"lengths: expected shape {(B,)}, got {tuple(lengths.shape)}")
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"lengths: expected int32 or int64, got {lengths.dtype}")
+    if lengths.device != ref.device:
+        raise ValueError(f"lengths is on {lengths.device}, expected {ref.device}")
+    return lengths.contiguous()
+
+
+def check_active(active: Optional[torch.Tensor], ref: torch.Tensor, B: int) -> Optional[torch.Tensor]:
+    if active is None:
+        return None
+    check_like(active, ref, (B,), "active", torch.bool)
+    return active.contiguous()
+
+
+def valid_rows(lengths: Optional[torch.Tensor], B: int, T: int, device) -> Optional[torch.Tensor]:
+    """[B, T] truth values, or None where every row counts."""
+    if lengths is None:
+        return None
+    return torch.arange(T, device=device) < lengths.clamp(0, T)[:, None]
+
+
+def adjacent(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The tensor with elements of its last dimension adjacent (a copy only where they are not)."""
+    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def dense_f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A parameter as the kernels read it."""
+    return None if t is None else t.float().contiguous()
+
+
+def wants_grad(*ts: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None:
+    """`out` of a single-token step: shaped like the state, which it may be; memory it shares with the state otherwise would
+    be overwritten before it is read."""
+    if out is None:
+        return
+    check_like(out, src, src.shape, name, src.dtype)
+    require(not (torch.is_grad_enabled() and out.requires_grad), f"{name} requires a gradient; a step form has none")
+    same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
+    require(all(st > 0 or n <= 1 for st, n in zip(out.stride(), out.shape)), f"{name}: its rows overlap one another")
+    if not same and out.numel():
+        span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
+        (a0, a1), (b0, b1) = span(out), span(src)
+        require(a1 <= b0 or b1 <= a0 or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr(),
+                f"{name} overlaps the state without being it")
