@@ -307,6 +307,44 @@ int bdh_causal_conv_bwd(const BdhConvDesc* d, float* dw, float* db, float* parti
 // byte is 0 gives y = 0 and keeps its state.
 int bdh_causal_conv_step(const BdhConvDesc* d, const unsigned char* active, cudaStream_t s);
 
+// RMS norm of every head of q and k, then the rotation of its channel pairs (2i, 2i + 1), i < P (norm_rotate.cu):
+// v = x / sqrt(mean x^2 + eps) * w + b; (o0, o1) = (v0 cos - v1 sin, v1 cos + v0 sin). q, k: strides in elements of the
+// batch, a token and a head; q_out, k_out and the backward tensors: contiguous [B, T, heads, Dh]. Weights and biases
+// fp32 [Dh], or [heads, Dh] with per_head (null: ones, zeros). Angles: `angles` (radians, P adjacent), or
+// 2 pi frac(position * freqs[2 i]), position = positions[b, t] (int32 / int64; null: pos0 + t). lengths as above:
+// rows behind a length give 0 and take no part in any gradient.
+typedef struct {
+  const void* q;
+  const void* k;              // or null with Hk = 0
+  long long q_sb, q_st, q_sh, k_sb, k_st, k_sh;
+  const float *q_weight, *k_weight, *q_bias, *k_bias;
+  int per_head;
+  const float* angles;
+  long long ang_sb, ang_st;
+  const float* freqs;         // [2 P], cycles per position; the two channels of a pair alike
+  const void* positions;
+  int positions64;
+  long long pos_sb, pos_st, pos0;
+  const void* lengths;
+  int lengths64;
+  int B, T, Hq, Hk, Dh, P;    // Dh even, <= 512
+  int dtype;
+  float eps;
+  void* q_out;
+  void* k_out;
+  const void* dq_out;         // backward only, from here on
+  const void* dk_out;
+  void* dq;
+  void* dk;
+} BdhNormRotateDesc;
+
+int bdh_norm_rotate_fwd(const BdhNormRotateDesc* d, cudaStream_t s);
+// fp32 scratch of the backward pass
+long long bdh_norm_rotate_scratch(const BdhNormRotateDesc* d, int want_weight, int want_bias, int want_angles);
+// The fp32 gradients (any may be null; shaped like the weights, biases and [B, T, P]) are written, not added to.
+int bdh_norm_rotate_bwd(const BdhNormRotateDesc* d, float* dq_weight, float* dk_weight, float* dq_bias, float* dk_bias,
+                        float* dangles, float* scratch, cudaStream_t s);
+
 // Checked build (-DBDH_DEBUG_BOUNDS; csrc/debug_bounds.cuh): the first data-dependent index that was
 // out of range in the kernels of rowwise.cu / graph.cu. out5 = {checked build?, site, index, extent, where}.
 int bdh_bounds_record_rowwise(long long* out5, int clear);

@@ -153,6 +153,118 @@ void causal_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, con
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
 }
 
+// ---- per-head norm + rotation ------------------------------------------------------------------------
+BdhNormRotateDesc norm_desc(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                            const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
+                            const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
+  TORCH_CHECK(q.dim() == 4, "q: [B, T, heads, Dh]");
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), Dh = q.size(3);
+  BdhNormRotateDesc d{};
+  d.dtype = elem_type(q, "q");
+  check_rows(q, q, q.scalar_type(), q.sizes(), "q");
+  d.q = q.const_data_ptr(); d.q_sb = q.stride(0); d.q_st = q.stride(1); d.q_sh = q.stride(2);
+  int64_t Hk = 0;
+  if (given(k)) {
+    TORCH_CHECK(k->dim() == 4, "k: [B, T, heads, Dh]");
+    Hk = k->size(2);
+    check_rows(*k, q, q.scalar_type(), {B, T, Hk, Dh}, "k");
+    d.k = k->const_data_ptr(); d.k_sb = k->stride(0); d.k_st = k->stride(1); d.k_sh = k->stride(2);
+  }
+  for (const OptTensor* w : {&q_weight, &k_weight, &q_bias, &k_bias})
+    if (given(*w) && (*w)->dim() == 2) d.per_head = 1;
+  const auto check_param = [&](const OptTensor& t, int64_t heads, const char* name) {
+    if (d.per_head) check_f32(t, q, {heads, Dh}, name);
+    else check_f32(t, q, {Dh}, name);
+    return f32_ptr(t);
+  };
+  d.q_weight = check_param(q_weight, Hq, "q_weight"); d.q_bias = check_param(q_bias, Hq, "q_bias");
+  d.k_weight = check_param(k_weight, Hk, "k_weight"); d.k_bias = check_param(k_bias, Hk, "k_bias");
+  int64_t P = 0;
+  if (given(angles)) {
+    TORCH_CHECK(angles->dim() == 3, "angles: [B, T, pairs]");
+    P = angles->size(2);
+    check_rows(*angles, q, at::kFloat, {B, T, P}, "angles");
+    d.angles = angles->const_data_ptr<float>(); d.ang_sb = angles->stride(0); d.ang_st = angles->stride(1);
+  } else if (given(freqs)) {
+    TORCH_CHECK(freqs->dim() == 1 && freqs->size(0) % 2 == 0, "freqs: [2 * pairs]");
+    check_dense(*freqs, q, at::kFloat, freqs->sizes(), "freqs");
+    P = freqs->size(0) / 2;
+    d.freqs = freqs->const_data_ptr<float>();
+  }
+  TORCH_CHECK(2 * P <= Dh, "more rotated channels than a head has");
+  d.pos0 = pos0;
+  if (given(positions)) {
+    TORCH_CHECK(positions->is_cuda() && positions->device() == q.device() && positions->dim() == 2 && positions->size(0) == B &&
+                positions->size(1) == T && (positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong),
+                "positions: expected int32 or int64 [B, T] on ", q.device());
+    d.positions = positions->const_data_ptr(); d.positions64 = positions->scalar_type() == at::kLong;
+    d.pos_sb = positions->stride(0); d.pos_st = positions->stride(1);
+  }
+  set_lengths(lengths, q, B, d.lengths, d.lengths64);
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.Hq = to_int(Hq, "heads"); d.Hk = to_int(Hk, "heads"); d.Dh = to_int(Dh, "Dh");
+  d.P = static_cast<int>(P);
+  d.eps = static_cast<float>(eps);
+  return d;
+}
+
+void norm_rotate_fwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& q_bias,
+                     const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs, const OptTensor& positions,
+                     int64_t pos0, const OptTensor& lengths, double eps, Tensor& q_out, const OptTensor& k_out) {
+  c10::cuda::CUDAGuard guard(q.device());
+  BdhNormRotateDesc d = norm_desc(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+  check_dense(q_out, q, q.scalar_type(), q.sizes(), "q_out");
+  d.q_out = q_out.data_ptr();
+  if (given(k)) {
+    TORCH_CHECK(given(k_out), "k_out: needed");
+    check_dense(*k_out, q, q.scalar_type(), k->sizes(), "k_out");
+    d.k_out = k_out->data_ptr();
+  }
+  check_rc(bdh_norm_rotate_fwd(&d, cur_stream()), "norm_rotate_fwd");
+}
+
+int64_t norm_rotate_scratch(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t Dh, int64_t P, bool per_head, bool want_weight,
+                            bool want_bias, bool want_angles) {
+  BdhNormRotateDesc d{};
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.Hq = to_int(Hq, "heads"); d.Hk = to_int(Hk, "heads"); d.Dh = to_int(Dh, "Dh");
+  d.P = to_int(P, "pairs"); d.per_head = per_head;
+  return bdh_norm_rotate_scratch(&d, want_weight, want_bias, want_angles);
+}
+
+void norm_rotate_bwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& q_bias,
+                     const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs, const OptTensor& positions,
+                     int64_t pos0, const OptTensor& lengths, double eps, const Tensor& dq_out, const OptTensor& dk_out, Tensor& dq,
+                     const OptTensor& dk, const OptTensor& dq_weight, const OptTensor& dk_weight, const OptTensor& dq_bias,
+                     const OptTensor& dk_bias, const OptTensor& dangles, const OptTensor& scratch) {
+  c10::cuda::CUDAGuard guard(q.device());
+  BdhNormRotateDesc d = norm_desc(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+  const auto type = q.scalar_type();
+  check_dense(dq_out, q, type, q.sizes(), "dq_out");
+  check_dense(dq, q, type, q.sizes(), "dq");
+  d.dq_out = dq_out.const_data_ptr(); d.dq = dq.data_ptr();
+  if (given(k)) {
+    TORCH_CHECK(given(dk_out) && given(dk), "dk_out, dk: needed");
+    check_dense(*dk_out, q, type, k->sizes(), "dk_out");
+    check_dense(*dk, q, type, k->sizes(), "dk");
+    d.dk_out = dk_out->const_data_ptr(); d.dk = dk->data_ptr();
+  }
+  const auto check_grad = [&](const OptTensor& t, int64_t heads, const char* name) {
+    if (d.per_head) check_f32(t, q, {heads, d.Dh}, name);
+    else check_f32(t, q, {d.Dh}, name);
+    return f32_out(t);
+  };
+  float* gqw = check_grad(dq_weight, d.Hq, "dq_weight");
+  float* gkw = check_grad(dk_weight, d.Hk, "dk_weight");
+  float* gqb = check_grad(dq_bias, d.Hq, "dq_bias");
+  float* gkb = check_grad(dk_bias, d.Hk, "dk_bias");
+  check_f32(dangles, q, {d.B, d.T, d.P}, "dangles");
+  const long long need = bdh_norm_rotate_scratch(&d, gqw || gkw || gqb || gkb, gqb || gkb, given(dangles));
+  if (need > 0) {
+    TORCH_CHECK(given(scratch) && scratch->numel() >= need, "scratch: too small");
+    check_f32(scratch, q, {scratch->numel()}, "scratch");
+  }
+  check_rc(bdh_norm_rotate_bwd(&d, gqw, gkw, gqb, gkb, f32_out(dangles), f32_out(scratch), cur_stream()), "norm_rotate_bwd");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(bdh, m) {
@@ -163,13 +275,24 @@ TORCH_LIBRARY_FRAGMENT(bdh, m) {
         "Tensor? dstate_out, Tensor(a!) dx, Tensor(b!)? dstate, Tensor(c!)? dw, Tensor(d!)? db, Tensor(e!)? partial) -> ()");
   m.def("causal_conv_step(Tensor x, Tensor state, Tensor w, Tensor? bias, Tensor? active, bool silu, Tensor(a!) y, "
         "Tensor(b!) state_out) -> ()");
+  m.def("norm_rotate_fwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
+        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor(a!) q_out, Tensor(b!)? k_out) -> ()");
+  m.def("norm_rotate_scratch(int B, int T, int Hq, int Hk, int Dh, int P, bool per_head, bool want_weight, bool want_bias, "
+        "bool want_angles) -> int");
+  m.def("norm_rotate_bwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
+        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor dq_out, Tensor? dk_out, Tensor(a!) dq, "
+        "Tensor(b!)? dk, Tensor(c!)? dq_weight, Tensor(d!)? dk_weight, Tensor(e!)? dq_bias, Tensor(f!)? dk_bias, "
+        "Tensor(g!)? dangles, Tensor(h!)? scratch) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
+  m.impl("norm_rotate_fwd", &norm_rotate_fwd);
+  m.impl("norm_rotate_bwd", &norm_rotate_bwd);
   m.impl("causal_conv_fwd", &causal_conv_fwd);
   m.impl("causal_conv_bwd", &causal_conv_bwd);
   m.impl("causal_conv_step", &causal_conv_step);
 }
 TORCH_LIBRARY_IMPL(bdh, CompositeExplicitAutograd, m) {
   m.impl("causal_conv_partials", &causal_conv_partials);
+  m.impl("norm_rotate_scratch", &norm_rotate_scratch);
 }

@@ -1,0 +1,152 @@
+"""RMS norm of every query and key head together with its rotation, in one pass (`csrc/norm_rotate.cu`).
+
+    v = x / sqrt(mean x^2 + eps) * weight + bias          over the Dh channels of a head
+    (o_2i, o_2i+1) = (v_2i cos - v_2i+1 sin, v_2i+1 cos + v_2i sin)     for the first pairs; the other channels stay
+
+The angle of a pair comes from the token's position, 2 pi frac(position * freq) with `freqs` as
+`reference.build_freqs(..., "rope")` makes them, or is given for every token (the cumulative, learned angles of a
+state-space layer whose C and B are the queries and keys). Gradients: q, k, weights, biases, angles.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import native
+from . import seqargs as A
+
+
+def _turn(v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    n = 2 * cos.shape[-1]
+    a, b = v[..., 0:n:2], v[..., 1:n:2]
+    return torch.cat((torch.stack((a * cos - b * sin, b * cos + a * sin), -1).flatten(-2), v[..., n:]), -1)
+
+
+def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, k_bias=None, *, angles=None, freqs=None, positions=0,
+                          lengths=None, eps: float = 1e-5):
+    """Torch statement of `norm_rotate` (any device and floating type, differentiable)."""
+    B, T = q.shape[:2]
+    ct = torch.promote_types(q.dtype, torch.float32)
+    if angles is None and freqs is not None:
+        pos = positions if isinstance(positions, torch.Tensor) else positions + torch.arange(T, device=q.device)
+        turns = pos.double()[..., None] * freqs[0::2].double()
+        angles = (turns - turns.floor()) * (2 * math.pi)
+        angles = angles.expand(B, T, -1)
+    keep = A.valid_rows(lengths, B, T, q.device)
+    keep = keep[..., None, None] if keep is not None else None
+    outs = []
+    for x, w, b in ((q, q_weight, q_bias), (k, k_weight, k_bias)):
+        if x is None:
+            outs.append(None)
+            continue
+        xs = x.to(ct) if keep is None else torch.where(keep, x.to(ct), 0.0)
+        v = xs * torch.rsqrt(xs.square().mean(-1, keepdim=True) + eps)
+        v = v * w.to(ct) if w is not None else v
+        v = v + b.to(ct) if b is not None else v
+        if angles is not None:
+            an = angles if keep is None else torch.where(keep[..., 0], angles, 0.0)
+            v = _turn(v, an.cos().to(ct)[:, :, None], an.sin().to(ct)[:, :, None])
+        outs.append((v if keep is None else torch.where(keep, v, 0.0)).to(x.dtype))
+    return tuple(outs)
+
+
+def _forward(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps):
+    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    ko = torch.empty(k.shape, device=q.device, dtype=q.dtype) if k is not None else None
+    native.ops.norm_rotate_fwd(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps, qo, ko)
+    return qo, ko
+
+
+class _NormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, qw, kw, qb, kb, angles, freqs, positions, lengths)
+        ctx.pos0, ctx.eps = pos0, eps
+        return _forward(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dqo, dko):
+        q, k, qw, kw, qb, kb, angles, freqs, positions, lengths = ctx.saved_tensors
+        if dqo is None and dko is None:
+            return (None,) * 12
+        need = ctx.needs_input_grad
+        like = lambda t, want: torch.empty_like(t) if t is not None and want else None                    # noqa: E731
+        gqw, gkw, gqb, gkb = (like(t, w) for t, w in zip((qw, kw, qb, kb), need[2:6]))
+        gan = torch.empty(angles.shape, device=q.device, dtype=torch.float32) if angles is not None and need[6] else None
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if k is not None else None
+        B, T, Hq, Dh = q.shape
+        if B * T == 0:
+            for t in (gqw, gkw, gqb, gkb):
+                if t is not None:
+                    t.zero_()
+            return dq, dk, gqw, gkw, gqb, gkb, gan, None, None, None, None, None
+        dqo = dqo.contiguous() if dqo is not None else torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+        if k is not None:
+            dko = dko.contiguous() if dko is not None else torch.zeros(k.shape, device=q.device, dtype=q.dtype)
+        bias = gqb is not None or gkb is not None
+        weight = bias or gqw is not None or gkw is not None
+        P = angles.shape[-1] if angles is not None else freqs.shape[0] // 2 if freqs is not None else 0
+        per_head = any(t is not None and t.dim() == 2 for t in (qw, kw, qb, kb))
+        n = native.ops.norm_rotate_scratch(B, T, Hq, k.shape[2] if k is not None else 0, Dh, P, per_head, weight, bias, gan is not None)
+        scratch = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+        native.ops.norm_rotate_bwd(q, k, qw, kw, qb, kb, angles, freqs, positions, ctx.pos0, lengths, ctx.eps, dqo, dko, dq, dk,
+                                   gqw, gkw, gqb, gkb, gan, scratch)
+        return dq, dk, gqw, gkw, gqb, gkb, gan, None, None, None, None, None
+
+
+def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                k_weight: Optional[torch.Tensor] = None, q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, *,
+                angles: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
+                positions: Union[int, torch.Tensor] = 0, lengths: Optional[torch.Tensor] = None,
+                eps: float = 1e-5) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """RMS norm and rotation of q [B, T, Hq, Dh] and k [B, T, Hk, Dh] (or None): -> (q', k'), contiguous, in their type.
+    Rows are fp32, fp16 or bf16 and may be views into a wider projection (channels adjacent); Dh is even and at most
+    512. Weights and biases: [Dh] for all heads or [heads, Dh], all of them alike (None: 1 and 0).
+    Rotation, if any: `angles` [B, T, pairs] in radians, or `freqs` [2 * pairs] in cycles per position with `positions`
+    - the first token's (an int), or [T] or [B, T] integers (the single-token form has T = 1 and one position a stream).
+    `lengths` [B]: rows behind a sequence's length give 0 and take no part in any gradient."""
+    A.require(q.dim() == 4 and q.is_floating_point(), f"q: expected a floating [B, T, heads, Dh] tensor, got {q.dtype} {tuple(q.shape)}")
+    B, T, Hq, Dh = q.shape
+    A.require(Hq >= 1 and Dh >= 2 and Dh % 2 == 0 and Dh <= 512, f"q: expected at least one head and an even Dh up to 512, got {tuple(q.shape)}")
+    A.require(k is None or (k.dim() == 4 and k.shape[2] >= 1), "k: expected [B, T, heads, Dh]")
+    Hk = k.shape[2] if k is not None else 0
+    A.check_like(k, q, (B, T, Hk, Dh), "k", q.dtype)
+    A.require(k is not None or (k_weight is None and k_bias is None), "k_weight and k_bias come with k")
+    params = ((q_weight, Hq, "q_weight"), (k_weight, Hk, "k_weight"), (q_bias, Hq, "q_bias"), (k_bias, Hk, "k_bias"))
+    per_head = any(t is not None and t.dim() == 2 for t, _, _ in params)
+    for t, H, name in params:
+        A.check_like(t, q, (H, Dh) if per_head else (Dh,), name)
+    A.require(angles is None or freqs is None, "angles and freqs: one of the two at most")
+    pos0 = 0
+    if angles is not None:
+        A.require(angles.dim() == 3 and 2 * angles.shape[2] <= Dh, f"angles: expected [B, T, pairs] with pairs up to {Dh // 2}, got {tuple(angles.shape)}")
+        A.check_like(angles, q, (B, T, angles.shape[2]), "angles")
+        A.require(isinstance(positions, int) and positions == 0, "positions come with freqs")
+    elif freqs is not None:
+        A.require(freqs.dim() == 1 and freqs.shape[0] % 2 == 0 and freqs.shape[0] <= Dh, f"freqs: expected an even number up to {Dh}, got {tuple(freqs.shape)}")
+        A.check_like(freqs, q, freqs.shape, "freqs")
+        A.require(not A.wants_grad(freqs), "freqs has no gradient; pass angles")
+        if isinstance(positions, torch.Tensor):
+            A.require(positions.dtype in (torch.int32, torch.int64), f"positions: expected int32 or int64, got {positions.dtype}")
+            A.require(tuple(positions.shape) in ((T,), (B, T)), f"positions: expected {(T,)} or {(B, T)}, got {tuple(positions.shape)}")
+            A.require(positions.device == q.device, f"positions is on {positions.device}, expected {q.device}")
+        else:
+            pos0 = int(positions)
+    else:
+        A.require(isinstance(positions, int) and positions == 0, "positions come with freqs")
+    lengths = A.check_lengths(lengths, q, B)
+    if not A.on_kernels(q):
+        return norm_rotate_reference(q, k, q_weight, k_weight, q_bias, k_bias, angles=angles, freqs=freqs, positions=positions,
+                                     lengths=lengths, eps=eps)
+    A.require(B * T <= 1 << 30, "more than 2^30 tokens")
+    pos = positions.expand(B, T) if isinstance(positions, torch.Tensor) else None
+    args = (A.adjacent(q), A.adjacent(k), A.dense_f32(q_weight), A.dense_f32(k_weight), A.dense_f32(q_bias), A.dense_f32(k_bias),
+            A.adjacent(angles.float()) if angles is not None else None, A.dense_f32(freqs), pos, pos0, lengths, float(eps))
+    if A.wants_grad(q, k, q_weight, k_weight, q_bias, k_bias, angles):
+        return _NormRotate.apply(*args)
+    return _forward(*args)
