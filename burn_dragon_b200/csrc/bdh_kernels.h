@@ -345,6 +345,46 @@ long long bdh_norm_rotate_scratch(const BdhNormRotateDesc* d, int want_weight, i
 int bdh_norm_rotate_bwd(const BdhNormRotateDesc* d, float* dq_weight, float* dk_weight, float* dq_bias, float* dk_bias,
                         float* dangles, float* scratch, cudaStream_t s);
 
+// Selective scan (selective_scan.cu): dt' = softplus(dt + dt_bias) or dt + dt_bias; h_t = exp(dt'_t A) h_{t-1} + dt'_t u_t B_t;
+// y_t = C_t . h_t + skip u_t, for channels d < D with N <= 64 states each. u, dt, dy [B, T, D] and B, C [B, T, N]: strides
+// in elements of the batch and of a row; A [D, N], dt_bias, skip [D], h0, hT, dhT, dh0 [B, D, N] fp32 contiguous; y, du,
+// ddt contiguous. lengths as above: behind a length the state stays, y and all gradients are 0.
+typedef struct {
+  const void* u;
+  const void* dt;
+  const void* B_;
+  const void* C_;
+  long long u_sb, u_st, dt_sb, dt_st, b_sb, b_st, c_sb, c_st;
+  const float* A;
+  const float* dt_bias;       // or null
+  const float* skip;          // or null
+  const float* h0;            // or null: zeros
+  const void* lengths;
+  int lengths64;
+  int B, T, D, N;
+  int dtype, softplus;
+  void* y;
+  float* hT;
+  const void* dy;             // backward only, from here on
+  long long dy_sb, dy_st;
+  const float* dhT;           // gradient of hT, or null
+  void* du;
+  void* ddt;
+  float* dh0;                 // or null
+} BdhScanDesc;
+
+// fp32 elements: `marks` (states at the tiles' starts: written by a forward pass that a backward pass follows, which
+// reads them) and the scratch of either pass
+void bdh_selective_scan_sizes(const BdhScanDesc* d, long long* marks, long long* fwd_scratch, long long* bwd_scratch);
+int bdh_selective_scan_fwd(const BdhScanDesc* d, float* marks, float* scratch, cudaStream_t s);     // marks may be null
+// dA [D, N], dD, dbias [D] fp32 (dD, dbias may be null); dB, dC [B, T, N] in the rows' type
+int bdh_selective_scan_bwd(const BdhScanDesc* d, const float* marks, float* scratch, float* dA, float* dD, float* dbias,
+                           void* dB, void* dC, cudaStream_t s);
+// One row per sequence: y [B, D]; the new state goes to `out` (rows [D, N] dense, batch strides h_sb, out_sb), which may
+// be h. active as above.
+int bdh_selective_scan_step(const BdhScanDesc* d, const float* h, long long h_sb, float* out, long long out_sb,
+                            const unsigned char* active, cudaStream_t s);
+
 // Checked build (-DBDH_DEBUG_BOUNDS; csrc/debug_bounds.cuh): the first data-dependent index that was
 // out of range in the kernels of rowwise.cu / graph.cu. out5 = {checked build?, site, index, extent, where}.
 int bdh_bounds_record_rowwise(long long* out5, int clear);

@@ -265,6 +265,104 @@ void norm_rotate_bwd(const Tensor& q, const OptTensor& k, const OptTensor& q_wei
   check_rc(bdh_norm_rotate_bwd(&d, gqw, gkw, gqb, gkb, f32_out(dangles), f32_out(scratch), cur_stream()), "norm_rotate_bwd");
 }
 
+// ---- selective scan ----------------------------------------------------------------------------------
+BdhScanDesc scan_desc(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
+                      const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths) {
+  TORCH_CHECK(u.dim() == 3 && A.dim() == 2, "u: [B, T, D], A: [D, N]");
+  const int64_t B = u.size(0), T = u.size(1), D = u.size(2), N = A.size(1);
+  const auto type = u.scalar_type();
+  BdhScanDesc d{};
+  d.dtype = elem_type(u, "u");
+  check_rows(u, u, type, {B, T, D}, "u");
+  check_rows(dt, u, type, {B, T, D}, "dt");
+  check_rows(Bm, u, type, {B, T, N}, "B");
+  check_rows(Cm, u, type, {B, T, N}, "C");
+  check_dense(A, u, at::kFloat, {D, N}, "A");
+  check_f32(skip, u, {D}, "D");
+  check_f32(dt_bias, u, {D}, "dt_bias");
+  check_f32(h0, u, {B, D, N}, "h0");
+  d.u = u.const_data_ptr(); d.u_sb = u.stride(0); d.u_st = u.stride(1);
+  d.dt = dt.const_data_ptr(); d.dt_sb = dt.stride(0); d.dt_st = dt.stride(1);
+  d.B_ = Bm.const_data_ptr(); d.b_sb = Bm.stride(0); d.b_st = Bm.stride(1);
+  d.C_ = Cm.const_data_ptr(); d.c_sb = Cm.stride(0); d.c_st = Cm.stride(1);
+  d.A = A.const_data_ptr<float>(); d.skip = f32_ptr(skip); d.dt_bias = f32_ptr(dt_bias); d.h0 = f32_ptr(h0);
+  set_lengths(lengths, u, B, d.lengths, d.lengths64);
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.D = to_int(D, "D"); d.N = to_int(N, "N");
+  d.softplus = softplus;
+  return d;
+}
+
+std::tuple<int64_t, int64_t, int64_t> selective_scan_sizes(int64_t B, int64_t T, int64_t D, int64_t N) {
+  BdhScanDesc d{};
+  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.D = to_int(D, "D"); d.N = to_int(N, "N");
+  long long marks, fwd, bwd;
+  bdh_selective_scan_sizes(&d, &marks, &fwd, &bwd);
+  return {marks, fwd, bwd};
+}
+
+float* scratch_of(const OptTensor& t, const Tensor& on, long long need, const char* name) {
+  if (need <= 0) return nullptr;
+  TORCH_CHECK(given(t) && t->numel() >= need, name, ": too small");
+  check_f32(t, on, {t->numel()}, name);
+  return t->data_ptr<float>();
+}
+
+void selective_scan_fwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
+                        const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths, Tensor& y, Tensor& hT,
+                        const OptTensor& marks, const OptTensor& scratch) {
+  c10::cuda::CUDAGuard guard(u.device());
+  BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
+  check_dense(y, u, u.scalar_type(), u.sizes(), "y");
+  check_dense(hT, u, at::kFloat, {d.B, d.D, d.N}, "hT");
+  d.y = y.data_ptr(); d.hT = hT.data_ptr<float>();
+  long long n_marks, n_fwd, n_bwd;
+  bdh_selective_scan_sizes(&d, &n_marks, &n_fwd, &n_bwd);
+  float* m = given(marks) ? scratch_of(marks, u, n_marks, "marks") : nullptr;
+  check_rc(bdh_selective_scan_fwd(&d, m, scratch_of(scratch, u, n_fwd, "scratch"), cur_stream()), "selective_scan_fwd");
+}
+
+void selective_scan_bwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
+                        const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths, const Tensor& marks,
+                        const Tensor& scratch, const Tensor& dy, const OptTensor& dhT, Tensor& du, Tensor& ddt, Tensor& dA, Tensor& dB,
+                        Tensor& dC, const OptTensor& dskip, const OptTensor& ddt_bias, const OptTensor& dh0) {
+  c10::cuda::CUDAGuard guard(u.device());
+  BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
+  const auto type = u.scalar_type();
+  check_rows(dy, u, type, u.sizes(), "dy");
+  check_dense(du, u, type, u.sizes(), "du");
+  check_dense(ddt, u, type, u.sizes(), "ddt");
+  check_dense(dA, u, at::kFloat, A.sizes(), "dA");
+  check_dense(dB, u, type, Bm.sizes(), "dB");
+  check_dense(dC, u, type, Cm.sizes(), "dC");
+  check_f32(dskip, u, {d.D}, "dD");
+  check_f32(ddt_bias, u, {d.D}, "ddt_bias");
+  check_f32(dhT, u, {d.B, d.D, d.N}, "dhT");
+  check_f32(dh0, u, {d.B, d.D, d.N}, "dh0");
+  d.dy = dy.const_data_ptr(); d.dy_sb = dy.stride(0); d.dy_st = dy.stride(1);
+  d.du = du.data_ptr(); d.ddt = ddt.data_ptr(); d.dhT = f32_ptr(dhT); d.dh0 = f32_out(dh0);
+  long long n_marks, n_fwd, n_bwd;
+  bdh_selective_scan_sizes(&d, &n_marks, &n_fwd, &n_bwd);
+  const float* m = scratch_of(marks, u, n_marks, "marks");
+  check_rc(bdh_selective_scan_bwd(&d, m, scratch_of(scratch, u, n_bwd, "scratch"), dA.data_ptr<float>(), f32_out(dskip), f32_out(ddt_bias),
+                                  dB.data_ptr(), dC.data_ptr(), cur_stream()), "selective_scan_bwd");
+}
+
+void selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const Tensor& h,
+                         const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& active, Tensor& y, Tensor& out) {
+  c10::cuda::CUDAGuard guard(u.device());
+  TORCH_CHECK(u.dim() == 2 && dt.dim() == 2 && Bm.dim() == 2 && Cm.dim() == 2, "u, dt: [B, D], B, C: [B, N]");
+  BdhScanDesc d = scan_desc(u.unsqueeze(1), dt.unsqueeze(1), A, Bm.unsqueeze(1), Cm.unsqueeze(1), skip, dt_bias, softplus, c10::nullopt,
+                            c10::nullopt);
+  check_dense(y, u, u.scalar_type(), u.sizes(), "y");
+  d.y = y.data_ptr();
+  for (const Tensor* t : {&h, static_cast<const Tensor*>(&out)}) {
+    check_rows(*t, u, at::kFloat, {d.B, d.D, d.N}, "h");
+    TORCH_CHECK(d.D == 1 || t->stride(1) == d.N, "h: expected dense [D, N] states");
+  }
+  check_rc(bdh_selective_scan_step(&d, h.const_data_ptr<float>(), h.stride(0), out.data_ptr<float>(), out.stride(0),
+                                   active_ptr(active, u, d.B), cur_stream()), "selective_scan_step");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(bdh, m) {
@@ -283,9 +381,20 @@ TORCH_LIBRARY_FRAGMENT(bdh, m) {
         "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor dq_out, Tensor? dk_out, Tensor(a!) dq, "
         "Tensor(b!)? dk, Tensor(c!)? dq_weight, Tensor(d!)? dk_weight, Tensor(e!)? dq_bias, Tensor(f!)? dk_bias, "
         "Tensor(g!)? dangles, Tensor(h!)? scratch) -> ()");
+  m.def("selective_scan_sizes(int B, int T, int D, int N) -> (int, int, int)");
+  m.def("selective_scan_fwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
+        "Tensor? lengths, Tensor(a!) y, Tensor(b!) hT, Tensor(c!)? marks, Tensor(d!)? scratch) -> ()");
+  m.def("selective_scan_bwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
+        "Tensor? lengths, Tensor marks, Tensor(a!) scratch, Tensor dy, Tensor? dhT, Tensor(b!) du, Tensor(c!) ddt, Tensor(d!) dA, "
+        "Tensor(e!) dB, Tensor(f!) dC, Tensor(g!)? dD, Tensor(h!)? ddt_bias, Tensor(i!)? dh0) -> ()");
+  m.def("selective_scan_step(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor h, Tensor? D, Tensor? dt_bias, bool softplus, "
+        "Tensor? active, Tensor(a!) y, Tensor(b!) out) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
+  m.impl("selective_scan_fwd", &selective_scan_fwd);
+  m.impl("selective_scan_bwd", &selective_scan_bwd);
+  m.impl("selective_scan_step", &selective_scan_step);
   m.impl("norm_rotate_fwd", &norm_rotate_fwd);
   m.impl("norm_rotate_bwd", &norm_rotate_bwd);
   m.impl("causal_conv_fwd", &causal_conv_fwd);
@@ -295,4 +404,5 @@ TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
 TORCH_LIBRARY_IMPL(bdh, CompositeExplicitAutograd, m) {
   m.impl("causal_conv_partials", &causal_conv_partials);
   m.impl("norm_rotate_scratch", &norm_rotate_scratch);
+  m.impl("selective_scan_sizes", &selective_scan_sizes);
 }
