@@ -1,0 +1,1075 @@
+// Selective scan: a diagonal recurrence with an input-dependent step per channel,
+//
+//   dt' = softplus(dt + bias)  (or dt + bias);   a_tn = exp(dt'_t A_n);   h_tn = a_tn h_{t-1,n} + dt'_t u_t B_tn
+//   y_t = sum_n C_tn h_tn + D u_t
+//   g_tn = C_tn dy_t + r_{t+1,n},  r_tn = a_tn g_tn  (r behind the last step: the gradient of the last state);  q_tn = r_tn h_{t-1,n}
+//   ddt' = sum_n A_n q_n + u sum_n g_n B_n;  du = dt' sum_n g_n B_n + D dy;  dA_n = sum_t dt' q_n;
+//   dB_n = sum_channels g_n dt' u;  dC_n = sum_channels dy h_n;  dD = sum dy u;  dbias = sum ddt
+//
+// for every channel d (u, dt, A[d], D, bias of its own; B_t and C_t shared by all channels). Bound by the exponentials
+// (one per step, channel and state; 16 a clock and SM) and, backward, by the issue of the products around them; the
+// tensors themselves are read and written once.
+//
+// Layout: 4 states a lane, G = NP / 4 lanes a channel (NP: the states padded to 8, 16, 32 or 64), CT channels a lane, so
+// that h stays in registers along time and a warp holds 32 * 4 * CT states. Sums over states go over the G lanes, sums
+// over channels over the 32 / G others, both by halving exchanges (n values over n lanes cost n - 1 shuffles and leave
+// one sum in each lane). Time runs in tiles of 16 steps: a block fetches the next tile into registers while it works on
+// the present one, whose steps (dt', dt' u) and rows of B and C lie in shared memory as fp32.
+// Long sequences with too few channels to fill the GPU are cut into segments: one launch computes every segment's
+// state from zero and its total step, the next starts each segment from the combination of those before it.
+// Backward: the forward pass leaves h at every tile's start; a tile's states are computed again from there into shared
+// memory and walked through in reverse. States, sums and gradients are fp32; sums over channel blocks, segments
+// and sequences are made from partial sums in a fixed order (no atomics: two runs give the same bits).
+#pragma once
+#include "bdh_kernels.h"
+#include "device_once.h"
+#include "element_io.cuh"
+
+#include <type_traits>
+
+namespace bdh {
+namespace {
+
+constexpr int LT = 16;                 // steps per tile
+constexpr int FWD_WARPS = 2;           // independent warps of a block, forward and sweeps
+constexpr int BWD_WARPS = 4;           // warps of a block that add their sums over channels up, backward
+constexpr int STEP_THREADS = 128;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E_LO = 1.925963033500e-08f;      // log2(e) - LOG2E
+constexpr float LN2 = 0.6931471805599453f;
+
+struct ScanArgs {
+  BdhScanDesc d;
+  Lengths len;
+  int tiles, per_seg, segs;            // tiles per sequence, per segment; segments
+  int parts;                           // warps (forward) or blocks (backward) across the channels
+  const float* seg_state;              // [B][segs][D][NP]: states of the segments from zero (forward or reverse)
+  const float* seg_dt;                 // [B][segs][D]: their total steps
+};
+
+// ---- two fp32 operations in one instruction ------------------------------------------------------------
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float x, float y) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ f2 ex2x2(f2 v) {
+  float x, y;
+  unpack2(v, x, y);
+  return pack2(ex2(x), ex2(y));
+}
+__device__ __forceinline__ float sum2(f2 v) {
+  float x, y;
+  unpack2(v, x, y);
+  return x + y;
+}
+__device__ __forceinline__ void load4(const float* p, f2& x, f2& y) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  x = v.x;
+  y = v.y;
+}
+
+// exp(-|x|), to about 2^-22 of itself: the rounding of |x| log2(e) is put back as a factor 1 + its residual ln(2).
+__device__ __forceinline__ f2 exp_minus_abs(f2 x) {
+  float a, b;
+  unpack2(x, a, b);
+  const f2 m = pack2(-fminf(fabsf(a), 120.f), -fminf(fabsf(b), 120.f));
+  const f2 y = mul2(m, both(LOG2E));
+  const f2 lo = fma2(m, both(LOG2E_LO), fma2(m, both(LOG2E), mul2(y, both(-1.f))));
+  const f2 t = ex2x2(y);
+  return fma2(t, mul2(lo, both(LN2)), t);
+}
+
+// softplus(x) = max(x, 0) + log1p(exp(-|x|)) for two steps at once. log1p(t) / t on [0, 1] is the polynomial of degree 9
+// through its values at the Chebyshev nodes: off by at most 5.4e-9 of itself (the nearest singularity, t = -1,
+// makes the error fall by 3 + 2 sqrt(2) a degree), so the result is off by the 32-bit rounding.
+__device__ __forceinline__ f2 softplus2(f2 x) {
+  constexpr float P[10] = {1.0f, -0.49999892711639404f, 0.33329710364341736f, -0.24951615929603577f, 0.1966327428817749f,
+                           -0.1526966691017151f, 0.10543623566627502f, -0.056373611092567444f, 0.019542526453733444f,
+                           -0.0031760570127516985f};
+  const f2 t = exp_minus_abs(x);
+  f2 p = both(P[9]);
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = fma2(p, t, both(P[i]));
+  float a, b, ma, mb;
+  unpack2(x, a, b);
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(ma) : "f"(a));
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(mb) : "f"(b));
+  return fma2(p, t, pack2(ma, mb));
+}
+// its derivative, 1 / (1 + exp(-x))
+__device__ __forceinline__ f2 sigmoid2(f2 x) {
+  float a, b, ta, tb;
+  unpack2(x, a, b);
+  unpack2(exp_minus_abs(x), ta, tb);
+  return pack2(__fdividef(a < 0.f ? ta : 1.f, 1.f + ta), __fdividef(b < 0.f ? tb : 1.f, 1.f + tb));
+}
+
+// Sums of v[0..NV) over the lanes that differ in the bits FIRST .. FIRST * LANES / 2 of the lane number: the number of
+// values halves with every exchange while there is more than one. Leaves max(1, NV / LANES) sums; the first of them is
+// that of value `at`; `once` marks one lane of those that hold the same.
+template <int NV, int LANES, int FIRST>
+__device__ __forceinline__ void sum_over(float (&v)[NV], int lane, int& at, bool& once) {
+  at = 0;
+  once = true;
+  int n = NV;
+#pragma unroll
+  for (int o = LANES * FIRST / 2; o >= FIRST; o >>= 1) {
+    const bool up = lane & o;
+    if (n > 1) {
+      n >>= 1;
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        if (i >= n) break;
+        const float keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+      at += up ? n : 0;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      once = once && !up;
+    }
+  }
+}
+
+// A warp's part of a tile: 16 steps of CW channels; for loading and storing, lane l has the step l / 2 and the first or
+// second half of the channels (and of the states of B and C).
+template <typename T, int G, int CT>
+struct Shape {
+  static constexpr int NP = 4 * G;
+  static constexpr int LANES = 32 / G;                 // channel lanes
+  static constexpr int CW = LANES * CT;                // channels of a warp
+  static constexpr int E = CW / 2;                     // elements of a lane
+  static constexpr int V = E < 16 / static_cast<int>(sizeof(T)) ? E : 16 / static_cast<int>(sizeof(T));
+  static constexpr int NV = E / V;                     // its packs
+  static constexpr int NB = NP / 8;                    // packs of 4 states of B (or C) of a lane
+};
+
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ Pack<T, V> load_row(const T* p, int c, int D) {
+  Pack<T, V> r;
+  if constexpr (VEC) {
+    if (c < D) r.load(p + c); else r.zero();
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.e[i] = c + i < D ? p[c + i] : elem_from_float<T>(0.f);
+  }
+  return r;
+}
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void store_row(T* p, int c, int D, const Pack<T, V>& r) {
+  if constexpr (VEC) {
+    if (c < D) r.store(p + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < D) p[c + i] = r.e[i];
+  }
+}
+
+// The rows of one tile on their way from memory: what lies behind `len` reads as 0
+template <typename T, int G, int CT, bool VEC, bool DY>
+struct Tile {
+  using S = Shape<T, G, CT>;
+  Pack<T, S::V> u[S::NV], dt[S::NV], dy[DY ? S::NV : 1];
+  Pack<T, 4> B[S::NB], C[S::NB];
+
+  template <bool WANT_B = true, bool WANT_C = true>
+  __device__ __forceinline__ void load(const BdhScanDesc& d, int b, int c0, int t0, int len) {
+    const int lane = threadIdx.x & 31, t = t0 + lane / 2, c = c0 + (lane & 1) * S::E, n = (lane & 1) * (S::NP / 2);
+    const bool in = t < len;
+    const T* pu = static_cast<const T*>(d.u) + b * d.u_sb + t * d.u_st;
+    const T* pt = static_cast<const T*>(d.dt) + b * d.dt_sb + t * d.dt_st;
+    const T* pb = static_cast<const T*>(d.B_) + b * d.b_sb + t * d.b_st;
+    const T* pc = static_cast<const T*>(d.C_) + b * d.c_sb + t * d.c_st;
+    const int D = in ? d.D : 0, N = in ? d.N : 0;
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i) {
+      u[i] = load_row<T, S::V, VEC>(pu, c + i * S::V, D);
+      dt[i] = load_row<T, S::V, VEC>(pt, c + i * S::V, D);
+      if constexpr (DY)
+        dy[i] = load_row<T, S::V, VEC>(static_cast<const T*>(d.dy) + b * d.dy_sb + t * d.dy_st, c + i * S::V, D);
+    }
+#pragma unroll
+    for (int i = 0; i < S::NB; ++i) {
+      if constexpr (WANT_B) B[i] = load_row<T, 4, VEC>(pb, n + 4 * i, N);
+      if constexpr (WANT_C) C[i] = load_row<T, 4, VEC>(pc, n + 4 * i, N);
+    }
+  }
+};
+
+// What a warp's compute loop reads: rows padded by 16 bytes, so that eight lanes that store four rows meet no bank twice
+template <int G, int CT, bool DY>
+struct alignas(16) WarpMem {
+  static constexpr int NP = 4 * G, CW = 32 / G * CT;
+  float2 step[LT][CW + 2];                             // dt', dt' u
+  float B[LT][NP], C[LT][NP];
+  float dy[DY ? LT : 1][CW + 4];
+  float bias[CW], skip[CW];
+
+  __device__ __forceinline__ void params(const BdhScanDesc& d, int c0) {
+    for (int i = threadIdx.x & 31; i < CW; i += 32) {
+      bias[i] = (d.dt_bias && c0 + i < d.D) ? d.dt_bias[c0 + i] : 0.f;
+      skip[i] = (d.skip && c0 + i < d.D) ? d.skip[c0 + i] : 0.f;
+    }
+  }
+  // channels behind D and rows behind `len` get dt' = 0: their states stay as they are
+  template <typename T, bool VEC, bool WANT_B = true, bool WANT_C = true>
+  __device__ __forceinline__ void put(const BdhScanDesc& d, const Tile<T, G, CT, VEC, DY>& x, int c0, int t0, int len) {
+    using S = Shape<T, G, CT>;
+    const int lane = threadIdx.x & 31, t = lane / 2, c = (lane & 1) * S::E, n = (lane & 1) * (NP / 2);
+    const int have = t0 + t < len ? d.D - c0 - c : 0;  // of this lane's channels
+    float dt[S::E + 1], uu[S::E + 1];
+    dt[S::E] = uu[S::E] = 0.f;
+#pragma unroll
+    for (int j = 0; j < S::E; ++j) {
+      dt[j] = x.dt[j / S::V][j % S::V] + bias[c + j];
+      uu[j] = x.u[j / S::V][j % S::V];
+    }
+#pragma unroll
+    for (int j = 0; j < S::E; j += 2) {
+      f2 s = pack2(dt[j], dt[j + 1]);
+      if (d.softplus) s = softplus2(s);
+      float s0, s1;
+      unpack2(s, s0, s1);
+      s0 = j < have ? s0 : 0.f;
+      s1 = j + 1 < have ? s1 : 0.f;
+      const float v0 = j < have ? s0 * uu[j] : 0.f, v1 = j + 1 < have ? s1 * uu[j + 1] : 0.f;
+      if constexpr (S::E > 1)
+        *reinterpret_cast<float4*>(&step[t][c + j]) = make_float4(s0, v0, s1, v1);
+      else
+        step[t][c] = make_float2(s0, v0);
+    }
+    if constexpr (DY)
+#pragma unroll
+      for (int j = 0; j < S::E; ++j) dy[t][c + j] = x.dy[j / S::V][j % S::V];
+#pragma unroll
+    for (int i = 0; i < S::NB; ++i) {
+      if constexpr (WANT_B) *reinterpret_cast<float4*>(&B[t][n + 4 * i]) = make_float4(x.B[i][0], x.B[i][1], x.B[i][2], x.B[i][3]);
+      if constexpr (WANT_C) *reinterpret_cast<float4*>(&C[t][n + 4 * i]) = make_float4(x.C[i][0], x.C[i][1], x.C[i][2], x.C[i][3]);
+    }
+  }
+  __device__ __forceinline__ void steps(int t, int cl, f2 (&dt)[CT], f2 (&du)[CT]) const {
+    if constexpr (CT == 2) {
+      const float4 v = *reinterpret_cast<const float4*>(&step[t][cl]);
+      dt[0] = both(v.x); du[0] = both(v.y);
+      dt[1] = both(v.z); du[1] = both(v.w);
+    } else {
+      const float2 v = step[t][cl];
+      dt[0] = both(v.x);
+      du[0] = both(v.y);
+    }
+  }
+  __device__ __forceinline__ void dys(int t, int cl, f2 (&g)[CT]) const {
+    if constexpr (CT == 2) {
+      const float2 v = *reinterpret_cast<const float2*>(&dy[t][cl]);
+      g[0] = both(v.x);
+      g[1] = both(v.y);
+    } else {
+      g[0] = both(dy[t][cl]);
+    }
+  }
+};
+
+// This lane's 4 states (n0 ..) of channel c in a [.., D, N] tensor
+__device__ __forceinline__ void load_state(const float* p, int c, int n0, const BdhScanDesc& d, f2 (&h)[2]) {
+  float v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = (p != nullptr && c < d.D && n0 + j < d.N) ? p[static_cast<long long>(c) * d.N + n0 + j] : 0.f;
+  h[0] = pack2(v[0], v[1]);
+  h[1] = pack2(v[2], v[3]);
+}
+__device__ __forceinline__ void store_state(float* p, int c, int n0, const BdhScanDesc& d, const f2 (&h)[2]) {
+  float v[4];
+  unpack2(h[0], v[0], v[1]);
+  unpack2(h[1], v[2], v[3]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c < d.D && n0 + j < d.N) p[static_cast<long long>(c) * d.N + n0 + j] = v[j];
+}
+
+// A2 = A log2(e); 0 for padding
+template <int CT>
+__device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (&A2)[CT][2]) {
+#pragma unroll
+  for (int k = 0; k < CT; ++k) {
+    load_state(d.A, c + k, n0, d, A2[k]);
+    A2[k][0] = mul2(A2[k][0], both(LOG2E));
+    A2[k][1] = mul2(A2[k][1], both(LOG2E));
+  }
+}
+
+// The state a segment starts from: `h` (the sequence's own) carried through the segments before it, in order; in reverse
+// through those behind it.
+template <int CT, int NP>
+__device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to, int by, int c, int n0, const f2 (&A2)[CT][2], f2 (&h)[CT][2]) {
+  for (int s = from; s != to; s += by) {
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+      if (c + k >= a.d.D) continue;
+      const long long at = (static_cast<long long>(b) * a.segs + s) * a.d.D + c + k;
+      const f2 dt = both(a.seg_dt[at]);
+      f2 s0, s1;
+      load4(a.seg_state + at * NP + n0, s0, s1);
+      h[k][0] = fma2(ex2x2(mul2(dt, A2[k][0])), h[k][0], s0);
+      h[k][1] = fma2(ex2x2(mul2(dt, A2[k][1])), h[k][1], s1);
+    }
+  }
+}
+
+struct Where {
+  int part, b, seg;                    // channels, sequence, segment
+};
+__device__ __forceinline__ Where where(const ScanArgs& a, long long unit) {
+  Where w;
+  w.part = static_cast<int>(unit % a.parts);
+  const int bs = static_cast<int>(unit / a.parts);
+  w.b = bs / a.segs;
+  w.seg = bs - w.b * a.segs;
+  return w;
+}
+
+// ---- forward -----------------------------------------------------------------------------------------
+// Each warp on its own. The partial sums over a lane's 4 states go through shared memory: a channel's G lanes are
+// added up where the outputs are written, which costs a store a step instead of a chain of exchanges.
+template <int G, int CT>
+struct FwdMem : WarpMem<G, CT, false> {
+  alignas(16) float part[LT][CT * 32 + 4];
+};
+
+template <typename T, int G, int CT, bool VEC>
+__global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_fwd_kernel(const ScanArgs a, long long units, float* marks) {
+  using S = Shape<T, G, CT>;
+  __shared__ __align__(16) FwdMem<G, CT> mem[FWD_WARPS];
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * FWD_WARPS + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  FwdMem<G, CT>& sh = mem[threadIdx.x >> 5];
+  const BdhScanDesc& d = a.d;
+  const Where w = where(a, unit);
+  const int n0 = lane % G * 4, cl = lane / G * CT, c0 = w.part * S::CW, c = c0 + cl;
+  const int len = a.len.get(w.b, d.T);
+  f2 A2[CT][2], h[CT][2];
+  load_a<CT>(d, c, n0, A2);
+#pragma unroll
+  for (int k = 0; k < CT; ++k)
+    load_state(d.h0 ? d.h0 + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, h[k]);
+  carry<CT, S::NP>(a, w.b, 0, w.seg, 1, c, n0, A2, h);
+  sh.params(d, c0);
+  const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles);
+  Tile<T, G, CT, VEC, false> x;
+  x.load(d, w.b, c0, first * LT, len);
+  __syncwarp();
+  const int row = lane / 2, col = (lane & 1) * S::E;
+  for (int tile = first; tile < last; ++tile) {
+    const int t0 = tile * LT;
+    const bool any = t0 < len;
+    Pack<T, S::V> u[S::NV];
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i) u[i] = x.u[i];
+    if (any) {
+      sh.put(d, x, c0, t0, len);
+      __syncwarp();
+      if (tile + 1 < last) x.load(d, w.b, c0, t0 + LT, len);
+      if (marks != nullptr)
+#pragma unroll
+        for (int k = 0; k < CT; ++k)
+          if (c + k < d.D)
+            *reinterpret_cast<ulonglong2*>(marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0) =
+                make_ulonglong2(h[k][0], h[k][1]);
+      constexpr int GS = 8 / CT;                       // the exponentials of a group of steps ahead of the chain through h
+#pragma unroll
+      for (int s0 = 0; s0 < LT; s0 += GS) {
+        f2 e[GS][CT][2], in[GS][CT][2];
+#pragma unroll
+        for (int s = 0; s < GS; ++s) {
+          f2 dt[CT], du[CT], b0, b1;
+          sh.steps(s0 + s, cl, dt, du);
+          load4(&sh.B[s0 + s][n0], b0, b1);
+#pragma unroll
+          for (int k = 0; k < CT; ++k) {
+            e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
+            e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
+            in[s][k][0] = mul2(du[k], b0);
+            in[s][k][1] = mul2(du[k], b1);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < GS; ++s) {
+          f2 k0, k1;
+          load4(&sh.C[s0 + s][n0], k0, k1);
+#pragma unroll
+          for (int k = 0; k < CT; ++k) {
+            h[k][0] = fma2(e[s][k][0], h[k][0], in[s][k][0]);
+            h[k][1] = fma2(e[s][k][1], h[k][1], in[s][k][1]);
+            sh.part[s0 + s][k * 32 + lane] = sum2(fma2(k1, h[k][1], mul2(k0, h[k][0])));
+          }
+        }
+      }
+      __syncwarp();
+    }
+    if (t0 + row < d.T) {
+      T* y = static_cast<T*>(d.y) + (static_cast<long long>(w.b) * d.T + t0 + row) * d.D;
+      const bool in = t0 + row < len;
+#pragma unroll
+      for (int i = 0; i < S::NV; ++i) {
+        Pack<T, S::V> o;
+#pragma unroll
+        for (int j = 0; j < S::V; ++j) {
+          const int cc = col + i * S::V + j;
+          float v = 0.f;
+          if (in) {
+            const float* p = &sh.part[row][cc % CT * 32 + cc / CT * G];
+            if constexpr (G == 2) {
+              const float2 q = *reinterpret_cast<const float2*>(p);
+              v = q.x + q.y;
+            } else {
+#pragma unroll
+              for (int g = 0; g < G; g += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(p + g);
+                v += (q.x + q.y) + (q.z + q.w);
+              }
+            }
+            v = fmaf(sh.skip[cc], u[i][j], v);
+          }
+          o.set(j, v);
+        }
+        store_row<T, S::V, VEC>(y, c0 + col + i * S::V, d.D, o);
+      }
+    }
+  }
+  if (w.seg == a.segs - 1)
+#pragma unroll
+    for (int k = 0; k < CT; ++k) store_state(d.hT + static_cast<long long>(w.b) * d.D * d.N, c + k, n0, d, h[k]);
+}
+
+// States of the segments from zero: h_t = a_t h_{t-1} + dt' u B_t, or in reverse r_t = a_t (r_{t+1} + dy_t C_t); and the
+// sum of the segment's steps. Each warp on its own.
+template <typename T, int G, int CT, bool VEC, bool REV>
+__global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_sweep_kernel(const ScanArgs a, long long units, float* seg_state, float* seg_dt) {
+  using S = Shape<T, G, CT>;
+  __shared__ __align__(16) WarpMem<G, CT, REV> mem[FWD_WARPS];
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * FWD_WARPS + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  WarpMem<G, CT, REV>& sh = mem[threadIdx.x >> 5];
+  const BdhScanDesc& d = a.d;
+  const Where w = where(a, unit);
+  const int n0 = lane % G * 4, cl = lane / G * CT, c0 = w.part * S::CW, c = c0 + cl;
+  const int len = a.len.get(w.b, d.T);
+  f2 A2[CT][2], h[CT][2], total = both(0.f);
+  load_a<CT>(d, c, n0, A2);
+#pragma unroll
+  for (int k = 0; k < CT; ++k) h[k][0] = h[k][1] = both(0.f);
+  sh.params(d, c0);
+  const int first = w.seg * a.per_seg, end = min(min(first + a.per_seg, a.tiles), (len + LT - 1) / LT);
+  const int n = end - first;
+  Tile<T, G, CT, VEC, REV> x;
+  if (n > 0) x.template load<!REV, REV>(d, w.b, c0, (REV ? end - 1 : first) * LT, len);
+  __syncwarp();
+  for (int i = 0; i < n; ++i) {
+    const int t0 = (REV ? end - 1 - i : first + i) * LT;
+    sh.template put<T, VEC, !REV, REV>(d, x, c0, t0, len);
+    __syncwarp();
+    if (i + 1 < n) x.template load<!REV, REV>(d, w.b, c0, REV ? t0 - LT : t0 + LT, len);
+    constexpr int GS = 8 / CT;
+#pragma unroll
+    for (int s0 = 0; s0 < LT; s0 += GS) {
+      f2 e[GS][CT][2], in[GS][CT][2];
+#pragma unroll
+      for (int s = 0; s < GS; ++s) {
+        const int t = REV ? LT - 1 - s0 - s : s0 + s;
+        f2 dt[CT], du[CT], b0, b1;
+        sh.steps(t, cl, dt, du);
+        load4(REV ? &sh.C[t][n0] : &sh.B[t][n0], b0, b1);
+        if constexpr (REV) sh.dys(t, cl, du);
+#pragma unroll
+        for (int k = 0; k < CT; ++k) {
+          e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
+          e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
+          in[s][k][0] = mul2(du[k], b0);
+          in[s][k][1] = mul2(du[k], b1);
+        }
+        float p, q;
+        if constexpr (CT == 2) {
+          float r;
+          unpack2(dt[0], p, r);
+          unpack2(dt[1], q, r);
+        } else {
+          unpack2(dt[0], p, q);
+        }
+        total = add2(total, pack2(p, q));
+      }
+#pragma unroll
+      for (int s = 0; s < GS; ++s)
+#pragma unroll
+        for (int k = 0; k < CT; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            h[k][j] = REV ? mul2(e[s][k][j], add2(h[k][j], in[s][k][j])) : fma2(e[s][k][j], h[k][j], in[s][k][j]);
+    }
+    __syncwarp();
+  }
+  float sums[2];
+  unpack2(total, sums[0], sums[1]);
+#pragma unroll
+  for (int k = 0; k < CT; ++k)
+    if (c + k < d.D) {
+      const long long at = (static_cast<long long>(w.b) * a.segs + w.seg) * d.D + c + k;
+      *reinterpret_cast<ulonglong2*>(seg_state + at * S::NP + n0) = make_ulonglong2(h[k][0], h[k][1]);
+      if (n0 == 0) seg_dt[at] = sums[k];
+    }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------
+struct ScanGrads {
+  const float* marks;                  // [B][tiles][D][NP]: h at the start of every tile
+  float* bc;                           // [channel blocks][B][T][2 NP]: partial dB | dC
+  float* da;                           // [B][segs][D][NP]: partial dA
+  float* per_channel;                  // [2][B][segs][D]: partial dD, dbias
+};
+
+template <int G, int CT>
+struct BwdMem {
+  static constexpr int NP = 4 * G, CW = 32 / G * CT;
+  struct PerWarp {
+    WarpMem<G, CT, true> in;
+    float2 out[LT][CW + 2];            // sum g B, sum A2 q
+    ulonglong2 h[LT][CT][32];          // h_{t-1}, each lane its own
+  } warp[BWD_WARPS];
+  alignas(16) float bc[BWD_WARPS][LT][2 * NP];     // the warps' sums over their channels
+};
+
+template <typename T, int G, int CT, bool VEC>
+__global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(const ScanArgs a, const ScanGrads o) {
+  using S = Shape<T, G, CT>;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  BwdMem<G, CT>& all = *reinterpret_cast<BwdMem<G, CT>*>(smem_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  typename BwdMem<G, CT>::PerWarp& sh = all.warp[warp];
+  const BdhScanDesc& d = a.d;
+  const Where w = where(a, blockIdx.x);
+  const int n0 = lane % G * 4, cl = lane / G * CT, c0 = (w.part * BWD_WARPS + warp) * S::CW, c = c0 + cl;
+  const int len = a.len.get(w.b, d.T);
+  f2 A2[CT][2], r[CT][2], da[CT][2];
+  load_a<CT>(d, c, n0, A2);
+#pragma unroll
+  for (int k = 0; k < CT; ++k) {
+    load_state(d.dhT ? d.dhT + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, r[k]);
+    da[k][0] = da[k][1] = both(0.f);
+  }
+  carry<CT, S::NP>(a, w.b, a.segs - 1, w.seg, -1, c, n0, A2, r);
+  sh.in.params(d, c0);
+  float sum_skip[S::E], sum_bias[S::E];                // of this lane's channels, over its rows
+#pragma unroll
+  for (int j = 0; j < S::E; ++j) sum_skip[j] = sum_bias[j] = 0.f;
+  const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles);
+  const int row = lane / 2, col = (lane & 1) * S::E;
+  Tile<T, G, CT, VEC, true> x;
+  x.load(d, w.b, c0, (last - 1) * LT, len);
+  __syncwarp();
+  for (int tile = last - 1; tile >= first; --tile) {
+    const int t0 = tile * LT;
+    const bool any = t0 < len;                         // (the same for the whole block)
+    Pack<T, S::V> u[S::NV], dt_raw[S::NV], dy[S::NV];
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i) {
+      u[i] = x.u[i];
+      dt_raw[i] = x.dt[i];
+      dy[i] = x.dy[i];
+    }
+    if (any) {
+      f2 h[CT][2], dat[CT][2];
+      sh.in.put(d, x, c0, t0, len);
+#pragma unroll
+      for (int k = 0; k < CT; ++k) {
+        h[k][0] = h[k][1] = dat[k][0] = dat[k][1] = both(0.f);
+        if (c + k < d.D)
+          load4(o.marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0, h[k][0], h[k][1]);
+      }
+      __syncwarp();
+      if (tile > first) x.load(d, w.b, c0, t0 - LT, len);
+      constexpr int GS = 8 / CT;
+#pragma unroll
+      for (int s0 = 0; s0 < LT; s0 += GS) {
+        f2 e[GS][CT][2], in[GS][CT][2];
+#pragma unroll
+        for (int s = 0; s < GS; ++s) {
+          f2 dt[CT], du[CT], b0, b1;
+          sh.in.steps(s0 + s, cl, dt, du);
+          load4(&sh.in.B[s0 + s][n0], b0, b1);
+#pragma unroll
+          for (int k = 0; k < CT; ++k) {
+            e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
+            e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
+            in[s][k][0] = mul2(du[k], b0);
+            in[s][k][1] = mul2(du[k], b1);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < GS; ++s)
+#pragma unroll
+          for (int k = 0; k < CT; ++k) {
+            sh.h[s0 + s][k][lane] = make_ulonglong2(h[k][0], h[k][1]);
+            h[k][0] = fma2(e[s][k][0], h[k][0], in[s][k][0]);
+            h[k][1] = fma2(e[s][k][1], h[k][1], in[s][k][1]);
+          }
+      }
+#pragma unroll 4
+      for (int t = LT - 1; t >= 0; --t) {
+        f2 dt[CT], du[CT], gy[CT], b0, b1, k0, k1, sb0, sb1, sc0, sc1;
+        sh.in.steps(t, cl, dt, du);
+        sh.in.dys(t, cl, gy);
+        load4(&sh.in.B[t][n0], b0, b1);
+        load4(&sh.in.C[t][n0], k0, k1);
+        float nv[2 * CT];
+#pragma unroll
+        for (int k = 0; k < CT; ++k) {
+          const f2 g0 = fma2(gy[k], k0, r[k][0]), g1 = fma2(gy[k], k1, r[k][1]);
+          const ulonglong2 hp = sh.h[t][k][lane];
+          if (k == 0) {
+            sb0 = mul2(g0, du[k]); sb1 = mul2(g1, du[k]);
+            sc0 = mul2(gy[k], h[k][0]); sc1 = mul2(gy[k], h[k][1]);
+          } else {
+            sb0 = fma2(g0, du[k], sb0); sb1 = fma2(g1, du[k], sb1);
+            sc0 = fma2(gy[k], h[k][0], sc0); sc1 = fma2(gy[k], h[k][1], sc1);
+          }
+          r[k][0] = mul2(ex2x2(mul2(dt[k], A2[k][0])), g0);
+          r[k][1] = mul2(ex2x2(mul2(dt[k], A2[k][1])), g1);
+          const f2 q0 = mul2(r[k][0], hp.x), q1 = mul2(r[k][1], hp.y);
+          dat[k][0] = fma2(dt[k], q0, dat[k][0]);
+          dat[k][1] = fma2(dt[k], q1, dat[k][1]);
+          nv[2 * k] = sum2(fma2(g1, b1, mul2(g0, b0)));
+          nv[2 * k + 1] = sum2(fma2(A2[k][1], q1, mul2(A2[k][0], q0)));
+          h[k][0] = hp.x;
+          h[k][1] = hp.y;
+        }
+        int at;
+        bool once;
+        sum_over<2 * CT, G, 1>(nv, lane, at, once);
+        constexpr int NLEFT = 2 * CT / G > 1 ? 2 * CT / G : 1;
+        if (once)
+#pragma unroll
+          for (int i = 0; i < NLEFT; ++i) reinterpret_cast<float*>(&sh.out[t][cl])[at + i] = nv[i];
+        float cv[8];                                   // dB of the 4 states, then dC
+        unpack2(sb0, cv[0], cv[1]);
+        unpack2(sb1, cv[2], cv[3]);
+        unpack2(sc0, cv[4], cv[5]);
+        unpack2(sc1, cv[6], cv[7]);
+        sum_over<8, S::LANES, G>(cv, lane, at, once);
+        constexpr int CLEFT = 8 / S::LANES > 1 ? 8 / S::LANES : 1;
+        if (once)
+#pragma unroll
+          for (int i = 0; i < CLEFT; ++i) all.bc[warp][t][(at + i) / 4 * S::NP + n0 + (at + i) % 4] = cv[i];
+      }
+#pragma unroll
+      for (int k = 0; k < CT; ++k) {                   // sums of tiles: a chain of 16, then one of the tiles
+        da[k][0] = add2(da[k][0], dat[k][0]);
+        da[k][1] = add2(da[k][1], dat[k][1]);
+      }
+    } else if (tile > first) {
+      x.load(d, w.b, c0, t0 - LT, len);
+    }
+    __syncthreads();
+    if (t0 + row < d.T) {
+      const bool in = t0 + row < len;
+      const long long at = (static_cast<long long>(w.b) * d.T + t0 + row) * d.D;
+#pragma unroll
+      for (int i = 0; i < S::NV; ++i) {
+        Pack<T, S::V> pu, pd;
+        float raw[S::V + 1], dd[S::V + 1];
+        raw[S::V] = dd[S::V] = 0.f;
+#pragma unroll
+        for (int j = 0; j < S::V; ++j) {
+          const int cc = col + i * S::V + j;
+          raw[j] = dt_raw[i][j] + sh.in.bias[cc];
+          float du = 0.f;
+          dd[j] = 0.f;
+          if (in) {
+            const float2 s = sh.out[row][cc];
+            du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
+            dd[j] = fmaf(u[i][j], s.x, LN2 * s.y);
+            sum_skip[i * S::V + j] = fmaf(dy[i][j], u[i][j], sum_skip[i * S::V + j]);
+          }
+          pu.set(j, du);
+        }
+        if (d.softplus && in)
+#pragma unroll
+          for (int j = 0; j < S::V; j += 2) {
+            float s0, s1;
+            unpack2(sigmoid2(pack2(raw[j], raw[j + 1])), s0, s1);
+            dd[j] *= s0;
+            dd[j + 1] *= s1;
+          }
+#pragma unroll
+        for (int j = 0; j < S::V; ++j) {
+          pd.set(j, dd[j]);
+          sum_bias[i * S::V + j] += dd[j];
+        }
+        store_row<T, S::V, VEC>(static_cast<T*>(d.du) + at, c0 + col + i * S::V, d.D, pu);
+        store_row<T, S::V, VEC>(static_cast<T*>(d.ddt) + at, c0 + col + i * S::V, d.D, pd);
+      }
+    }
+    for (int i = threadIdx.x; i < LT * S::NP / 2; i += 32 * BWD_WARPS) {
+      const int t = i / (S::NP / 2), n = i % (S::NP / 2) * 4;
+      if (t0 + t >= d.T) break;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (any)
+#pragma unroll
+        for (int k = 0; k < BWD_WARPS; ++k) {
+          const float4 q = *reinterpret_cast<const float4*>(&all.bc[k][t][n]);
+          s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+        }
+      *reinterpret_cast<float4*>(o.bc + ((static_cast<long long>(w.part) * d.B + w.b) * d.T + t0 + t) * (2 * S::NP) + n) = s;
+    }
+    __syncthreads();
+  }
+  const long long seg = static_cast<long long>(w.b) * a.segs + w.seg;
+#pragma unroll
+  for (int k = 0; k < CT; ++k) {
+    if (c + k < d.D) *reinterpret_cast<ulonglong2*>(o.da + (seg * d.D + c + k) * S::NP + n0) = make_ulonglong2(da[k][0], da[k][1]);
+    if (w.seg == 0 && d.dh0 != nullptr) store_state(d.dh0 + static_cast<long long>(w.b) * d.D * d.N, c + k, n0, d, r[k]);
+  }
+  // the 16 lanes of a warp that share channels add their sums up
+#pragma unroll
+  for (int j = 0; j < S::E; ++j) {
+#pragma unroll
+    for (int off = 16; off > 1; off >>= 1) {
+      sum_skip[j] += __shfl_xor_sync(0xffffffffu, sum_skip[j], off);
+      sum_bias[j] += __shfl_xor_sync(0xffffffffu, sum_bias[j], off);
+    }
+    const int cc = c0 + col + j;
+    if (lane < 2 && cc < d.D) {
+      o.per_channel[seg * d.D + cc] = sum_skip[j];
+      o.per_channel[(static_cast<long long>(d.B) * a.segs + seg) * d.D + cc] = sum_bias[j];
+    }
+  }
+}
+
+// dB, dC: sums over the channel blocks, in order
+template <typename T>
+__global__ void __launch_bounds__(256) selective_scan_bc_kernel(const float* part, int blocks, long long rows, int NP, int N, T* dB, T* dC) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, all = rows * 2 * NP;
+  if (i >= all) return;
+  const int n = static_cast<int>(i % (2 * NP));
+  if (n % NP >= N) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < blocks; ++k) s += part[k * all + i];
+  (n >= NP ? dC : dB)[i / (2 * NP) * N + n % NP] = elem_from_float<T>(s);
+}
+
+// dA, dD, dbias: sums over sequences and segments, in order
+__global__ void __launch_bounds__(256) selective_scan_params_kernel(const float* da, const float* per_channel, int parts, int D, int NP, int N,
+                                                                    float* dA, float* dD, float* dbias) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, na = static_cast<long long>(D) * NP;
+  float s = 0.f;
+  if (i < na) {
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) s += da[k * na + i];
+    const int n = static_cast<int>(i % NP);
+    if (n < N) dA[i / NP * N + n] = s;
+  } else if (i < na + 2 * D) {
+    const long long j = i - na, what = j / D;
+    for (int k = 0; k < parts; ++k) s += per_channel[(what * parts + k) * D + j % D];
+    float* p = what ? dbias : dD;
+    if (p != nullptr) p[j % D] = s;
+  }
+}
+
+// ---- one token ---------------------------------------------------------------------------------------
+// Bound by the states: 4 B N D read and written per stream.
+template <typename T, int G>
+__global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const BdhScanDesc d, const float* h, long long h_sb, float* out, long long out_sb,
+                                                                 const unsigned char* active, int vec4) {
+  const int lane = threadIdx.x & 31, ng = lane % G, n0 = 4 * ng;
+  const long long i = (static_cast<long long>(blockIdx.x) * STEP_THREADS + threadIdx.x) / G;
+  const int b = static_cast<int>(i / d.D), c = static_cast<int>(i % d.D);
+  const bool live = b < d.B, on = live && (active == nullptr || active[b] != 0);
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, y = 0.f, u = 0.f;
+  const long long at = static_cast<long long>(c) * d.N + n0;
+  if (live) {
+    const float* hp = h + b * h_sb + at;
+    if (vec4 && n0 < d.N) {
+      const float4 t = *reinterpret_cast<const float4*>(hp);
+      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = n0 + j < d.N ? hp[j] : 0.f;
+    }
+    if (on) {
+      u = elem_to_float<T>(static_cast<const T*>(d.u)[b * d.u_sb + c]);
+      const float raw = elem_to_float<T>(static_cast<const T*>(d.dt)[b * d.dt_sb + c]) + (d.dt_bias ? d.dt_bias[c] : 0.f);
+      float dt = raw, same;
+      if (d.softplus) unpack2(softplus2(both(raw)), dt, same);
+      const float du = dt * u;
+      const T* bp = static_cast<const T*>(d.B_) + b * d.b_sb + n0;
+      const T* cp = static_cast<const T*>(d.C_) + b * d.c_sb + n0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + j < d.N) {
+          v[j] = fmaf(ex2(dt * (d.A[at + j] * LOG2E)), v[j], du * elem_to_float<T>(bp[j]));
+          y = fmaf(elem_to_float<T>(cp[j]), v[j], y);
+        }
+    }
+  }
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  if (!live) return;
+  float* op = out + b * out_sb + at;
+  if (on || op != h + b * h_sb + at) {
+    if (vec4 && n0 < d.N) {
+      *reinterpret_cast<float4*>(op) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + j < d.N) op[j] = v[j];
+    }
+  }
+  if (ng == 0)
+    static_cast<T*>(d.y)[static_cast<long long>(b) * d.D + c] = elem_from_float<T>(on ? fmaf(d.skip ? d.skip[c] : 0.f, u, y) : 0.f);
+}
+
+// ---- host --------------------------------------------------------------------------------------------
+bool multiple(const void* p, long long bytes) { return reinterpret_cast<unsigned long long>(p) % bytes == 0; }
+
+int checked(const BdhScanDesc& d) {
+  if (d.dtype < 0 || d.dtype > 2 || d.B < 0 || d.T < 0 || d.D < 1 || d.N < 1 || d.N > 64) return BDH_ERR_ARGUMENT;
+  return BDH_OK;
+}
+
+int lanes_for(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+
+struct Plan {
+  int G, CT, parts, tiles, per_seg, segs;
+};
+
+Plan plan(const BdhScanDesc& d, int CT, int warps, long long segs) {
+  Plan p;
+  p.G = lanes_for(d.N);
+  p.CT = CT;
+  const int cb = warps * 32 / p.G * CT;
+  p.parts = (d.D + cb - 1) / cb;
+  p.tiles = (d.T + LT - 1) / LT;
+  if (segs > p.tiles) segs = p.tiles > 0 ? p.tiles : 1;
+  p.per_seg = static_cast<int>((p.tiles + segs - 1) / segs);
+  if (p.per_seg < 1) p.per_seg = 1;
+  p.segs = p.tiles > 0 ? (p.tiles + p.per_seg - 1) / p.per_seg : 1;
+  return p;
+}
+
+constexpr int MOST_SEGS = 64;          // so that combining the segments stays cheap beside them
+
+// One or two channels a lane (two: fewer reads of B and C a channel; one: twice the warps), and how many segments
+// (which cost the exponentials a second time): the smaller of the times that a tile takes a warp on its own and a
+// scheduler (592 of them) that is kept busy, in clocks.
+Plan fwd_plan(const BdhScanDesc& d) {
+  Plan best = plan(d, 2, 1, 1);
+  double least = 0;
+  for (int CT = 1; CT <= 2; ++CT)
+    for (int segs = 1; segs <= MOST_SEGS; segs += segs < 8 ? 1 : 4) {
+      const Plan p = plan(d, CT, 1, segs);
+      const double alone = CT == 2 ? 1900 : 1300, busy = CT == 2 ? 1150 : 650;
+      const double per_scheduler = static_cast<double>(d.B) * p.segs * p.parts / 592;
+      const double tile = alone > busy * per_scheduler ? alone : busy * per_scheduler;
+      const double t = p.per_seg * tile * (p.segs > 1 ? 1.7 : 1) + (p.segs > 1 ? 6000 + 40.0 * p.segs : 0);
+      if (least == 0 || t < least) {
+        least = t;
+        best = p;
+      }
+    }
+  return best;
+}
+
+// Two blocks fit an SM: whole rounds of 296, with segments as long as that leaves them.
+Plan bwd_plan(const BdhScanDesc& d) {
+  Plan best = plan(d, 2, BWD_WARPS, 1);
+  double least = 0;
+  for (int segs = 1; segs <= MOST_SEGS; ++segs) {
+    const Plan p = plan(d, 2, BWD_WARPS, segs);
+    const long long blocks = static_cast<long long>(d.B) * p.segs * p.parts;
+    const double rounds = blocks <= 148 ? 0.7 : static_cast<double>((blocks + 295) / 296);
+    const double t = rounds * (p.per_seg + 1) * (p.segs > 1 ? 1.3 : 1) + (p.segs > 1 ? 2 : 0);
+    if (least == 0 || t < least) {
+      least = t;
+      best = p;
+    }
+  }
+  return best;
+}
+
+long long round4(long long n) { return (n + 3) / 4 * 4; }          // pieces of the scratch start on 16 bytes
+
+long long seg_floats(const BdhScanDesc& d, const Plan& p) {
+  return p.segs > 1 ? round4(static_cast<long long>(d.B) * p.segs * d.D * (4 * p.G + 1)) : 0;
+}
+long long bc_floats(const BdhScanDesc& d, const Plan& p) { return static_cast<long long>(p.parts) * d.B * d.T * 8 * p.G; }
+long long da_floats(const BdhScanDesc& d, const Plan& p) { return static_cast<long long>(d.B) * p.segs * d.D * 4 * p.G; }
+
+ScanArgs args_for(const BdhScanDesc& d, const Plan& p, const float* seg) {
+  ScanArgs a;
+  a.d = d;
+  a.len = Lengths{d.lengths, d.lengths64};
+  a.tiles = p.tiles; a.per_seg = p.per_seg; a.segs = p.segs; a.parts = p.parts;
+  a.seg_state = seg;
+  a.seg_dt = seg ? seg + static_cast<long long>(d.B) * p.segs * d.D * (4 * p.G) : nullptr;
+  return a;
+}
+
+// Can rows be moved in packs of 16 bytes, and those of B and C in packs of 4 states?
+bool packs_fit(const BdhScanDesc& d, int size) {
+  const int V = 16 / size;
+  if (d.D % V || d.N % 4) return false;
+  for (const void* q : {d.u, d.dt, d.dy, static_cast<const void*>(d.y), static_cast<const void*>(d.du), static_cast<const void*>(d.ddt)})
+    if (!multiple(q, 16)) return false;
+  for (long long s : {d.u_sb, d.u_st, d.dt_sb, d.dt_st, d.dy_sb, d.dy_st})
+    if (s % V) return false;
+  if (!multiple(d.B_, 4 * size) || !multiple(d.C_, 4 * size)) return false;
+  for (long long s : {d.b_sb, d.b_st, d.c_sb, d.c_st})
+    if (s % 4) return false;
+  return true;
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? BDH_OK : BDH_ERR_LAUNCH; }
+
+template <typename T, int G, int CT, bool VEC, bool REV>
+int sweep_launch(const ScanArgs& a, const Plan& p, float* seg, cudaStream_t s) {
+  // (a sweep's warps: those of the pass that it serves, whose segments it shares)
+  ScanArgs sw = a;
+  sw.parts = (a.d.D + Shape<T, G, CT>::CW - 1) / Shape<T, G, CT>::CW;
+  const long long units = static_cast<long long>(a.d.B) * p.segs * sw.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
+  if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
+  selective_scan_sweep_kernel<T, G, CT, VEC, REV><<<static_cast<unsigned>(grid), 32 * FWD_WARPS, 0, s>>>(sw, units, seg, const_cast<float*>(a.seg_dt));
+  return launched();
+}
+
+template <typename T, int G, int CT, bool VEC>
+int fwd_launch(const BdhScanDesc& d, const Plan& p, float* marks, float* seg, cudaStream_t s) {
+  const ScanArgs a = args_for(d, p, p.segs > 1 ? seg : nullptr);
+  if (p.segs > 1)
+    if (const int rc = sweep_launch<T, G, CT, VEC, false>(a, p, seg, s)) return rc;
+  const long long units = static_cast<long long>(d.B) * p.segs * p.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
+  if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
+  selective_scan_fwd_kernel<T, G, CT, VEC><<<static_cast<unsigned>(grid), 32 * FWD_WARPS, 0, s>>>(a, units, marks);
+  return launched();
+}
+
+struct BwdOut {
+  float *dA, *dD, *dbias;
+  void *dB, *dC;
+};
+
+template <typename T, int G, bool VEC>
+int bwd_launch(const BdhScanDesc& d, const Plan& p, const ScanGrads& o, float* seg, const BwdOut& out, cudaStream_t s) {
+  constexpr int CT = 2;
+  const ScanArgs a = args_for(d, p, p.segs > 1 ? seg : nullptr);
+  if (p.segs > 1)
+    if (const int rc = sweep_launch<T, G, CT, VEC, true>(a, p, seg, s)) return rc;
+  const long long grid = static_cast<long long>(d.B) * p.segs * p.parts;
+  if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
+  auto kernel = selective_scan_bwd_kernel<T, G, CT, VEC>;
+  constexpr int smem = sizeof(BwdMem<G, CT>);
+  static PerDeviceOnce once;
+  if (once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess ? 0 : 1; }))
+    return BDH_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(grid), 32 * BWD_WARPS, smem, s>>>(a, o);
+  if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
+  const int NP = 4 * G;
+  const long long rows = static_cast<long long>(d.B) * d.T;
+  if ((rows * 2 * NP + 255) / 256 > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
+  selective_scan_bc_kernel<T><<<static_cast<unsigned>((rows * 2 * NP + 255) / 256), 256, 0, s>>>(o.bc, p.parts, rows, NP, d.N,
+                                                                                              static_cast<T*>(out.dB), static_cast<T*>(out.dC));
+  if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
+  const long long n = static_cast<long long>(d.D) * (NP + 2);
+  selective_scan_params_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(o.da, o.per_channel, d.B * p.segs, d.D, NP, d.N, out.dA,
+                                                                                   out.dD, out.dbias);
+  return launched();
+}
+
+template <typename F>
+int by_lanes(int G, const F& f) {
+  switch (G) {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+  }
+  return f(std::integral_constant<int, 16>{});
+}
+}  // namespace
+
+// Of one row type each: compiled in a file of their own (selective_scan_f32.cu, _f16.cu, _bf16.cu).
+template <typename T>
+int selective_scan_fwd_of(const BdhScanDesc& d, float* marks, float* scratch, cudaStream_t s) {
+  const Plan p = fwd_plan(d);
+  if (p.segs > 1 && scratch == nullptr) return BDH_ERR_ARGUMENT;
+  const bool vec = packs_fit(d, sizeof(T));
+  return by_lanes(p.G, [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    if (vec) return p.CT == 2 ? fwd_launch<T, G, 2, true>(d, p, marks, scratch, s) : fwd_launch<T, G, 1, true>(d, p, marks, scratch, s);
+    return p.CT == 2 ? fwd_launch<T, G, 2, false>(d, p, marks, scratch, s) : fwd_launch<T, G, 1, false>(d, p, marks, scratch, s);
+  });
+}
+
+template <typename T>
+int selective_scan_bwd_of(const BdhScanDesc& d, const float* marks, float* scratch, float* dA, float* dD, float* dbias, void* dB, void* dC,
+                          cudaStream_t s) {
+  const Plan p = bwd_plan(d);
+  ScanGrads o;
+  float* seg = scratch;
+  o.marks = marks;
+  o.bc = seg + seg_floats(d, p);
+  o.da = o.bc + bc_floats(d, p);
+  o.per_channel = o.da + da_floats(d, p);
+  const BwdOut out{dA, dD, dbias, dB, dC};
+  const bool vec = packs_fit(d, sizeof(T));
+  return by_lanes(p.G, [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    return vec ? bwd_launch<T, G, true>(d, p, o, seg, out, s) : bwd_launch<T, G, false>(d, p, o, seg, out, s);
+  });
+}
+
+// One token. Bound by the states: 8 B N D bytes a stream.
+template <typename T>
+int selective_scan_step_of(const BdhScanDesc& d, const float* h, long long h_sb, float* out, long long out_sb, const unsigned char* active,
+                           cudaStream_t s) {
+  const int vec4 = d.N % 4 == 0 && h_sb % 4 == 0 && out_sb % 4 == 0 && multiple(h, 16) && multiple(out, 16);
+  return by_lanes(lanes_for(d.N), [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    const long long blocks = (static_cast<long long>(d.B) * d.D * G + STEP_THREADS - 1) / STEP_THREADS;
+    if (blocks > 0x7fffffffLL) return static_cast<int>(BDH_ERR_TOO_LARGE);
+    selective_scan_step_kernel<T, G><<<static_cast<unsigned>(blocks), STEP_THREADS, 0, s>>>(d, h, h_sb, out, out_sb, active, vec4);
+    return launched();
+  });
+}
+
+#define BDH_SCAN_OF(EXTERN, T)                                                                                                          \
+  EXTERN template int selective_scan_fwd_of<T>(const BdhScanDesc&, float*, float*, cudaStream_t);                                       \
+  EXTERN template int selective_scan_bwd_of<T>(const BdhScanDesc&, const float*, float*, float*, float*, float*, void*, void*,         \
+                                               cudaStream_t);                                                                           \
+  EXTERN template int selective_scan_step_of<T>(const BdhScanDesc&, const float*, long long, float*, long long, const unsigned char*,   \
+                                                cudaStream_t);
+
+}  // namespace bdh
