@@ -25,6 +25,7 @@
 #include "device_once.h"
 #include "element_io.cuh"
 
+#include <cmath>
 #include <type_traits>
 
 namespace bdh {
@@ -33,6 +34,9 @@ namespace {
 constexpr int LT = 16;                 // steps per tile
 constexpr int FWD_WARPS = 2;           // independent warps of a block, forward and sweeps
 constexpr int BWD_WARPS = 4;           // warps of a block that add their sums over channels up, backward
+constexpr int FWD_BLOCKS = 6;          // blocks an SM that leave a thread the registers to run ahead (measured: 4 to 8 within 3 %;
+                                       // left to itself the compiler takes 96 and spills: 20 % slower on few warps)
+constexpr int BWD_BLOCKS = 2;
 constexpr int STEP_THREADS = 128;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LOG2E_LO = 1.925963033500e-08f;      // log2(e) - LOG2E
@@ -66,6 +70,9 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// One value with both of a pair (the moves that make the pair cost less than two plain products)
+__device__ __forceinline__ f2 mul1(float a, f2 b) { return mul2(both(a), b); }
+__device__ __forceinline__ f2 fma1(float a, f2 b, f2 c) { return fma2(both(a), b, c); }
 __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   f2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -190,38 +197,122 @@ __device__ __forceinline__ void store_row(T* p, int c, int D, const Pack<T, V>& 
   }
 }
 
-// The rows of one tile on their way from memory: what lies behind `len` reads as 0
+// The rows of one tile on their way from memory (what lies behind `len` reads as 0), in registers: the bits as they were
+// loaded, since taking elements out of them right behind the load would wait for it.
 template <typename T, int G, int CT, bool VEC, bool DY>
 struct Tile {
   using S = Shape<T, G, CT>;
-  Pack<T, S::V> u[S::NV], dt[S::NV], dy[DY ? S::NV : 1];
-  Pack<T, 4> B[S::NB], C[S::NB];
+  using Raw = typename Pack<T, S::V>::Raw;
+  using Raw4 = typename Pack<T, 4>::Raw;
+  Raw ru[S::NV], rdt[S::NV], rdy[DY ? S::NV : 1];
+  Raw4 rB[S::NB], rC[S::NB];
 
-  template <bool WANT_B = true, bool WANT_C = true>
+  template <int V>
+  static __device__ __forceinline__ typename Pack<T, V>::Raw fetch(const T* p, int c, int D) {
+    const Pack<T, V> r = load_row<T, V, VEC>(p, c, D);
+    return *reinterpret_cast<const typename Pack<T, V>::Raw*>(&r);
+  }
+  template <int V>
+  static __device__ __forceinline__ Pack<T, V> bits(const typename Pack<T, V>::Raw& r) {
+    Pack<T, V> p;
+    *reinterpret_cast<typename Pack<T, V>::Raw*>(&p) = r;
+    return p;
+  }
   __device__ __forceinline__ void load(const BdhScanDesc& d, int b, int c0, int t0, int len) {
     const int lane = threadIdx.x & 31, t = t0 + lane / 2, c = c0 + (lane & 1) * S::E, n = (lane & 1) * (S::NP / 2);
     const bool in = t < len;
-    const T* pu = static_cast<const T*>(d.u) + b * d.u_sb + t * d.u_st;
-    const T* pt = static_cast<const T*>(d.dt) + b * d.dt_sb + t * d.dt_st;
-    const T* pb = static_cast<const T*>(d.B_) + b * d.b_sb + t * d.b_st;
-    const T* pc = static_cast<const T*>(d.C_) + b * d.c_sb + t * d.c_st;
     const int D = in ? d.D : 0, N = in ? d.N : 0;
 #pragma unroll
     for (int i = 0; i < S::NV; ++i) {
-      u[i] = load_row<T, S::V, VEC>(pu, c + i * S::V, D);
-      dt[i] = load_row<T, S::V, VEC>(pt, c + i * S::V, D);
-      if constexpr (DY)
-        dy[i] = load_row<T, S::V, VEC>(static_cast<const T*>(d.dy) + b * d.dy_sb + t * d.dy_st, c + i * S::V, D);
+      ru[i] = fetch<S::V>(static_cast<const T*>(d.u) + b * d.u_sb + t * d.u_st, c + i * S::V, D);
+      rdt[i] = fetch<S::V>(static_cast<const T*>(d.dt) + b * d.dt_sb + t * d.dt_st, c + i * S::V, D);
+      if constexpr (DY) rdy[i] = fetch<S::V>(static_cast<const T*>(d.dy) + b * d.dy_sb + t * d.dy_st, c + i * S::V, D);
     }
 #pragma unroll
     for (int i = 0; i < S::NB; ++i) {
-      if constexpr (WANT_B) B[i] = load_row<T, 4, VEC>(pb, n + 4 * i, N);
-      if constexpr (WANT_C) C[i] = load_row<T, 4, VEC>(pc, n + 4 * i, N);
+      rB[i] = fetch<4>(static_cast<const T*>(d.B_) + b * d.b_sb + t * d.b_st, n + 4 * i, N);
+      rC[i] = fetch<4>(static_cast<const T*>(d.C_) + b * d.c_sb + t * d.c_st, n + 4 * i, N);
     }
   }
+  __device__ __forceinline__ Pack<T, S::V> u(int i) const { return bits<S::V>(ru[i]); }
+  __device__ __forceinline__ Pack<T, S::V> dt(int i) const { return bits<S::V>(rdt[i]); }
+  __device__ __forceinline__ Pack<T, S::V> dy(int i) const { return bits<S::V>(rdy[i]); }
+  __device__ __forceinline__ Pack<T, 4> B(int i) const { return bits<4>(rB[i]); }
+  __device__ __forceinline__ Pack<T, 4> C(int i) const { return bits<4>(rC[i]); }
 };
 
-// What a warp's compute loop reads: rows padded by 16 bytes, so that eight lanes that store four rows meet no bank twice
+// The same in shared memory, fetched by asynchronous copies RING - 1 tiles ahead: a warp alone on its scheduler takes less
+// time for a tile than one load from memory. Every lane reads back only what it copied itself.
+constexpr int RING = 3;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
+  const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(BYTES), "r"(in ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory"); }
+
+template <typename T, int G, int CT, bool VEC, bool DY>
+struct Ring {
+  using S = Shape<T, G, CT>;
+  struct alignas(16) Stage {
+    T u[LT * S::CW], dt[LT * S::CW], dy[DY ? LT * S::CW : 8];
+    T B[LT * S::NP], C[LT * S::NP];
+  } stage[RING];
+
+  template <int V>
+  static __device__ __forceinline__ void fetch(T* to, const T* base, long long at, int c, int D) {
+    constexpr int BYTES = V * static_cast<int>(sizeof(T));
+    if constexpr (VEC && BYTES >= 4) {
+      copy_async<BYTES>(to, c < D ? base + at + c : base, c < D);
+    } else {
+      const Pack<T, V> r = load_row<T, V, VEC>(base + at, c, D);
+      r.store(to);
+    }
+  }
+  // always closes a group, so that the groups count the tiles; nothing is copied past the segment's `end`
+  template <bool WANT_B, bool WANT_C>
+  __device__ __forceinline__ void load(const BdhScanDesc& d, int tile, int end, int b, int c0, int len) {
+    const int lane = threadIdx.x & 31, t = tile * LT + lane / 2, c = c0 + (lane & 1) * S::E, n = (lane & 1) * (S::NP / 2);
+    if (tile >= 0 && tile < end) {
+      Stage& s = stage[tile % RING];
+      const int D = t < len ? d.D : 0, N = t < len ? d.N : 0;
+#pragma unroll
+      for (int i = 0; i < S::NV; ++i) {
+        const int at = lane * S::E + i * S::V;
+        fetch<S::V>(s.u + at, static_cast<const T*>(d.u), b * d.u_sb + t * d.u_st, c + i * S::V, D);
+        fetch<S::V>(s.dt + at, static_cast<const T*>(d.dt), b * d.dt_sb + t * d.dt_st, c + i * S::V, D);
+        if constexpr (DY) fetch<S::V>(s.dy + at, static_cast<const T*>(d.dy), b * d.dy_sb + t * d.dy_st, c + i * S::V, D);
+      }
+#pragma unroll
+      for (int i = 0; i < S::NB; ++i) {
+        const int at = lane * (S::NP / 2) + 4 * i;
+        if constexpr (WANT_B) fetch<4>(s.B + at, static_cast<const T*>(d.B_), b * d.b_sb + t * d.b_st, n + 4 * i, N);
+        if constexpr (WANT_C) fetch<4>(s.C + at, static_cast<const T*>(d.C_), b * d.c_sb + t * d.c_st, n + 4 * i, N);
+      }
+    }
+    copy_close();
+  }
+  struct View {
+    const Stage& s;
+    template <int V>
+    static __device__ __forceinline__ Pack<T, V> get(const T* p) {
+      Pack<T, V> r;
+      r.load(p);
+      return r;
+    }
+    __device__ __forceinline__ int lane() const { return threadIdx.x & 31; }
+    __device__ __forceinline__ Pack<T, S::V> u(int i) const { return get<S::V>(s.u + lane() * S::E + i * S::V); }
+    __device__ __forceinline__ Pack<T, S::V> dt(int i) const { return get<S::V>(s.dt + lane() * S::E + i * S::V); }
+    __device__ __forceinline__ Pack<T, S::V> dy(int i) const { return get<S::V>(s.dy + lane() * S::E + i * S::V); }
+    __device__ __forceinline__ Pack<T, 4> B(int i) const { return get<4>(s.B + lane() * (S::NP / 2) + 4 * i); }
+    __device__ __forceinline__ Pack<T, 4> C(int i) const { return get<4>(s.C + lane() * (S::NP / 2) + 4 * i); }
+  };
+  __device__ __forceinline__ View at(int tile) const { return View{stage[tile % RING]}; }
+};
+
+// What a warp's compute loop reads. Rows are padded by 16 bytes, so that eight lanes that store four rows meet no bank twice.
 template <int G, int CT, bool DY>
 struct alignas(16) WarpMem {
   static constexpr int NP = 4 * G, CW = 32 / G * CT;
@@ -236,60 +327,75 @@ struct alignas(16) WarpMem {
       skip[i] = (d.skip && c0 + i < d.D) ? d.skip[c0 + i] : 0.f;
     }
   }
-  // channels behind D and rows behind `len` get dt' = 0: their states stay as they are
-  template <typename T, bool VEC, bool WANT_B = true, bool WANT_C = true>
-  __device__ __forceinline__ void put(const BdhScanDesc& d, const Tile<T, G, CT, VEC, DY>& x, int c0, int t0, int len) {
+  // Rows behind `len` get dt' = 0: the states stay as they are. (Channels behind D need nothing: their u, dy and A
+  // read as 0.)
+  template <typename T, bool WANT_B, bool WANT_C, typename Source>
+  __device__ __forceinline__ void put(const BdhScanDesc& d, const Source& x, int t0, int len) {
     using S = Shape<T, G, CT>;
     const int lane = threadIdx.x & 31, t = lane / 2, c = (lane & 1) * S::E, n = (lane & 1) * (NP / 2);
-    const int have = t0 + t < len ? d.D - c0 - c : 0;  // of this lane's channels
+    const float keep = t0 + t < len ? 1.f : 0.f;
     float dt[S::E + 1], uu[S::E + 1];
     dt[S::E] = uu[S::E] = 0.f;
 #pragma unroll
-    for (int j = 0; j < S::E; ++j) {
-      dt[j] = x.dt[j / S::V][j % S::V] + bias[c + j];
-      uu[j] = x.u[j / S::V][j % S::V];
+    for (int i = 0; i < S::NV; ++i) {
+      const Pack<T, S::V> pd = x.dt(i), pu = x.u(i);
+#pragma unroll
+      for (int j = 0; j < S::V; ++j) {
+        dt[i * S::V + j] = pd[j] + bias[c + i * S::V + j];
+        uu[i * S::V + j] = pu[j];
+      }
     }
 #pragma unroll
     for (int j = 0; j < S::E; j += 2) {
       f2 s = pack2(dt[j], dt[j + 1]);
       if (d.softplus) s = softplus2(s);
-      float s0, s1;
+      s = mul2(s, both(keep));
+      float s0, s1, v0, v1;
       unpack2(s, s0, s1);
-      s0 = j < have ? s0 : 0.f;
-      s1 = j + 1 < have ? s1 : 0.f;
-      const float v0 = j < have ? s0 * uu[j] : 0.f, v1 = j + 1 < have ? s1 * uu[j + 1] : 0.f;
+      unpack2(mul2(s, pack2(uu[j], uu[j + 1])), v0, v1);
       if constexpr (S::E > 1)
         *reinterpret_cast<float4*>(&step[t][c + j]) = make_float4(s0, v0, s1, v1);
       else
         step[t][c] = make_float2(s0, v0);
     }
-    if constexpr (DY)
+    if constexpr (DY) {
 #pragma unroll
-      for (int j = 0; j < S::E; ++j) dy[t][c + j] = x.dy[j / S::V][j % S::V];
+      for (int i = 0; i < S::NV; ++i) {
+        const Pack<T, S::V> p = x.dy(i);
+#pragma unroll
+        for (int j = 0; j < S::V; ++j) dy[t][c + i * S::V + j] = p[j];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < S::NB; ++i) {
-      if constexpr (WANT_B) *reinterpret_cast<float4*>(&B[t][n + 4 * i]) = make_float4(x.B[i][0], x.B[i][1], x.B[i][2], x.B[i][3]);
-      if constexpr (WANT_C) *reinterpret_cast<float4*>(&C[t][n + 4 * i]) = make_float4(x.C[i][0], x.C[i][1], x.C[i][2], x.C[i][3]);
+      if constexpr (WANT_B) {
+        const Pack<T, 4> p = x.B(i);
+        *reinterpret_cast<float4*>(&B[t][n + 4 * i]) = make_float4(p[0], p[1], p[2], p[3]);
+      }
+      if constexpr (WANT_C) {
+        const Pack<T, 4> p = x.C(i);
+        *reinterpret_cast<float4*>(&C[t][n + 4 * i]) = make_float4(p[0], p[1], p[2], p[3]);
+      }
     }
   }
-  __device__ __forceinline__ void steps(int t, int cl, f2 (&dt)[CT], f2 (&du)[CT]) const {
+  __device__ __forceinline__ void steps(int t, int cl, float (&dt)[CT], float (&du)[CT]) const {
     if constexpr (CT == 2) {
       const float4 v = *reinterpret_cast<const float4*>(&step[t][cl]);
-      dt[0] = both(v.x); du[0] = both(v.y);
-      dt[1] = both(v.z); du[1] = both(v.w);
+      dt[0] = v.x; du[0] = v.y;
+      dt[1] = v.z; du[1] = v.w;
     } else {
       const float2 v = step[t][cl];
-      dt[0] = both(v.x);
-      du[0] = both(v.y);
+      dt[0] = v.x;
+      du[0] = v.y;
     }
   }
-  __device__ __forceinline__ void dys(int t, int cl, f2 (&g)[CT]) const {
+  __device__ __forceinline__ void dys(int t, int cl, float (&g)[CT]) const {
     if constexpr (CT == 2) {
       const float2 v = *reinterpret_cast<const float2*>(&dy[t][cl]);
-      g[0] = both(v.x);
-      g[1] = both(v.y);
+      g[0] = v.x;
+      g[1] = v.y;
     } else {
-      g[0] = both(dy[t][cl]);
+      g[0] = dy[t][cl];
     }
   }
 };
@@ -340,6 +446,31 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
   }
 }
 
+// The factors of a few steps, made ahead of the chain through h: its loads must not stand behind the stores of the steps
+// before, which the compiler cannot tell from them.
+template <int G, int CT, bool DY, bool WANT_C>
+struct Steps {
+  static constexpr int N = 4 / CT;
+  f2 e[N][CT][2], in[N][CT][2], k[WANT_C ? N : 1][2];
+  __device__ __forceinline__ void make(const WarpMem<G, CT, DY>& sh, int t, int cl, int n0, const f2 (&A2)[CT][2]) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      float dt[CT], du[CT];
+      f2 b0, b1;
+      sh.steps(t + s, cl, dt, du);
+      load4(&sh.B[t + s][n0], b0, b1);
+      if constexpr (WANT_C) load4(&sh.C[t + s][n0], k[s][0], k[s][1]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        e[s][c][0] = ex2x2(mul1(dt[c], A2[c][0]));
+        e[s][c][1] = ex2x2(mul1(dt[c], A2[c][1]));
+        in[s][c][0] = mul1(du[c], b0);
+        in[s][c][1] = mul1(du[c], b1);
+      }
+    }
+  }
+};
+
 struct Where {
   int part, b, seg;                    // channels, sequence, segment
 };
@@ -355,79 +486,65 @@ __device__ __forceinline__ Where where(const ScanArgs& a, long long unit) {
 // ---- forward -----------------------------------------------------------------------------------------
 // Each warp on its own. The partial sums over a lane's 4 states go through shared memory: a channel's G lanes are
 // added up where the outputs are written, which costs a store a step instead of a chain of exchanges.
-template <int G, int CT>
-struct FwdMem : WarpMem<G, CT, false> {
+template <typename T, int G, int CT, bool VEC>
+struct FwdMem {
+  WarpMem<G, CT, false> in;
   alignas(16) float part[LT][CT * 32 + 4];
+  Ring<T, G, CT, VEC, false> ring;
 };
 
 template <typename T, int G, int CT, bool VEC>
-__global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_fwd_kernel(const ScanArgs a, long long units, float* marks) {
+__global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd_kernel(const ScanArgs a, long long units, float* marks) {
   using S = Shape<T, G, CT>;
-  __shared__ __align__(16) FwdMem<G, CT> mem[FWD_WARPS];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * FWD_WARPS + (threadIdx.x >> 5);
   if (unit >= units) return;
-  FwdMem<G, CT>& sh = mem[threadIdx.x >> 5];
+  FwdMem<T, G, CT, VEC>& sh = reinterpret_cast<FwdMem<T, G, CT, VEC>*>(smem_raw)[threadIdx.x >> 5];
   const BdhScanDesc& d = a.d;
   const Where w = where(a, unit);
   const int n0 = lane % G * 4, cl = lane / G * CT, c0 = w.part * S::CW, c = c0 + cl;
   const int len = a.len.get(w.b, d.T);
+  const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles), end = min(last, (len + LT - 1) / LT);
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) sh.ring.template load<true, true>(d, first + i, end, w.b, c0, len);
   f2 A2[CT][2], h[CT][2];
   load_a<CT>(d, c, n0, A2);
 #pragma unroll
   for (int k = 0; k < CT; ++k)
     load_state(d.h0 ? d.h0 + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, h[k]);
   carry<CT, S::NP>(a, w.b, 0, w.seg, 1, c, n0, A2, h);
-  sh.params(d, c0);
-  const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles);
-  Tile<T, G, CT, VEC, false> x;
-  x.load(d, w.b, c0, first * LT, len);
+  sh.in.params(d, c0);
   __syncwarp();
   const int row = lane / 2, col = (lane & 1) * S::E;
   for (int tile = first; tile < last; ++tile) {
     const int t0 = tile * LT;
-    const bool any = t0 < len;
-    Pack<T, S::V> u[S::NV];
-#pragma unroll
-    for (int i = 0; i < S::NV; ++i) u[i] = x.u[i];
-    if (any) {
-      sh.put(d, x, c0, t0, len);
+    if (tile < end) {
+      copy_wait();
+      sh.in.template put<T, true, true>(d, sh.ring.at(tile), t0, len);
       __syncwarp();
-      if (tile + 1 < last) x.load(d, w.b, c0, t0 + LT, len);
+      sh.ring.template load<true, true>(d, tile + RING - 1, end, w.b, c0, len);
       if (marks != nullptr)
 #pragma unroll
         for (int k = 0; k < CT; ++k)
           if (c + k < d.D)
             *reinterpret_cast<ulonglong2*>(marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0) =
                 make_ulonglong2(h[k][0], h[k][1]);
-      constexpr int GS = 8 / CT;                       // the exponentials of a group of steps ahead of the chain through h
+      using Group = Steps<G, CT, false, true>;
+      Group now, next;
+      now.make(sh.in, 0, cl, n0, A2);
 #pragma unroll
-      for (int s0 = 0; s0 < LT; s0 += GS) {
-        f2 e[GS][CT][2], in[GS][CT][2];
+      for (int s0 = 0; s0 < LT; s0 += Group::N) {
+        if (s0 + Group::N < LT) next.make(sh.in, s0 + Group::N, cl, n0, A2);
 #pragma unroll
-        for (int s = 0; s < GS; ++s) {
-          f2 dt[CT], du[CT], b0, b1;
-          sh.steps(s0 + s, cl, dt, du);
-          load4(&sh.B[s0 + s][n0], b0, b1);
-#pragma unroll
-          for (int k = 0; k < CT; ++k) {
-            e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
-            e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
-            in[s][k][0] = mul2(du[k], b0);
-            in[s][k][1] = mul2(du[k], b1);
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < GS; ++s) {
-          f2 k0, k1;
-          load4(&sh.C[s0 + s][n0], k0, k1);
+        for (int s = 0; s < Group::N; ++s)
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
-            h[k][0] = fma2(e[s][k][0], h[k][0], in[s][k][0]);
-            h[k][1] = fma2(e[s][k][1], h[k][1], in[s][k][1]);
-            sh.part[s0 + s][k * 32 + lane] = sum2(fma2(k1, h[k][1], mul2(k0, h[k][0])));
+            h[k][0] = fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]);
+            h[k][1] = fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]);
+            sh.part[s0 + s][k * 32 + lane] = sum2(fma2(now.k[s][1], h[k][1], mul2(now.k[s][0], h[k][0])));
           }
-        }
+        now = next;
       }
       __syncwarp();
     }
@@ -436,7 +553,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_fwd_kernel(cons
       const bool in = t0 + row < len;
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
-        Pack<T, S::V> o;
+        Pack<T, S::V> o, u = sh.ring.at(tile).u(i);
 #pragma unroll
         for (int j = 0; j < S::V; ++j) {
           const int cc = col + i * S::V + j;
@@ -453,7 +570,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_fwd_kernel(cons
                 v += (q.x + q.y) + (q.z + q.w);
               }
             }
-            v = fmaf(sh.skip[cc], u[i][j], v);
+            v = fmaf(sh.in.skip[cc], u[j], v);
           }
           o.set(j, v);
         }
@@ -469,32 +586,45 @@ __global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_fwd_kernel(cons
 // States of the segments from zero: h_t = a_t h_{t-1} + dt' u B_t, or in reverse r_t = a_t (r_{t+1} + dy_t C_t); and the
 // sum of the segment's steps. Each warp on its own.
 template <typename T, int G, int CT, bool VEC, bool REV>
-__global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_sweep_kernel(const ScanArgs a, long long units, float* seg_state, float* seg_dt) {
+struct SweepMem {
+  WarpMem<G, CT, REV> in;
+  Ring<T, G, CT, VEC, REV> ring;
+};
+
+template <typename T, int G, int CT, bool VEC, bool REV>
+__global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_sweep_kernel(const ScanArgs a, long long units, float* seg_state, float* seg_dt) {
   using S = Shape<T, G, CT>;
-  __shared__ __align__(16) WarpMem<G, CT, REV> mem[FWD_WARPS];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * FWD_WARPS + (threadIdx.x >> 5);
   if (unit >= units) return;
-  WarpMem<G, CT, REV>& sh = mem[threadIdx.x >> 5];
+  SweepMem<T, G, CT, VEC, REV>& sh = reinterpret_cast<SweepMem<T, G, CT, VEC, REV>*>(smem_raw)[threadIdx.x >> 5];
   const BdhScanDesc& d = a.d;
   const Where w = where(a, unit);
   const int n0 = lane % G * 4, cl = lane / G * CT, c0 = w.part * S::CW, c = c0 + cl;
   const int len = a.len.get(w.b, d.T);
-  f2 A2[CT][2], h[CT][2], total = both(0.f);
-  load_a<CT>(d, c, n0, A2);
-#pragma unroll
-  for (int k = 0; k < CT; ++k) h[k][0] = h[k][1] = both(0.f);
-  sh.params(d, c0);
   const int first = w.seg * a.per_seg, end = min(min(first + a.per_seg, a.tiles), (len + LT - 1) / LT);
   const int n = end - first;
-  Tile<T, G, CT, VEC, REV> x;
-  if (n > 0) x.template load<!REV, REV>(d, w.b, c0, (REV ? end - 1 : first) * LT, len);
+  // the i-th tile of the walk; the copies run ahead in the same order
+  const auto tile_of = [&](int i) { return REV ? end - 1 - i : first + i; };
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) sh.ring.template load<!REV, REV>(d, i < n ? tile_of(i) : -1, end, w.b, c0, len);
+  f2 A2[CT][2], h[CT][2];
+  float total[CT];
+  load_a<CT>(d, c, n0, A2);
+#pragma unroll
+  for (int k = 0; k < CT; ++k) {
+    h[k][0] = h[k][1] = both(0.f);
+    total[k] = 0.f;
+  }
+  sh.in.params(d, c0);
   __syncwarp();
   for (int i = 0; i < n; ++i) {
-    const int t0 = (REV ? end - 1 - i : first + i) * LT;
-    sh.template put<T, VEC, !REV, REV>(d, x, c0, t0, len);
+    const int tile = tile_of(i);
+    copy_wait();
+    sh.in.template put<T, !REV, REV>(d, sh.ring.at(tile), tile * LT, len);
     __syncwarp();
-    if (i + 1 < n) x.template load<!REV, REV>(d, w.b, c0, REV ? t0 - LT : t0 + LT, len);
+    sh.ring.template load<!REV, REV>(d, i + RING - 1 < n ? tile_of(i + RING - 1) : -1, end, w.b, c0, len);
     constexpr int GS = 8 / CT;
 #pragma unroll
     for (int s0 = 0; s0 < LT; s0 += GS) {
@@ -502,26 +632,19 @@ __global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_sweep_kernel(co
 #pragma unroll
       for (int s = 0; s < GS; ++s) {
         const int t = REV ? LT - 1 - s0 - s : s0 + s;
-        f2 dt[CT], du[CT], b0, b1;
-        sh.steps(t, cl, dt, du);
-        load4(REV ? &sh.C[t][n0] : &sh.B[t][n0], b0, b1);
-        if constexpr (REV) sh.dys(t, cl, du);
+        float dt[CT], du[CT];
+        f2 b0, b1;
+        sh.in.steps(t, cl, dt, du);
+        load4(REV ? &sh.in.C[t][n0] : &sh.in.B[t][n0], b0, b1);
+        if constexpr (REV) sh.in.dys(t, cl, du);
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
-          e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
-          e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
-          in[s][k][0] = mul2(du[k], b0);
-          in[s][k][1] = mul2(du[k], b1);
+          e[s][k][0] = ex2x2(mul1(dt[k], A2[k][0]));
+          e[s][k][1] = ex2x2(mul1(dt[k], A2[k][1]));
+          in[s][k][0] = mul1(du[k], b0);
+          in[s][k][1] = mul1(du[k], b1);
+          total[k] += dt[k];
         }
-        float p, q;
-        if constexpr (CT == 2) {
-          float r;
-          unpack2(dt[0], p, r);
-          unpack2(dt[1], q, r);
-        } else {
-          unpack2(dt[0], p, q);
-        }
-        total = add2(total, pack2(p, q));
       }
 #pragma unroll
       for (int s = 0; s < GS; ++s)
@@ -533,14 +656,12 @@ __global__ void __launch_bounds__(32 * FWD_WARPS) selective_scan_sweep_kernel(co
     }
     __syncwarp();
   }
-  float sums[2];
-  unpack2(total, sums[0], sums[1]);
 #pragma unroll
   for (int k = 0; k < CT; ++k)
     if (c + k < d.D) {
       const long long at = (static_cast<long long>(w.b) * a.segs + w.seg) * d.D + c + k;
       *reinterpret_cast<ulonglong2*>(seg_state + at * S::NP + n0) = make_ulonglong2(h[k][0], h[k][1]);
-      if (n0 == 0) seg_dt[at] = sums[k];
+      if (n0 == 0) seg_dt[at] = total[k];
     }
 }
 
@@ -563,8 +684,24 @@ struct BwdMem {
   alignas(16) float bc[BWD_WARPS][LT][2 * NP];     // the warps' sums over their channels
 };
 
+// What a step of the reverse walk reads
+template <int G, int CT>
+struct BwdStep {
+  float dt[CT], du[CT], gy[CT];
+  f2 b[2], c[2];
+  ulonglong2 h[CT];
+  __device__ __forceinline__ void load(const typename BwdMem<G, CT>::PerWarp& sh, int t, int lane, int cl, int n0) {
+    sh.in.steps(t, cl, dt, du);
+    sh.in.dys(t, cl, gy);
+    load4(&sh.in.B[t][n0], b[0], b[1]);
+    load4(&sh.in.C[t][n0], c[0], c[1]);
+#pragma unroll
+    for (int k = 0; k < CT; ++k) h[k] = sh.h[t][k][lane];
+  }
+};
+
 template <typename T, int G, int CT, bool VEC>
-__global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(const ScanArgs a, const ScanGrads o) {
+__global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd_kernel(const ScanArgs a, const ScanGrads o) {
   using S = Shape<T, G, CT>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   BwdMem<G, CT>& all = *reinterpret_cast<BwdMem<G, CT>*>(smem_raw);
@@ -590,6 +727,16 @@ __global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(cons
   const int row = lane / 2, col = (lane & 1) * S::E;
   Tile<T, G, CT, VEC, true> x;
   x.load(d, w.b, c0, (last - 1) * LT, len);
+  f2 mark[CT][2];                                      // the next tile's first state, fetched with its rows
+  const auto load_marks = [&](int tile) {
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+      mark[k][0] = mark[k][1] = both(0.f);
+      if (c + k < d.D && tile * LT < len)
+        load4(o.marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0, mark[k][0], mark[k][1]);
+    }
+  };
+  load_marks(last - 1);
   __syncwarp();
   for (int tile = last - 1; tile >= first; --tile) {
     const int t0 = tile * LT;
@@ -597,75 +744,68 @@ __global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(cons
     Pack<T, S::V> u[S::NV], dt_raw[S::NV], dy[S::NV];
 #pragma unroll
     for (int i = 0; i < S::NV; ++i) {
-      u[i] = x.u[i];
-      dt_raw[i] = x.dt[i];
-      dy[i] = x.dy[i];
+      u[i] = x.u(i);
+      dt_raw[i] = x.dt(i);
+      dy[i] = x.dy(i);
     }
     if (any) {
       f2 h[CT][2], dat[CT][2];
-      sh.in.put(d, x, c0, t0, len);
+      sh.in.template put<T, true, true>(d, x, t0, len);
 #pragma unroll
       for (int k = 0; k < CT; ++k) {
-        h[k][0] = h[k][1] = dat[k][0] = dat[k][1] = both(0.f);
-        if (c + k < d.D)
-          load4(o.marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0, h[k][0], h[k][1]);
+        h[k][0] = mark[k][0];
+        h[k][1] = mark[k][1];
+        dat[k][0] = dat[k][1] = both(0.f);
       }
       __syncwarp();
-      if (tile > first) x.load(d, w.b, c0, t0 - LT, len);
-      constexpr int GS = 8 / CT;
+      if (tile > first) {
+        x.load(d, w.b, c0, t0 - LT, len);
+        load_marks(tile - 1);
+      }
+      using Group = Steps<G, CT, true, false>;
+      Group now, next;
+      now.make(sh.in, 0, cl, n0, A2);
 #pragma unroll
-      for (int s0 = 0; s0 < LT; s0 += GS) {
-        f2 e[GS][CT][2], in[GS][CT][2];
+      for (int s0 = 0; s0 < LT; s0 += Group::N) {
+        if (s0 + Group::N < LT) next.make(sh.in, s0 + Group::N, cl, n0, A2);
 #pragma unroll
-        for (int s = 0; s < GS; ++s) {
-          f2 dt[CT], du[CT], b0, b1;
-          sh.in.steps(s0 + s, cl, dt, du);
-          load4(&sh.in.B[s0 + s][n0], b0, b1);
-#pragma unroll
-          for (int k = 0; k < CT; ++k) {
-            e[s][k][0] = ex2x2(mul2(dt[k], A2[k][0]));
-            e[s][k][1] = ex2x2(mul2(dt[k], A2[k][1]));
-            in[s][k][0] = mul2(du[k], b0);
-            in[s][k][1] = mul2(du[k], b1);
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < GS; ++s)
+        for (int s = 0; s < Group::N; ++s)
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
             sh.h[s0 + s][k][lane] = make_ulonglong2(h[k][0], h[k][1]);
-            h[k][0] = fma2(e[s][k][0], h[k][0], in[s][k][0]);
-            h[k][1] = fma2(e[s][k][1], h[k][1], in[s][k][1]);
+            h[k][0] = fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]);
+            h[k][1] = fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]);
           }
+        now = next;
       }
+      BwdStep<G, CT> at_t, before;
+      at_t.load(sh, LT - 1, lane, cl, n0);
 #pragma unroll 4
       for (int t = LT - 1; t >= 0; --t) {
-        f2 dt[CT], du[CT], gy[CT], b0, b1, k0, k1, sb0, sb1, sc0, sc1;
-        sh.in.steps(t, cl, dt, du);
-        sh.in.dys(t, cl, gy);
-        load4(&sh.in.B[t][n0], b0, b1);
-        load4(&sh.in.C[t][n0], k0, k1);
+        before.load(sh, t > 0 ? t - 1 : 0, lane, cl, n0);              // ahead of this step's stores
+        f2 sb0, sb1, sc0, sc1;
         float nv[2 * CT];
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
-          const f2 g0 = fma2(gy[k], k0, r[k][0]), g1 = fma2(gy[k], k1, r[k][1]);
-          const ulonglong2 hp = sh.h[t][k][lane];
+          const float dt = at_t.dt[k], du = at_t.du[k], gy = at_t.gy[k];
+          const f2 g0 = fma1(gy, at_t.c[0], r[k][0]), g1 = fma1(gy, at_t.c[1], r[k][1]);
+          const f2 e0 = ex2x2(mul1(dt, A2[k][0])), e1 = ex2x2(mul1(dt, A2[k][1]));
           if (k == 0) {
-            sb0 = mul2(g0, du[k]); sb1 = mul2(g1, du[k]);
-            sc0 = mul2(gy[k], h[k][0]); sc1 = mul2(gy[k], h[k][1]);
+            sb0 = mul1(du, g0); sb1 = mul1(du, g1);
+            sc0 = mul1(gy, h[k][0]); sc1 = mul1(gy, h[k][1]);
           } else {
-            sb0 = fma2(g0, du[k], sb0); sb1 = fma2(g1, du[k], sb1);
-            sc0 = fma2(gy[k], h[k][0], sc0); sc1 = fma2(gy[k], h[k][1], sc1);
+            sb0 = fma1(du, g0, sb0); sb1 = fma1(du, g1, sb1);
+            sc0 = fma1(gy, h[k][0], sc0); sc1 = fma1(gy, h[k][1], sc1);
           }
-          r[k][0] = mul2(ex2x2(mul2(dt[k], A2[k][0])), g0);
-          r[k][1] = mul2(ex2x2(mul2(dt[k], A2[k][1])), g1);
-          const f2 q0 = mul2(r[k][0], hp.x), q1 = mul2(r[k][1], hp.y);
-          dat[k][0] = fma2(dt[k], q0, dat[k][0]);
-          dat[k][1] = fma2(dt[k], q1, dat[k][1]);
-          nv[2 * k] = sum2(fma2(g1, b1, mul2(g0, b0)));
+          r[k][0] = mul2(e0, g0);
+          r[k][1] = mul2(e1, g1);
+          h[k][0] = at_t.h[k].x;
+          h[k][1] = at_t.h[k].y;
+          const f2 q0 = mul2(r[k][0], h[k][0]), q1 = mul2(r[k][1], h[k][1]);
+          dat[k][0] = fma1(dt, q0, dat[k][0]);
+          dat[k][1] = fma1(dt, q1, dat[k][1]);
+          nv[2 * k] = sum2(fma2(g1, at_t.b[1], mul2(g0, at_t.b[0])));
           nv[2 * k + 1] = sum2(fma2(A2[k][1], q1, mul2(A2[k][0], q0)));
-          h[k][0] = hp.x;
-          h[k][1] = hp.y;
         }
         int at;
         bool once;
@@ -684,6 +824,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(cons
         if (once)
 #pragma unroll
           for (int i = 0; i < CLEFT; ++i) all.bc[warp][t][(at + i) / 4 * S::NP + n0 + (at + i) % 4] = cv[i];
+        at_t = before;
       }
 #pragma unroll
       for (int k = 0; k < CT; ++k) {                   // sums of tiles: a chain of 16, then one of the tiles
@@ -692,6 +833,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS) selective_scan_bwd_kernel(cons
       }
     } else if (tile > first) {
       x.load(d, w.b, c0, t0 - LT, len);
+      load_marks(tile - 1);
     }
     __syncthreads();
     if (t0 + row < d.T) {
@@ -884,18 +1026,19 @@ Plan plan(const BdhScanDesc& d, int CT, int warps, long long segs) {
 constexpr int MOST_SEGS = 64;          // so that combining the segments stays cheap beside them
 
 // One or two channels a lane (two: fewer reads of B and C a channel; one: twice the warps), and how many segments
-// (which cost the exponentials a second time): the smaller of the times that a tile takes a warp on its own and a
-// scheduler (592 of them) that is kept busy, in clocks.
+// (which cost the exponentials a second time), by a model of the time of a tile: what a warp alone on its scheduler
+// takes and what a busy scheduler (592 of them) takes for one, joined as the root of the sum of squares; and what the
+// segments before each segment cost it, which grows with their number squared.
+// Measured for 16 states (clocks): one channel 1890 and 1355, two 2640 and 1885; a sweep is 0.76 of a pass.
 Plan fwd_plan(const BdhScanDesc& d) {
   Plan best = plan(d, 2, 1, 1);
   double least = 0;
   for (int CT = 1; CT <= 2; ++CT)
     for (int segs = 1; segs <= MOST_SEGS; segs += segs < 8 ? 1 : 4) {
       const Plan p = plan(d, CT, 1, segs);
-      const double alone = CT == 2 ? 1900 : 1300, busy = CT == 2 ? 1150 : 650;
-      const double per_scheduler = static_cast<double>(d.B) * p.segs * p.parts / 592;
-      const double tile = alone > busy * per_scheduler ? alone : busy * per_scheduler;
-      const double t = p.per_seg * tile * (p.segs > 1 ? 1.7 : 1) + (p.segs > 1 ? 6000 + 40.0 * p.segs : 0);
+      const double alone = CT == 2 ? 2640 : 1890, busy = (CT == 2 ? 1885 : 1355) * (static_cast<double>(d.B) * p.segs * p.parts / 592);
+      const double carry = 5000 + 150.0 * p.segs + 55.0 * p.segs * p.segs * d.B * p.parts / 592;
+      const double t = p.per_seg * sqrt(alone * alone + busy * busy) * (p.segs > 1 ? 1.76 : 1) + (p.segs > 1 ? carry : 0);
       if (least == 0 || t < least) {
         least = t;
         best = p;
@@ -904,7 +1047,8 @@ Plan fwd_plan(const BdhScanDesc& d) {
   return best;
 }
 
-// Two blocks fit an SM: whole rounds of 296, with segments as long as that leaves them.
+// Two blocks fit an SM, so blocks run in rounds of 296 (one alone on its SM takes 0.7 of the time of two); a sweep, which
+// segments need, is a quarter of the pass.
 Plan bwd_plan(const BdhScanDesc& d) {
   Plan best = plan(d, 2, BWD_WARPS, 1);
   double least = 0;
@@ -912,7 +1056,8 @@ Plan bwd_plan(const BdhScanDesc& d) {
     const Plan p = plan(d, 2, BWD_WARPS, segs);
     const long long blocks = static_cast<long long>(d.B) * p.segs * p.parts;
     const double rounds = blocks <= 148 ? 0.7 : static_cast<double>((blocks + 295) / 296);
-    const double t = rounds * (p.per_seg + 1) * (p.segs > 1 ? 1.3 : 1) + (p.segs > 1 ? 2 : 0);
+    const double carry = 1 + 0.042 * p.segs * p.segs * d.B * p.parts / 296;
+    const double t = rounds * (p.per_seg + 0.5) * (p.segs > 1 ? 1.25 : 1) + (p.segs > 1 ? carry : 0);
     if (least == 0 || t < least) {
       least = t;
       best = p;
@@ -955,6 +1100,13 @@ bool packs_fit(const BdhScanDesc& d, int size) {
 
 int launched() { return cudaGetLastError() == cudaSuccess ? BDH_OK : BDH_ERR_LAUNCH; }
 
+template <typename K>
+int allow_smem(PerDeviceOnce& once, K kernel, int bytes) {
+  return once.run([&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? BDH_OK : BDH_ERR_LAUNCH;
+  });
+}
+
 template <typename T, int G, int CT, bool VEC, bool REV>
 int sweep_launch(const ScanArgs& a, const Plan& p, float* seg, cudaStream_t s) {
   // (a sweep's warps: those of the pass that it serves, whose segments it shares)
@@ -962,7 +1114,11 @@ int sweep_launch(const ScanArgs& a, const Plan& p, float* seg, cudaStream_t s) {
   sw.parts = (a.d.D + Shape<T, G, CT>::CW - 1) / Shape<T, G, CT>::CW;
   const long long units = static_cast<long long>(a.d.B) * p.segs * sw.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
-  selective_scan_sweep_kernel<T, G, CT, VEC, REV><<<static_cast<unsigned>(grid), 32 * FWD_WARPS, 0, s>>>(sw, units, seg, const_cast<float*>(a.seg_dt));
+  auto kernel = selective_scan_sweep_kernel<T, G, CT, VEC, REV>;
+  constexpr int smem = FWD_WARPS * sizeof(SweepMem<T, G, CT, VEC, REV>);
+  static PerDeviceOnce once;
+  if (const int rc = allow_smem(once, kernel, smem)) return rc;
+  kernel<<<static_cast<unsigned>(grid), 32 * FWD_WARPS, smem, s>>>(sw, units, seg, const_cast<float*>(a.seg_dt));
   return launched();
 }
 
@@ -973,7 +1129,11 @@ int fwd_launch(const BdhScanDesc& d, const Plan& p, float* marks, float* seg, cu
     if (const int rc = sweep_launch<T, G, CT, VEC, false>(a, p, seg, s)) return rc;
   const long long units = static_cast<long long>(d.B) * p.segs * p.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
-  selective_scan_fwd_kernel<T, G, CT, VEC><<<static_cast<unsigned>(grid), 32 * FWD_WARPS, 0, s>>>(a, units, marks);
+  auto kernel = selective_scan_fwd_kernel<T, G, CT, VEC>;
+  constexpr int smem = FWD_WARPS * sizeof(FwdMem<T, G, CT, VEC>);
+  static PerDeviceOnce once;
+  if (const int rc = allow_smem(once, kernel, smem)) return rc;
+  kernel<<<static_cast<unsigned>(grid), 32 * FWD_WARPS, smem, s>>>(a, units, marks);
   return launched();
 }
 
@@ -993,8 +1153,7 @@ int bwd_launch(const BdhScanDesc& d, const Plan& p, const ScanGrads& o, float* s
   auto kernel = selective_scan_bwd_kernel<T, G, CT, VEC>;
   constexpr int smem = sizeof(BwdMem<G, CT>);
   static PerDeviceOnce once;
-  if (once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess ? 0 : 1; }))
-    return BDH_ERR_LAUNCH;
+  if (const int rc = allow_smem(once, kernel, smem)) return rc;
   kernel<<<static_cast<unsigned>(grid), 32 * BWD_WARPS, smem, s>>>(a, o);
   if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
   const int NP = 4 * G;
