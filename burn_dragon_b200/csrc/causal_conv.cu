@@ -10,12 +10,11 @@
 // in registers over every tile that a block walks, then over the block, then over the blocks in a fixed order (no
 // atomics: two runs give the same bits).
 #include "bdh_kernels.h"
-#include "element_io.cuh"
+#include "pair_math.cuh"
 
 namespace bdh {
 namespace {
 
-constexpr int ROWS = 4;              // rows of x in flight per thread
 constexpr int FWD_THREADS = 128;
 constexpr int BWD_LANES = 32;        // backward block: 32 channel packs x 4 tiles
 constexpr int BWD_TILES = 4;
@@ -27,25 +26,99 @@ struct ConvArgs {
   int tile, tiles;    // rows per tile, tiles per sequence
 };
 
-// Row r of [state | x] (r counts from the first row of x; negative: the state), V channels from c on.
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_seq(const BdhConvDesc& d, int b, int r, int len, int c) {
+// Row r of [state | x] (r counts from the first row of x; negative: the state), V channels from c on, as it lies in
+// memory. INSIDE: the row is one of x's for certain.
+template <typename T, int V, bool INSIDE>
+__device__ __forceinline__ typename Pack<T, V>::Raw load_seq(const BdhConvDesc& d, int b, int r, int len, int c) {
   Pack<T, V> p;
-  if (r >= 0 && r < len) {
-    p.load(static_cast<const T*>(d.x) + b * d.x_sb + r * d.x_st + c);
+  if (INSIDE || (r >= 0 && r < len)) {
+    return *reinterpret_cast<const typename Pack<T, V>::Raw*>(static_cast<const T*>(d.x) + b * d.x_sb + r * d.x_st + c);
   } else if (r < 0 && r + d.k - 1 >= 0 && d.state != nullptr) {
     p.load(static_cast<const T*>(d.state) + b * d.state_sb + (r + d.k - 1) * d.state_sr + c);
   } else {
     p.zero();
   }
-  return p;
+  return *reinterpret_cast<const typename Pack<T, V>::Raw*>(&p);
+}
+// K: the kernel width, or 0 for a width of up to 8 known at run time (taps then sit at the end of the window; the leading
+// ones are skipped, not multiplied by zero: a row there may hold anything). R: rows that a thread works on at once; with
+// the R rows before them they hold every window, and the two sets change places instead of moving.
+template <int V, int K>
+struct Taps {
+  static constexpr int KM = K ? K : 8, R = K ? 4 : 8, N = (V + 1) / 2;
+  static_assert(KM - 1 <= R, "a window lies within two sets of rows");
+  f2 w[KM][N], bias[N];
+  __device__ __forceinline__ void load(const BdhConvDesc& d, int k, int c, bool live) {
+    const auto one = [&](int j, int v) { return (live && v < V && j >= KM - k) ? d.w[static_cast<long long>(c + v) * k + j - (KM - k)] : 0.f; };
+    const auto off = [&](int v) { return (live && v < V && d.bias) ? d.bias[c + v] : 0.f; };
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int j = 0; j < KM; ++j) w[j][n] = pack2(one(j, 2 * n), one(j, 2 * n + 1));
+      bias[n] = pack2(off(2 * n), off(2 * n + 1));
+    }
+  }
+  __device__ __forceinline__ f2 pre(const f2 (&before)[R][N], const f2 (&s)[R][N], int r, int n, int k) const {
+    f2 x = bias[n];
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+      if (K || j >= KM - k) x = fma2(w[j][n], at(before, s, r - (KM - 1) + j, n), x);
+    return x;
+  }
+  static __device__ __forceinline__ f2 at(const f2 (&before)[R][N], const f2 (&s)[R][N], int row, int n) {
+    return row < 0 ? before[row < 0 ? row + R : 0][n] : s[row < 0 ? 0 : row][n];
+  }
+};
+
+// Rows t0 .. t1 of one sequence. The next rows are on their way (as raw bits: taking the elements out behind the load
+// would wait for it) while the present ones are worked on. INSIDE: every row that is read is one of x's, t1 - t0 is a
+// multiple of R.
+template <typename T, int V, int K, bool INSIDE>
+__device__ __forceinline__ void conv_fwd_tile(const BdhConvDesc& d, const Taps<V, K>& w, int b, int t0, int t1, int len, int c) {
+  using W = Taps<V, K>;
+  constexpr int R = W::R, N = W::N;
+  using Raw = typename Pack<T, V>::Raw;
+  const int k = K ? K : d.k;
+  f2 one[R][N], two[R][N];
+  Raw next[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) next[r] = load_seq<T, V, INSIDE>(d, b, t0 + r, min(len, t1), c);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r <= R - W::KM) continue;                                            // (not in any window)
+    Pairs<T, V>::get(load_seq<T, V, INSIDE>(d, b, t0 - R + r, len, c), one[r]);
+  }
+  T* y = static_cast<T*>(d.y) + (static_cast<long long>(b) * d.T + t0) * d.C + c;
+  const auto rows = [&](int t, const f2 (&before)[R][N], f2 (&s)[R][N]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) Pairs<T, V>::get(next[r], s[r]);
+    if (t + R < t1)
+#pragma unroll
+      for (int r = 0; r < R; ++r) next[r] = load_seq<T, V, INSIDE>(d, b, t + R + r, min(len, t1), c);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!INSIDE && t + r >= t1) break;
+      f2 o[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        o[n] = w.pre(before, s, r, n, k);
+        if (d.silu) o[n] = mul2(o[n], sigmoid_quick2(o[n]));
+        if (!INSIDE && t + r >= len) o[n] = both(0.f);
+      }
+      *reinterpret_cast<Raw*>(y) = Pairs<T, V>::put(o);
+      y += d.C;
+    }
+  };
+#pragma unroll 1
+  for (int t = t0; t < t1; t += 2 * R) {
+    rows(t, one, two);
+    if (t + R < t1) rows(t + R, two, one);
+  }
 }
 
-// K: the kernel width, or 0 for a width of up to 8 known at run time (taps then sit at the end of the window; the
-// leading ones are skipped, not multiplied by zero: a row there may hold anything).
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(FWD_THREADS) causal_conv_fwd_kernel(const ConvArgs a) {
-  constexpr int KM = K ? K : 8;
+  using W = Taps<V, K>;
   const BdhConvDesc& d = a.d;
   const int k = K ? K : d.k;
   const long long i = static_cast<long long>(blockIdx.x) * FWD_THREADS + threadIdx.x;
@@ -58,76 +131,141 @@ __global__ void __launch_bounds__(FWD_THREADS) causal_conv_fwd_kernel(const Conv
   if (tile == a.tiles) {
     if (d.state_out != nullptr)
       for (int j = 0; j < k - 1; ++j)
-        load_seq<T, V>(d, b, len - (k - 1) + j, len, c)
-            .store(static_cast<T*>(d.state_out) + b * d.state_out_sb + j * d.state_out_sr + c);
+        *reinterpret_cast<typename Pack<T, V>::Raw*>(static_cast<T*>(d.state_out) + b * d.state_out_sb + j * d.state_out_sr + c) =
+            load_seq<T, V, false>(d, b, len - (k - 1) + j, len, c);
     return;
   }
-  float w[KM][V], bias[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int j = 0; j < KM; ++j) w[j][v] = (j >= KM - k) ? d.w[static_cast<long long>(c + v) * k + j - (KM - k)] : 0.f;
-    bias[v] = d.bias ? d.bias[c + v] : 0.f;
-  }
+  W w;
+  w.load(d, k, c, true);
   const int t0 = tile * a.tile, t1 = min(t0 + a.tile, d.T);
-  float s[KM - 1 + ROWS][V];
+  if (t0 >= W::R && t1 <= len && (t1 - t0) % W::R == 0)
+    conv_fwd_tile<T, V, K, true>(d, w, b, t0, t1, len, c);
+  else
+    conv_fwd_tile<T, V, K, false>(d, w, b, t0, t1, len, c);
+}
+
+// Gradients of rows t0 .. t1: dx (and d state) need d pre of these rows and of the k - 1 behind them, which the thread
+// computes too. INSIDE: every row of x and dy that is read exists, and no row is one of the new state's. sw, sb: the
+// thread's sums for w and bias.
+template <typename T, int V, int K, bool INSIDE>
+__device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V, K>& w, f2 (&sw)[Taps<V, K>::KM][Taps<V, K>::N],
+                                              f2 (&sb)[Taps<V, K>::N], int b, int t0, int t1, int len, int c) {
+  using W = Taps<V, K>;
+  constexpr int KM = W::KM, R = W::R, N = W::N;
+  using Raw = typename Pack<T, V>::Raw;
+  const int k = K ? K : d.k;
+  const int first = (!INSIDE && t0 == 0 && d.dstate != nullptr) ? -(k - 1) : t0;      // first row whose gradient this tile writes
+  const auto load_dy = [&](int r) {
+    if (INSIDE || (r < len && r < t1 + k - 1))
+      return *reinterpret_cast<const Raw*>(static_cast<const T*>(d.dy) + b * d.dy_sb + r * d.dy_st + c);
+    Pack<T, V> p;
+    p.zero();
+    return *reinterpret_cast<const Raw*>(&p);
+  };
+  f2 s1[R][N], s2[R][N], g1[R][N], g2[R][N];
+  Raw nx[R], nd[R];
 #pragma unroll
-  for (int j = 0; j < KM - 1; ++j) {
-    const Pack<T, V> p = load_seq<T, V>(d, b, t0 - (KM - 1) + j, len, c);
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[j][v] = p[v];
+  for (int r = 0; r < R; ++r) {
+    nx[r] = load_seq<T, V, INSIDE>(d, b, t0 + r, len, c);
+    nd[r] = load_dy(t0 + r);
   }
-  T* y = static_cast<T*>(d.y) + (static_cast<long long>(b) * d.T) * d.C + c;
-  for (int t = t0; t < t1; t += ROWS) {
-    Pack<T, V> p[ROWS];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) p[r] = load_seq<T, V>(d, b, t + r, min(len, t1), c);
+  for (int r = 0; r < R; ++r) {
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int n = 0; n < N; ++n) g1[r][n] = both(0.f);
+    if (r <= R - KM) continue;
+    Pairs<T, V>::get(load_seq<T, V, INSIDE>(d, b, t0 - R + r, len, c), s1[r]);
+  }
+  // d pre of row t + r - (tap of j): K known at compile time, or found among the (at most 8) rows behind
+  const auto back = [&](const f2 (&gp)[R][N], const f2 (&g)[R][N], int r, int j, int n) {
+    if constexpr (K != 0) {
+      return W::at(gp, g, r - j, n);
+    } else {
+      f2 x = both(0.f);
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[KM - 1 + r][v] = p[r][v];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      if (t + r >= t1) break;
-      Pack<T, V> o;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float pre = bias[v];
-#pragma unroll
-        for (int j = 0; j < KM; ++j)
-          if (K || j >= KM - k) pre = fmaf(w[j][v], s[r + j][v], pre);
-        if (d.silu) pre *= sigmoid_f32(pre);
-        o.set(v, t + r < len ? pre : 0.f);
-      }
-      o.store(y + static_cast<long long>(t + r) * d.C);
+      for (int i = 0; i < KM; ++i)
+        if (i == j - (KM - k)) x = W::at(gp, g, r - i, n);
+      return x;
     }
+  };
+  const auto rows = [&](int t, const f2 (&sp)[R][N], f2 (&s)[R][N], const f2 (&gp)[R][N], f2 (&g)[R][N]) {
 #pragma unroll
-    for (int j = 0; j < KM - 1; ++j)
+    for (int r = 0; r < R; ++r) {
+      Pairs<T, V>::get(nx[r], s[r]);
+      Pairs<T, V>::get(nd[r], g[r]);                                         // dy for now
+    }
+    if (t + R < t1 + k - 1)
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[j][v] = s[j + ROWS][v];
+      for (int r = 0; r < R; ++r) {
+        nx[r] = load_seq<T, V, INSIDE>(d, b, t + R + r, len, c);
+        nd[r] = load_dy(t + R + r);
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool in = INSIDE || t + r < len;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (d.silu) {                                                        // silu' = sg (1 + pre (1 - sg))
+          const f2 pre = w.pre(sp, s, r, n, k), sg = sigmoid_quick2(pre);
+          g[r][n] = mul2(g[r][n], mul2(sg, fma2(pre, fma2(sg, both(-1.f), both(1.f)), both(1.f))));
+        }
+        if (!in) g[r][n] = both(0.f);
+        if (t + r < t1 && in) {
+          sb[n] = add2(sb[n], g[r][n]);
+#pragma unroll
+          for (int j = 0; j < KM; ++j)
+            if (K || j >= KM - k) sw[j][n] = fma2(g[r][n], W::at(sp, s, r - (KM - 1) + j, n), sw[j][n]);
+        }
+      }
+      const int row = t + r - (k - 1);                                       // complete now: every d pre it feeds is known
+      if (row >= first && row < t1) {
+        f2 o[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          o[n] = both(0.f);
+#pragma unroll
+          for (int j = 0; j < KM; ++j)                                       // tap j of output row + (k - 1) - j
+            if (K || j >= KM - k) o[n] = fma2(w.w[j][n], back(gp, g, r, j, n), o[n]);
+        }
+        const int j = row - (len - (k - 1));                                 // its place in the new state
+        if (!INSIDE && d.dstate_out != nullptr && j >= 0 && j < k - 1) {
+          f2 e[N];
+          Pairs<T, V>::get(*reinterpret_cast<const Raw*>(static_cast<const T*>(d.dstate_out) +
+                                                         (static_cast<long long>(b) * (k - 1) + j) * d.C + c), e);
+#pragma unroll
+          for (int n = 0; n < N; ++n) o[n] = add2(o[n], e[n]);
+        }
+        T* to = (INSIDE || row >= 0) ? static_cast<T*>(d.dx) + (static_cast<long long>(b) * d.T + row) * d.C + c
+                                     : static_cast<T*>(d.dstate) + (static_cast<long long>(b) * (k - 1) + row + k - 1) * d.C + c;
+        *reinterpret_cast<Raw*>(to) = Pairs<T, V>::put(o);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int t = t0; t < t1 + k - 1; t += 2 * R) {
+    rows(t, s1, s2, g1, g2);
+    if (t + R < t1 + k - 1) rows(t + R, s2, s1, g2, g1);
   }
 }
 
-// dx (and d state) of a tile need d pre of the tile and of the k - 1 rows behind it, which the thread computes too.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(BWD_LANES * BWD_TILES) causal_conv_bwd_kernel(const ConvArgs a, float* partial, int groups) {
-  constexpr int KM = K ? K : 8;
+  using W = Taps<V, K>;
+  constexpr int KM = W::KM, N = W::N;
   const BdhConvDesc& d = a.d;
   const int k = K ? K : d.k;
   const int cblocks = (a.packs + BWD_LANES - 1) / BWD_LANES;
   const int pack = (blockIdx.x % cblocks) * BWD_LANES + threadIdx.x, group = blockIdx.x / cblocks;
   const bool live = pack < a.packs;
   const int c = pack * V;
-  float w[KM][V], bias[V], gw[KM][V], gb[V];
+  W w;
+  w.load(d, k, c, live);
+  f2 sw[KM][N], sb[N];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+  for (int n = 0; n < N; ++n) {
 #pragma unroll
-    for (int j = 0; j < KM; ++j) {
-      w[j][v] = (live && j >= KM - k) ? d.w[static_cast<long long>(c + v) * k + j - (KM - k)] : 0.f;
-      gw[j][v] = 0.f;
-    }
-    bias[v] = (live && d.bias) ? d.bias[c + v] : 0.f;
-    gb[v] = 0.f;
+    for (int j = 0; j < KM; ++j) sw[j][n] = both(0.f);
+    sb[n] = both(0.f);
   }
   const long long all = static_cast<long long>(d.B) * a.tiles;
   for (long long bt = static_cast<long long>(group) * BWD_TILES + threadIdx.y; live && bt < all;
@@ -135,106 +273,31 @@ __global__ void __launch_bounds__(BWD_LANES * BWD_TILES) causal_conv_bwd_kernel(
     const int b = static_cast<int>(bt / a.tiles), tile = static_cast<int>(bt % a.tiles);
     const int len = a.len.get(b, d.T);
     const int t0 = tile * a.tile, t1 = min(t0 + a.tile, d.T);
-    float s[KM - 1 + ROWS][V], g[KM - 1 + ROWS][V];
-#pragma unroll
-    for (int j = 0; j < KM - 1; ++j) {
-      const Pack<T, V> p = load_seq<T, V>(d, b, t0 - (KM - 1) + j, len, c);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        s[j][v] = p[v];
-        g[j][v] = 0.f;
-      }
-    }
-    const int first = (t0 == 0 && d.dstate != nullptr) ? -(k - 1) : t0;      // first row whose gradient this tile writes
-    for (int t = t0; t < t1 + k - 1; t += ROWS) {
-      Pack<T, V> px[ROWS], pd[ROWS];
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        px[r] = load_seq<T, V>(d, b, t + r, len, c);
-        if (t + r < len && t + r < t1 + k - 1)
-          pd[r].load(static_cast<const T*>(d.dy) + b * d.dy_sb + (t + r) * d.dy_st + c);
-        else
-          pd[r].zero();
-      }
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[KM - 1 + r][v] = px[r][v];
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const bool in = t + r < len;
-        const bool mine = t + r < t1;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float gr = pd[r][v];
-          if (d.silu) {
-            float pre = bias[v];
-#pragma unroll
-            for (int j = 0; j < KM; ++j)
-              if (K || j >= KM - k) pre = fmaf(w[j][v], s[r + j][v], pre);
-            const float sg = sigmoid_f32(pre);
-            gr *= sg * fmaf(pre, 1.f - sg, 1.f);
-          }
-          gr = in ? gr : 0.f;
-          g[KM - 1 + r][v] = gr;
-          if (mine && in) {
-            gb[v] += gr;
-#pragma unroll
-            for (int j = 0; j < KM; ++j)
-              if (K || j >= KM - k) gw[j][v] = fmaf(gr, s[r + j][v], gw[j][v]);
-          }
-        }
-        const int row = t + r - (k - 1);                                     // complete now: every d pre it feeds is known
-        if (row >= first && row < t1) {
-          float o[V];
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            o[v] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KM; ++j)                                     // tap j of output row + (k - 1) - j
-              if (K || j >= KM - k) o[v] = fmaf(w[j][v], g[KM - 1 + r - (j - (KM - k))][v], o[v]);
-          }
-          const int j = row - (len - (k - 1));                               // its place in the new state
-          if (d.dstate_out != nullptr && j >= 0 && j < k - 1) {
-            Pack<T, V> e;
-            e.load(static_cast<const T*>(d.dstate_out) + (static_cast<long long>(b) * (k - 1) + j) * d.C + c);
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v] += e[v];
-          }
-          Pack<T, V> q;
-#pragma unroll
-          for (int v = 0; v < V; ++v) q.set(v, o[v]);
-          if (row >= 0)
-            q.store(static_cast<T*>(d.dx) + (static_cast<long long>(b) * d.T + row) * d.C + c);
-          else
-            q.store(static_cast<T*>(d.dstate) + (static_cast<long long>(b) * (k - 1) + row + k - 1) * d.C + c);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < KM - 1; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          s[j][v] = s[j + ROWS][v];
-          g[j][v] = g[j + ROWS][v];
-        }
-    }
+    if (t0 >= W::R && t1 + k + W::R <= len)             // rows up to t1 + k + R - 3 are read; the new state's are behind
+      conv_bwd_tile<T, V, K, true>(d, w, sw, sb, b, t0, t1, len, c);
+    else
+      conv_bwd_tile<T, V, K, false>(d, w, sw, sb, b, t0, t1, len, c);
   }
   if (partial == nullptr) return;
   // partial[group][tap or bias][channel]: the block's four tile rows added up
-  __shared__ float sum[BWD_TILES][V][BWD_LANES];
+  __shared__ f2 sum[BWD_TILES][N][BWD_LANES];
 #pragma unroll
   for (int j = 0; j <= KM; ++j) {
     if (j < KM - k) continue;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[threadIdx.y][v][threadIdx.x] = j < KM ? gw[j < KM ? j : 0][v] : gb[v];
+    for (int n = 0; n < N; ++n) sum[threadIdx.y][n][threadIdx.x] = j < KM ? sw[j < KM ? j : 0][n] : sb[n];
     __syncthreads();
     if (threadIdx.y == 0 && live) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float x = 0.f;
+      for (int n = 0; n < N; ++n) {
+        f2 x = sum[0][n][threadIdx.x];
 #pragma unroll
-        for (int y = 0; y < BWD_TILES; ++y) x += sum[y][v][threadIdx.x];
-        partial[(static_cast<long long>(group) * (k + 1) + j - (KM - k)) * d.C + c + v] = x;
+        for (int y = 1; y < BWD_TILES; ++y) x = add2(x, sum[y][n][threadIdx.x]);
+        float lo, hi;
+        unpack2(x, lo, hi);
+        float* to = partial + (static_cast<long long>(group) * (k + 1) + j - (KM - k)) * d.C + c + 2 * n;
+        to[0] = lo;
+        if (2 * n + 1 < V) to[1] = hi;
       }
     }
     __syncthreads();
@@ -268,35 +331,41 @@ __global__ void __launch_bounds__(FWD_THREADS) causal_conv_step_kernel(const Con
   const int k = d.k;
   const T* st = static_cast<const T*>(d.state) + b * d.state_sb + c;
   T* so = static_cast<T*>(d.state_out) + b * d.state_out_sb + c;
-  Pack<T, V> row[8];
+  using Raw = typename Pack<T, V>::Raw;
+  constexpr int N = (V + 1) / 2;
+  Raw row[7];
 #pragma unroll
   for (int j = 0; j < 7; ++j)
-    if (j < k - 1) row[j].load(st + j * d.state_sr);
-  row[7].load(static_cast<const T*>(d.x) + b * d.x_sb + c);
-  float pre[V];
+    if (j < k - 1) row[j] = *reinterpret_cast<const Raw*>(st + j * d.state_sr);
+  const Raw x = *reinterpret_cast<const Raw*>(static_cast<const T*>(d.x) + b * d.x_sb + c);
+  const auto tap = [&](int v, int j) { return v < V ? d.w[static_cast<long long>(c + v) * k + j] : 0.f; };
+  const auto add = [&](f2 (&o)[N], const Raw& r, int j) {
+    f2 e[N];
+    Pairs<T, V>::get(r, e);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    pre[v] = d.bias ? d.bias[c + v] : 0.f;
-    const float* w = d.w + static_cast<long long>(c + v) * k;
+    for (int n = 0; n < N; ++n) o[n] = fma2(pack2(tap(2 * n, j), tap(2 * n + 1, j)), e[n], o[n]);
+  };
+  f2 o[N];
 #pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < k - 1) pre[v] = fmaf(w[j], row[j][v], pre[v]);
-    pre[v] = fmaf(w[k - 1], row[7][v], pre[v]);
-    if (d.silu) pre[v] *= sigmoid_f32(pre[v]);
+  for (int n = 0; n < N; ++n) o[n] = d.bias ? pack2(d.bias[c + 2 * n], 2 * n + 1 < V ? d.bias[c + 2 * n + 1] : 0.f) : both(0.f);
+#pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (j < k - 1) add(o, row[j], j);
+  add(o, x, k - 1);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (d.silu) o[n] = mul2(o[n], sigmoid_quick2(o[n]));
+    if (!on) o[n] = both(0.f);
   }
-  Pack<T, V> o;
+  *reinterpret_cast<Raw*>(static_cast<T*>(d.y) + static_cast<long long>(b) * d.C + c) = Pairs<T, V>::put(o);
+  if (!on && so == st) return;
 #pragma unroll
-  for (int v = 0; v < V; ++v) o.set(v, on ? pre[v] : 0.f);
-  o.store(static_cast<T*>(d.y) + static_cast<long long>(b) * d.C + c);
-  if (on) {
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < k - 1) (j + 1 < k - 1 ? row[j < 6 ? j + 1 : 7] : row[7]).store(so + j * d.state_out_sr);
-  } else if (so != st) {
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (j < k - 1) row[j].store(so + j * d.state_out_sr);
-  }
+  for (int j = 0; j < 7; ++j)
+    if (j < k - 1) {
+      Raw r = row[j];
+      if (on) r = j + 1 < k - 1 ? row[j < 6 ? j + 1 : 6] : x;
+      *reinterpret_cast<Raw*>(so + j * d.state_out_sr) = r;
+    }
 }
 
 bool multiple(const void* p, long long bytes) { return reinterpret_cast<unsigned long long>(p) % bytes == 0; }

@@ -54,6 +54,4 @@ struct Lengths {
   }
 };
 
-__device__ __forceinline__ float sigmoid_f32(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-
 }  // namespace bdh

@@ -23,7 +23,7 @@
 #pragma once
 #include "bdh_kernels.h"
 #include "device_once.h"
-#include "element_io.cuh"
+#include "pair_math.cuh"
 
 #include <cmath>
 #include <type_traits>
@@ -51,48 +51,6 @@ struct ScanArgs {
   const float* seg_dt;                 // [B][segs][D]: their total steps
 };
 
-// ---- two fp32 operations in one instruction ------------------------------------------------------------
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pack2(float x, float y) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// One value with both of a pair (the moves that make the pair cost less than two plain products)
-__device__ __forceinline__ f2 mul1(float a, f2 b) { return mul2(both(a), b); }
-__device__ __forceinline__ f2 fma1(float a, f2 b, f2 c) { return fma2(both(a), b, c); }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  f2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ f2 ex2x2(f2 v) {
-  float x, y;
-  unpack2(v, x, y);
-  return pack2(ex2(x), ex2(y));
-}
-__device__ __forceinline__ float sum2(f2 v) {
-  float x, y;
-  unpack2(v, x, y);
-  return x + y;
-}
 __device__ __forceinline__ void load4(const float* p, f2& x, f2& y) {
   const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
   x = v.x;
