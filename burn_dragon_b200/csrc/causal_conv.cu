@@ -12,12 +12,19 @@
 #include "bdh_kernels.h"
 #include "pair_math.cuh"
 
+#include <type_traits>
+
 namespace bdh {
 namespace {
 
 constexpr int FWD_THREADS = 128;
+constexpr int FWD_ROWS = 8;          // rows that a thread works on at once, forward and (width 2 to 4) backward
+constexpr int BWD_ROWS = 4;
 constexpr int BWD_LANES = 32;        // backward block: 32 channel packs x 4 tiles
 constexpr int BWD_TILES = 4;
+constexpr int BWD_THREADS = BWD_LANES * BWD_TILES;
+enum { ANY_SET, FIRST_SET, MIDDLE_SET, LAST_SET };
+constexpr int AHEAD = 2;             // sets of rows on their way, backward (AHEAD + 1 sets of shared memory)
 
 struct ConvArgs {
   BdhConvDesc d;
@@ -43,9 +50,9 @@ __device__ __forceinline__ typename Pack<T, V>::Raw load_seq(const BdhConvDesc& 
 // K: the kernel width, or 0 for a width of up to 8 known at run time (taps then sit at the end of the window; the leading
 // ones are skipped, not multiplied by zero: a row there may hold anything). R: rows that a thread works on at once; with
 // the R rows before them they hold every window, and the two sets change places instead of moving.
-template <int V, int K>
+template <int V, int K, int R>
 struct Taps {
-  static constexpr int KM = K ? K : 8, R = K ? 4 : 8, N = (V + 1) / 2;
+  static constexpr int KM = K ? K : 8, N = (V + 1) / 2;
   static_assert(KM - 1 <= R, "a window lies within two sets of rows");
   f2 w[KM][N], bias[N];
   __device__ __forceinline__ void load(const BdhConvDesc& d, int k, int c, bool live) {
@@ -74,15 +81,22 @@ struct Taps {
 // would wait for it) while the present ones are worked on. INSIDE: every row that is read is one of x's, t1 - t0 is a
 // multiple of R.
 template <typename T, int V, int K, bool INSIDE>
-__device__ __forceinline__ void conv_fwd_tile(const BdhConvDesc& d, const Taps<V, K>& w, int b, int t0, int t1, int len, int c) {
-  using W = Taps<V, K>;
-  constexpr int R = W::R, N = W::N;
+__device__ __forceinline__ void conv_fwd_tile(const BdhConvDesc& d, const Taps<V, K, FWD_ROWS>& w, int b, int t0, int t1, int len, int c) {
+  using W = Taps<V, K, FWD_ROWS>;
+  constexpr int R = FWD_ROWS, N = W::N;
   using Raw = typename Pack<T, V>::Raw;
   const int k = K ? K : d.k;
   f2 one[R][N], two[R][N];
   Raw next[R];
+  const T* px = static_cast<const T*>(d.x) + b * d.x_sb + t0 * d.x_st + c;
+  const auto load = [&](int t) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) next[r] = load_seq<T, V, INSIDE>(d, b, t0 + r, min(len, t1), c);
+    for (int r = 0; r < R; ++r) {
+      next[r] = INSIDE ? *reinterpret_cast<const Raw*>(px) : load_seq<T, V, false>(d, b, t + r, min(len, t1), c);
+      px += d.x_st;
+    }
+  };
+  load(t0);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (r <= R - W::KM) continue;                                            // (not in any window)
@@ -92,9 +106,7 @@ __device__ __forceinline__ void conv_fwd_tile(const BdhConvDesc& d, const Taps<V
   const auto rows = [&](int t, const f2 (&before)[R][N], f2 (&s)[R][N]) {
 #pragma unroll
     for (int r = 0; r < R; ++r) Pairs<T, V>::get(next[r], s[r]);
-    if (t + R < t1)
-#pragma unroll
-      for (int r = 0; r < R; ++r) next[r] = load_seq<T, V, INSIDE>(d, b, t + R + r, min(len, t1), c);
+    if (t + R < t1) load(t + R);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (!INSIDE && t + r >= t1) break;
@@ -117,8 +129,8 @@ __device__ __forceinline__ void conv_fwd_tile(const BdhConvDesc& d, const Taps<V
 }
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(FWD_THREADS) causal_conv_fwd_kernel(const ConvArgs a) {
-  using W = Taps<V, K>;
+__global__ void __launch_bounds__(FWD_THREADS, 6) causal_conv_fwd_kernel(const ConvArgs a) {
+  using W = Taps<V, K, FWD_ROWS>;
   const BdhConvDesc& d = a.d;
   const int k = K ? K : d.k;
   const long long i = static_cast<long long>(blockIdx.x) * FWD_THREADS + threadIdx.x;
@@ -138,46 +150,60 @@ __global__ void __launch_bounds__(FWD_THREADS) causal_conv_fwd_kernel(const Conv
   W w;
   w.load(d, k, c, true);
   const int t0 = tile * a.tile, t1 = min(t0 + a.tile, d.T);
-  if (t0 >= W::R && t1 <= len && (t1 - t0) % W::R == 0)
+  if (t0 >= FWD_ROWS && t1 <= len && (t1 - t0) % FWD_ROWS == 0)
     conv_fwd_tile<T, V, K, true>(d, w, b, t0, t1, len, c);
   else
     conv_fwd_tile<T, V, K, false>(d, w, b, t0, t1, len, c);
 }
 
 // Gradients of rows t0 .. t1: dx (and d state) need d pre of these rows and of the k - 1 behind them, which the thread
-// computes too. INSIDE: every row of x and dy that is read exists, and no row is one of the new state's. sw, sb: the
-// thread's sums for w and bias.
+// computes too. INSIDE: every row of x and dy that is read exists, no row is one of the new state's, and t1 - t0 is an
+// even number of sets. sw, sb: the thread's sums for w and bias.
 template <typename T, int V, int K, bool INSIDE>
-__device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V, K>& w, f2 (&sw)[Taps<V, K>::KM][Taps<V, K>::N],
-                                              f2 (&sb)[Taps<V, K>::N], int b, int t0, int t1, int len, int c) {
-  using W = Taps<V, K>;
-  constexpr int KM = W::KM, R = W::R, N = W::N;
+struct BwdTile {
+  static constexpr int R = K ? BWD_ROWS : 8;
+  using W = Taps<V, K, R>;
+  static constexpr int KM = W::KM, N = W::N;
   using Raw = typename Pack<T, V>::Raw;
-  const int k = K ? K : d.k;
-  const int first = (!INSIDE && t0 == 0 && d.dstate != nullptr) ? -(k - 1) : t0;      // first row whose gradient this tile writes
-  const auto load_dy = [&](int r) {
-    if (INSIDE || (r < len && r < t1 + k - 1))
-      return *reinterpret_cast<const Raw*>(static_cast<const T*>(d.dy) + b * d.dy_sb + r * d.dy_st + c);
-    Pack<T, V> p;
-    p.zero();
-    return *reinterpret_cast<const Raw*>(&p);
-  };
-  f2 s1[R][N], s2[R][N], g1[R][N], g2[R][N];
+  // INSIDE: rows come by asynchronous copies AHEAD sets before their turn, each thread reading back its own; registers
+  // for that many would leave too few threads to cover the way to memory. Else one set ahead, in registers.
+  static constexpr bool RINGS = INSIDE && K != 0 && V * sizeof(T) >= 4;
+  static constexpr int BYTES = V * static_cast<int>(sizeof(T));
+  const BdhConvDesc& d;
+  const W& w;
+  f2 (&sw)[KM][N];
+  f2 (&sb)[N];
+  Raw* ring;
+  int b, t0, t1, len, c, k;
+  const T *px, *pd;                  // the next row to be fetched
+  T* pg;                             // the next row of dx
+  int set = 0;                       // of the next rows to be worked on
   Raw nx[R], nd[R];
+
+  __device__ __forceinline__ void load(int t, int to) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    nx[r] = load_seq<T, V, INSIDE>(d, b, t0 + r, len, c);
-    nd[r] = load_dy(t0 + r);
+    for (int r = 0; r < R; ++r) {
+      if constexpr (RINGS) {
+        if (t < t1 + k - 1) {
+          copy_async<BYTES>(ring + (to * R + r) * 2 * BWD_THREADS, px, true);
+          copy_async<BYTES>(ring + ((to * R + r) * 2 + 1) * BWD_THREADS, pd, true);
+        }
+      } else if (INSIDE || (t + r < len && t + r < t1 + k - 1)) {
+        nx[r] = *reinterpret_cast<const Raw*>(px);
+        nd[r] = *reinterpret_cast<const Raw*>(pd);
+      } else {
+        Pack<T, V> p;
+        p.zero();
+        nx[r] = nd[r] = *reinterpret_cast<const Raw*>(&p);
+      }
+      px += d.x_st;
+      pd += d.dy_st;
+    }
+    if constexpr (RINGS) copy_close();
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) g1[r][n] = both(0.f);
-    if (r <= R - KM) continue;
-    Pairs<T, V>::get(load_seq<T, V, INSIDE>(d, b, t0 - R + r, len, c), s1[r]);
-  }
-  // d pre of row t + r - (tap of j): K known at compile time, or found among the (at most 8) rows behind
-  const auto back = [&](const f2 (&gp)[R][N], const f2 (&g)[R][N], int r, int j, int n) {
+
+  // d pre of the row that tap j reaches back to: K known at compile time, or found among the (at most 8) rows behind
+  __device__ __forceinline__ f2 back(const f2 (&gp)[R][N], const f2 (&g)[R][N], int r, int j, int n) const {
     if constexpr (K != 0) {
       return W::at(gp, g, r - j, n);
     } else {
@@ -187,22 +213,36 @@ __device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V
         if (i == j - (KM - k)) x = W::at(gp, g, r - i, n);
       return x;
     }
-  };
-  const auto rows = [&](int t, const f2 (&sp)[R][N], f2 (&s)[R][N], const f2 (&gp)[R][N], f2 (&g)[R][N]) {
+  }
+
+  // One set of rows. Which of a tile's sets it is decides at compile time what INSIDE needs no test for: the first
+  // completes no row before t0, the last (behind t1) gives d pre only.
+  template <int SET>
+  __device__ __forceinline__ void rows(int t, int first, const f2 (&sp)[R][N], f2 (&s)[R][N], const f2 (&gp)[R][N], f2 (&g)[R][N]) {
+    if constexpr (RINGS) {
+      copy_wait<AHEAD - 1>();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        nx[r] = ring[(set * R + r) * 2 * BWD_THREADS];
+        nd[r] = ring[((set * R + r) * 2 + 1) * BWD_THREADS];
+      }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       Pairs<T, V>::get(nx[r], s[r]);
       Pairs<T, V>::get(nd[r], g[r]);                                         // dy for now
     }
-    if (t + R < t1 + k - 1)
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        nx[r] = load_seq<T, V, INSIDE>(d, b, t + R + r, len, c);
-        nd[r] = load_dy(t + R + r);
-      }
+    if constexpr (RINGS) {                                                   // into the set that was read before this one
+      if constexpr (SET != LAST_SET) load(t + AHEAD * R, set == 0 ? AHEAD : set - 1);
+      set = set == AHEAD ? 0 : set + 1;
+    } else {
+      if (t + R < t1 + k - 1) load(t + R, 0);
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool in = INSIDE || t + r < len;
+      if (SET == LAST_SET && r >= KM - 1) break;
+      const bool in = SET != ANY_SET || t + r < len;
+      const bool mine = SET == ANY_SET ? t + r < t1 && in : SET != LAST_SET;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         if (d.silu) {                                                        // silu' = sg (1 + pre (1 - sg))
@@ -210,7 +250,7 @@ __device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V
           g[r][n] = mul2(g[r][n], mul2(sg, fma2(pre, fma2(sg, both(-1.f), both(1.f)), both(1.f))));
         }
         if (!in) g[r][n] = both(0.f);
-        if (t + r < t1 && in) {
+        if (mine) {
           sb[n] = add2(sb[n], g[r][n]);
 #pragma unroll
           for (int j = 0; j < KM; ++j)
@@ -218,7 +258,7 @@ __device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V
         }
       }
       const int row = t + r - (k - 1);                                       // complete now: every d pre it feeds is known
-      if (row >= first && row < t1) {
+      if (SET == ANY_SET ? (row >= first && row < t1) : (SET != FIRST_SET || r >= KM - 1)) {
         f2 o[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -235,29 +275,66 @@ __device__ __forceinline__ void conv_bwd_tile(const BdhConvDesc& d, const Taps<V
 #pragma unroll
           for (int n = 0; n < N; ++n) o[n] = add2(o[n], e[n]);
         }
-        T* to = (INSIDE || row >= 0) ? static_cast<T*>(d.dx) + (static_cast<long long>(b) * d.T + row) * d.C + c
-                                     : static_cast<T*>(d.dstate) + (static_cast<long long>(b) * (k - 1) + row + k - 1) * d.C + c;
-        *reinterpret_cast<Raw*>(to) = Pairs<T, V>::put(o);
+        if (INSIDE || row >= 0) {
+          *reinterpret_cast<Raw*>(pg) = Pairs<T, V>::put(o);
+          pg += d.C;
+        } else {
+          *reinterpret_cast<Raw*>(static_cast<T*>(d.dstate) + (static_cast<long long>(b) * (k - 1) + row + k - 1) * d.C + c) =
+              Pairs<T, V>::put(o);
+        }
       }
     }
-  };
-#pragma unroll 1
-  for (int t = t0; t < t1 + k - 1; t += 2 * R) {
-    rows(t, s1, s2, g1, g2);
-    if (t + R < t1 + k - 1) rows(t + R, s2, s1, g2, g1);
   }
-}
+
+  __device__ __forceinline__ void run() {
+    f2 s1[R][N], s2[R][N], g1[R][N], g2[R][N];
+    px = static_cast<const T*>(d.x) + b * d.x_sb + t0 * d.x_st + c;
+    pd = static_cast<const T*>(d.dy) + b * d.dy_sb + t0 * d.dy_st + c;
+    pg = static_cast<T*>(d.dx) + (static_cast<long long>(b) * d.T + t0) * d.C + c;
+    load(t0, 0);
+    if constexpr (RINGS) {
+#pragma unroll
+      for (int i = 1; i < AHEAD; ++i) load(t0 + i * R, i);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) g1[r][n] = both(0.f);
+      if (r <= R - KM) continue;                                             // (not in any window)
+      Pairs<T, V>::get(load_seq<T, V, INSIDE>(d, b, t0 - R + r, len, c), s1[r]);
+    }
+    if constexpr (INSIDE && K != 0) {                                        // an even number of sets, and the one behind
+      rows<FIRST_SET>(t0, t0, s1, s2, g1, g2);
+      rows<MIDDLE_SET>(t0 + R, t0, s2, s1, g2, g1);
+#pragma unroll 1
+      for (int t = t0 + 2 * R; t < t1; t += 2 * R) {
+        rows<MIDDLE_SET>(t, t0, s1, s2, g1, g2);
+        rows<MIDDLE_SET>(t + R, t0, s2, s1, g2, g1);
+      }
+      rows<LAST_SET>(t1, t0, s1, s2, g1, g2);
+    } else {
+      const int first = (!INSIDE && t0 == 0 && d.dstate != nullptr) ? -(k - 1) : t0;  // first row whose gradient this tile writes
+#pragma unroll 1
+      for (int t = t0; t < t1 + k - 1; t += 2 * R) {
+        rows<ANY_SET>(t, first, s1, s2, g1, g2);
+        if (t + R < t1 + k - 1) rows<ANY_SET>(t + R, first, s2, s1, g2, g1);
+      }
+    }
+  }
+};
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(BWD_LANES * BWD_TILES) causal_conv_bwd_kernel(const ConvArgs a, float* partial, int groups) {
-  using W = Taps<V, K>;
-  constexpr int KM = W::KM, N = W::N;
+__global__ void __launch_bounds__(BWD_THREADS, K ? 3 : 2) causal_conv_bwd_kernel(const ConvArgs a, float* partial, int groups) {
+  using W = typename BwdTile<T, V, K, true>::W;
+  constexpr int KM = W::KM, N = W::N, R = BwdTile<T, V, K, true>::R;
   const BdhConvDesc& d = a.d;
   const int k = K ? K : d.k;
   const int cblocks = (a.packs + BWD_LANES - 1) / BWD_LANES;
   const int pack = (blockIdx.x % cblocks) * BWD_LANES + threadIdx.x, group = blockIdx.x / cblocks;
   const bool live = pack < a.packs;
   const int c = pack * V;
+  __shared__ typename Pack<T, V>::Raw ring[K ? (AHEAD + 1) * R * 2 * BWD_THREADS : 1];
+  typename Pack<T, V>::Raw* own = ring + (K ? threadIdx.y * BWD_LANES + threadIdx.x : 0);
   W w;
   w.load(d, k, c, live);
   f2 sw[KM][N], sb[N];
@@ -273,10 +350,11 @@ __global__ void __launch_bounds__(BWD_LANES * BWD_TILES) causal_conv_bwd_kernel(
     const int b = static_cast<int>(bt / a.tiles), tile = static_cast<int>(bt % a.tiles);
     const int len = a.len.get(b, d.T);
     const int t0 = tile * a.tile, t1 = min(t0 + a.tile, d.T);
-    if (t0 >= W::R && t1 + k + W::R <= len)             // rows up to t1 + k + R - 3 are read; the new state's are behind
-      conv_bwd_tile<T, V, K, true>(d, w, sw, sb, b, t0, t1, len, c);
+    // rows up to t1 + R + k are read inside; the new state's are behind them
+    if (t0 >= R && t1 + k + R <= len && (t1 - t0) % (2 * R) == 0)
+      BwdTile<T, V, K, true>{d, w, sw, sb, own, b, t0, t1, len, c, k}.run();
     else
-      conv_bwd_tile<T, V, K, false>(d, w, sw, sb, b, t0, t1, len, c);
+      BwdTile<T, V, K, false>{d, w, sw, sb, own, b, t0, t1, len, c, k}.run();
   }
   if (partial == nullptr) return;
   // partial[group][tap or bias][channel]: the block's four tile rows added up
@@ -386,11 +464,11 @@ int checked(const BdhConvDesc& d) {
   return BDH_OK;
 }
 
-// Rows per tile: 64 keeps the rows that two tiles both read at (k - 1) / 64; shorter tiles (not below 8) while there
-// are fewer than two waves of threads.
+// Rows per tile: 64 keeps the rows that two tiles both read at (k - 1) / 64; shorter tiles, not below 16, while there are
+// fewer threads than a quarter of what the GPU holds (4096 x 2048 bf16: 10.5 us, in tiles of 64 26 us).
 int tile_rows(const BdhConvDesc& d, int packs) {
   int tile = 64;
-  while (tile > 8 && static_cast<long long>(d.B) * ((d.T + tile - 1) / tile) * packs < 148LL * 1024) tile /= 2;
+  while (tile > 16 && static_cast<long long>(d.B) * ((d.T + tile - 1) / tile) * packs < 148LL * 512) tile /= 2;
   return tile;
 }
 
@@ -423,8 +501,7 @@ int fwd_width(const BdhConvDesc& d, cudaStream_t s) {
     case 3: return fwd_launch<T, V, 3>(d, s);
     case 4: return fwd_launch<T, V, 4>(d, s);
   }
-  // the window of 8 rows in registers: packs of half the bytes
-  return fwd_launch<T, (V > 4 ? 4 : V), 0>(d, s);
+  return fwd_launch<T, V, 0>(d, s);
 }
 
 int bwd_groups(const ConvArgs& a) {
@@ -469,18 +546,21 @@ int step_launch(const BdhConvDesc& d, const unsigned char* active, cudaStream_t 
   return launched();
 }
 
+// Channels a thread. Forward two: the most threads that still store a pair (8 x 2048 x 4096 bf16: 55 us; four 57,
+// eight 78 us, at 4096 x 2048 10.5, 18 and 26 us). Backward 8 bytes: rows come through shared memory there, and a
+// thread's overhead is shared by more elements.
 template <typename T>
 int fwd_type(const BdhConvDesc& d, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  return packs_fit(d, V, sizeof(T)) ? fwd_width<T, V>(d, s) : fwd_width<T, 1>(d, s);
+  return packs_fit(d, 2, sizeof(T)) ? fwd_width<T, 2>(d, s) : fwd_width<T, 1>(d, s);
 }
 template <typename T>
 int bwd_type(const BdhConvDesc& d, float* dw, float* db, float* partial, cudaStream_t s) {
-  return packs_fit(d, 4, sizeof(T)) ? bwd_width<T, 4>(d, dw, db, partial, s) : bwd_width<T, 1>(d, dw, db, partial, s);
+  constexpr int V = 8 / sizeof(T);
+  return packs_fit(d, V, sizeof(T)) ? bwd_width<T, V>(d, dw, db, partial, s) : bwd_width<T, 1>(d, dw, db, partial, s);
 }
 template <typename T>
 int step_type(const BdhConvDesc& d, const unsigned char* active, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 8 / sizeof(T);
   return packs_fit(d, V, sizeof(T)) ? step_launch<T, V>(d, active, s) : step_launch<T, 1>(d, active, s);
 }
 
@@ -503,7 +583,7 @@ extern "C" int bdh_causal_conv_fwd(const BdhConvDesc* d, cudaStream_t s) {
 extern "C" long long bdh_causal_conv_partials(const BdhConvDesc* d) {
   if (checked(*d) != BDH_OK) return 0;
   long long most = 0;
-  for (int v : {1, 4}) {
+  for (int v : {1, 2, 4}) {
     const long long n = static_cast<long long>(bwd_groups(args_for(*d, v))) * (d->k + 1) * d->C;
     most = n > most ? n : most;
   }

@@ -54,4 +54,15 @@ struct Lengths {
   }
 };
 
+// Asynchronous copies of 4, 8 or 16 bytes to shared memory (not `in`: zeros), closed into groups; a thread sees what it
+// copied itself once it has waited for all but the newest LEFT groups.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
+  const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(BYTES), "r"(in ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
 }  // namespace bdh

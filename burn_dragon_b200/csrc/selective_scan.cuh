@@ -203,14 +203,6 @@ struct Tile {
 // time for a tile than one load from memory. Every lane reads back only what it copied itself.
 constexpr int RING = 3;
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
-  const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(dst));
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(BYTES), "r"(in ? BYTES : 0) : "memory");
-}
-__device__ __forceinline__ void copy_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory"); }
-
 template <typename T, int G, int CT, bool VEC, bool DY>
 struct Ring {
   using S = Shape<T, G, CT>;
@@ -478,7 +470,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
   for (int tile = first; tile < last; ++tile) {
     const int t0 = tile * LT;
     if (tile < end) {
-      copy_wait();
+      copy_wait<RING - 2>();
       sh.in.template put<T, true, true>(d, sh.ring.at(tile), t0, len);
       __syncwarp();
       sh.ring.template load<true, true>(d, tile + RING - 1, end, w.b, c0, len);
@@ -579,7 +571,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
   __syncwarp();
   for (int i = 0; i < n; ++i) {
     const int tile = tile_of(i);
-    copy_wait();
+    copy_wait<RING - 2>();
     sh.in.template put<T, !REV, REV>(d, sh.ring.at(tile), tile * LT, len);
     __syncwarp();
     sh.ring.template load<!REV, REV>(d, i + RING - 1 < n ? tile_of(i + RING - 1) : -1, end, w.b, c0, len);
