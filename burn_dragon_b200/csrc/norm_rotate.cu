@@ -5,86 +5,94 @@
 //   d angle_i = sum over heads of v_2i dv_2i+1 - v_2i+1 dv_2i                     (a rotation keeps this cross product)
 //
 // The angle of a token's pair is given, or 2 pi frac(position * freq) with the product in 64 bits (a position of 10^6
-// leaves 4 of 24 bits of the fraction in 32). Bound by memory: ~10 (forward) or ~30 operations an element against one
-// tensor in and one out (two in, one out). A group of G lanes holds one head's row in registers, so x is read once;
-// the sines and cosines of a token are made once per block and shared by its heads through shared memory, because a
-// sine and cosine a pair and head would cost more than the rest of the row. Heads of q and k form one list; a block
-// takes a slice of it (whole, up to 2048 elements) and steps through the tokens, so that each thread stays with one
-// head and the gradients of its weights stay in registers. Sums are fp32, in a fixed order.
+// leaves 4 of 24 bits of the fraction in 32). Bound by memory: ~9 (forward) or ~13 operations an element against one
+// tensor in and one out (two in, one out). G lanes hold one head's row, so x is read once. A thread stays with its
+// token slot and its columns and goes through heads: sines and cosines are made once per token and block (one for
+// each pair and head would cost more than the rest of the row) and stay in registers over the heads; a row's slot is
+// refilled from the next token as soon as it has been unpacked, so that loads are always on their way. Heads come in
+// groups of hr rows, each of q or of k alone, so that a weight's gradient stays in registers over all rows that share
+// it. Sums are fp32, in a fixed order.
 #include "bdh_kernels.h"
-#include "element_io.cuh"
+#include "pair_math.cuh"
 
 #include <type_traits>
 
 namespace bdh {
 namespace {
 
-constexpr int NT = 256;
-constexpr int WARPS = NT / 32;
+constexpr int NT = 128;
 
 struct NormArgs {
   BdhNormRotateDesc d;
   Lengths len;
   int tokens;                // B * T
-  int H, G, rows;            // heads of q and k; lanes per row; rows per block
-  int HS, slices, TS;        // heads per slice; slices; tokens at once
-  int shared_w;              // one weight for all heads
+  int G, hr, TS;             // lanes per row; heads per group; tokens at once (TS * hr * G <= NT)
+  int q_groups, groups, per_block, slices;     // groups of q; of q and k; of a block (blockIdx.y: the slice)
 };
 
-struct Row {                 // one head of one token
-  bool live;                 // it exists
-  bool in;                   // and its token is not behind its sequence's length
-  int head, h;               // in the joint list; in its tensor
-  bool key;
-  int b, t;
-};
+// This thread's place, and its rows of the token group that starts at `first`
+template <typename T, int V, bool VEC, int NV>
+struct Place {
+  using Raw = typename Pack<T, V>::Raw;
+  static constexpr int N = V / 2;
+  int lane, ts, hl, g0, ng;  // lane of the row; token slot; head within a group; the slice's groups
+  bool slot_ok;
 
-__device__ __forceinline__ Row row_of(const NormArgs& a, int token, int head, bool slot_ok) {
-  Row r;
-  r.live = slot_ok && head < a.H && token < a.tokens;
-  r.head = head;
-  r.key = head >= a.d.Hq;
-  r.h = r.key ? head - a.d.Hq : head;
-  const int tk = r.live ? token : 0;
-  r.b = tk / a.d.T;
-  r.t = tk - r.b * a.d.T;
-  r.in = r.live && r.t < a.len.get(r.b, a.d.T);
-  return r;
-}
-
-__device__ __forceinline__ long long in_offset(const BdhNormRotateDesc& d, const Row& r) {
-  return r.key ? r.b * d.k_sb + r.t * d.k_st + r.h * d.k_sh : r.b * d.q_sb + r.t * d.q_st + r.h * d.q_sh;
-}
-__device__ __forceinline__ long long out_offset(const BdhNormRotateDesc& d, const Row& r) {
-  return ((static_cast<long long>(r.b) * d.T + r.t) * (r.key ? d.Hk : d.Hq) + r.h) * d.Dh;
-}
-
-// V elements from column c on, as fp32; columns behind Dh read as 0.
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void load_cols(const T* p, int c, int Dh, float (&f)[V]) {
-  if constexpr (VEC) {
-    Pack<T, V> k;
-    if (c < Dh) k.load(p + c); else k.zero();
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = k[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = c + i < Dh ? elem_to_float<T>(p[c + i]) : 0.f;
+  __device__ __forceinline__ Place(const NormArgs& a) {
+    lane = threadIdx.x % a.G;
+    const int slot = threadIdx.x / a.G;
+    ts = slot / a.hr;
+    hl = slot - ts * a.hr;
+    slot_ok = ts < a.TS;
+    g0 = blockIdx.y * a.per_block;
+    ng = min(a.per_block, a.groups - g0);
   }
+  __device__ __forceinline__ int column(const NormArgs& a, int n) const { return (n * a.G + lane) * V; }
+  __device__ __forceinline__ bool key(const NormArgs& a, int u) const { return g0 + u >= a.q_groups; }
+  __device__ __forceinline__ int head(const NormArgs& a, int u) const {      // in its tensor, or -1
+    const bool k = key(a, u);
+    const int h = (g0 + u - (k ? a.q_groups : 0)) * a.hr + hl;
+    return slot_ok && u < ng && h < (k ? a.d.Hk : a.d.Hq) ? h : -1;
+  }
+};
+
+struct Token {
+  int b, t;
+  bool live, in;             // it exists; it is not behind its sequence's length
+};
+__device__ __forceinline__ Token token_at(const NormArgs& a, long long i) {
+  Token k;
+  k.live = i < a.tokens;
+  const int at = k.live ? static_cast<int>(i) : 0;
+  k.b = at / a.d.T;
+  k.t = at - k.b * a.d.T;
+  k.in = k.live && k.t < a.len.get(k.b, a.d.T);
+  return k;
 }
 
+// V elements from column c on, as they lie in memory; columns behind Dh read as 0
 template <typename T, int V, bool VEC>
-__device__ __forceinline__ void store_cols(T* p, int c, int Dh, const float (&f)[V]) {
+__device__ __forceinline__ typename Pack<T, V>::Raw load_cols(const T* p, int c, int Dh) {
+  Pack<T, V> k;
   if constexpr (VEC) {
-    if (c >= Dh) return;
-    Pack<T, V> k;
-#pragma unroll
-    for (int i = 0; i < V; ++i) k.set(i, f[i]);
-    k.store(p + c);
+    if (c < Dh) return *reinterpret_cast<const typename Pack<T, V>::Raw*>(p + c);
+    k.zero();
   } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.e[i] = c + i < Dh ? p[c + i] : elem_from_float<T>(0.f);
+  }
+  return *reinterpret_cast<const typename Pack<T, V>::Raw*>(&k);
+}
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void store_cols(T* p, int c, int Dh, const f2 (&f)[V / 2]) {
+  const typename Pack<T, V>::Raw raw = Pairs<T, V>::put(f);
+  if constexpr (VEC) {
+    if (c < Dh) *reinterpret_cast<typename Pack<T, V>::Raw*>(p + c) = raw;
+  } else {
+    const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (c + i < Dh) p[c + i] = elem_from_float<T>(f[i]);
+      if (c + i < Dh) p[c + i] = e[i];
   }
 }
 
@@ -94,231 +102,334 @@ __device__ __forceinline__ float group_sum(float v, int G) {
 }
 
 // cs[s][i] = (cos, sin) of pair i of token first + s
-__device__ __forceinline__ void fill_angles(const NormArgs& a, float2* cs, int first, int count) {
+__device__ __forceinline__ void fill_angles(const NormArgs& a, float2* cs, long long first) {
   const BdhNormRotateDesc& d = a.d;
-  for (int s = threadIdx.x >> 5; s < count; s += WARPS) {
-    const int token = first + s;
-    if (token >= a.tokens) break;
-    const int b = token / d.T, t = token - b * d.T;
-    if (t >= a.len.get(b, d.T)) continue;                       // (an angle there may be anything; no row uses it)
-    double pos = 0;
-    if (d.angles == nullptr) {
-      const long long at = b * d.pos_sb + t * d.pos_st;
-      pos = static_cast<double>(d.positions == nullptr ? d.pos0 + t
-                                : d.positions64 ? static_cast<const long long*>(d.positions)[at]
-                                                : static_cast<long long>(static_cast<const int*>(d.positions)[at]));
-    }
-    for (int i = threadIdx.x & 31; i < d.P; i += 32) {
+  for (int item = threadIdx.x; item < a.TS * d.P; item += NT) {
+    const int slot = item / d.P, i = item - slot * d.P;
+    const Token k = token_at(a, first + slot);
+    if (k.in) {                                                 // (an angle behind a length may be anything; no row uses it)
       float sn, c;
       if (d.angles != nullptr) {
-        sincosf(d.angles[b * d.ang_sb + t * d.ang_st + i], &sn, &c);
+        sincosf(d.angles[k.b * d.ang_sb + k.t * d.ang_st + i], &sn, &c);
       } else {
-        const double turns = pos * static_cast<double>(d.freqs[2 * i]);
+        const long long at = k.b * d.pos_sb + k.t * d.pos_st;
+        const long long pos = d.positions == nullptr ? d.pos0 + k.t
+                              : d.positions64 ? static_cast<const long long*>(d.positions)[at]
+                                              : static_cast<long long>(static_cast<const int*>(d.positions)[at]);
+        const double turns = static_cast<double>(pos) * static_cast<double>(d.freqs[2 * i]);
         sincospif(2.f * static_cast<float>(turns - floor(turns)), &sn, &c);
       }
-      cs[s * d.P + i] = make_float2(c, sn);
+      cs[item] = make_float2(c, sn);
     }
   }
 }
 
-template <typename T, int V, bool VEC, int NV, int U>
-__global__ void __launch_bounds__(NT) norm_rotate_fwd_kernel(const NormArgs a) {
-  extern __shared__ float2 cs[];
-  const BdhNormRotateDesc& d = a.d;
-  const int lane = threadIdx.x % a.G, slot = threadIdx.x / a.G;
-  const int ts = slot / a.HS, head = blockIdx.y * a.HS + slot - ts * a.HS;
-  const bool slot_ok = slot < a.TS * a.HS;
-  const bool key = head >= d.Hq;
-  const float* wp = key ? d.k_weight : d.q_weight;
-  const float* bp = key ? d.k_bias : d.q_bias;
-  const long long w_at = a.shared_w ? 0 : static_cast<long long>(key ? head - d.Hq : head) * d.Dh;
-  const bool par = slot_ok && head < a.H;
-  float w[NV][V], bias[NV][V];
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (n * a.G + lane) * V + i;
-      w[n][i] = (par && wp && c < d.Dh) ? wp[w_at + c] : 1.f;
-      bias[n][i] = (par && bp && c < d.Dh) ? bp[w_at + c] : 0.f;
+// Weights and biases of a block's rows in shared memory: one row of Dh (padded to the lanes' columns) for each of q and k,
+// or for each of the slice's heads
+struct Weights {
+  float *w, *b;
+  int pitch, per_head;
+  __device__ __forceinline__ void fill(const NormArgs& a, float* at, int pitch_, int rows, int g0) {
+    const BdhNormRotateDesc& d = a.d;
+    pitch = pitch_;
+    per_head = d.per_head;
+    w = at;
+    b = at + rows * pitch;
+    for (int i = threadIdx.x; i < rows * pitch; i += NT) {
+      const int row = i / pitch, c = i - row * pitch;
+      const bool key = per_head ? g0 + row / a.hr >= a.q_groups : row == 1;
+      const int head = per_head ? (g0 + row / a.hr - (key ? a.q_groups : 0)) * a.hr + row % a.hr : 0;
+      const bool ok = c < d.Dh && (!per_head || head < (key ? d.Hk : d.Hq));
+      const float* pw = key ? d.k_weight : d.q_weight;
+      const float* pb = key ? d.k_bias : d.q_bias;
+      w[i] = ok && pw != nullptr ? pw[static_cast<long long>(head) * d.Dh + c] : 1.f;
+      b[i] = ok && pb != nullptr ? pb[static_cast<long long>(head) * d.Dh + c] : 0.f;
     }
-  for (int first = blockIdx.x * a.TS * U; first < a.tokens; first += gridDim.x * a.TS * U) {
-    Row r[U];
-    float x[U][NV][V];
+  }
+  __device__ __forceinline__ int row(const NormArgs& a, int u, int hl, bool key) const { return per_head ? u * a.hr + hl : key; }
+};
+
+template <int N>
+__device__ __forceinline__ void load_pairs(const float* p, f2 (&f)[N]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = row_of(a, first + u * a.TS + ts, head, slot_ok);
-      const T* p = static_cast<const T*>(r[u].key ? d.k : d.q) + (r[u].in ? in_offset(d, r[u]) : 0);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) load_cols<T, V, VEC>(p, r[u].in ? (n * a.G + lane) * V : d.Dh, d.Dh, x[u][n]);
-    }
-    fill_angles(a, cs, first, U * a.TS);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float ss = 0.f;
-#pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(x[u][n][i], x[u][n][i], ss);
-      const float rs = rsqrtf(group_sum(ss, a.G) / d.Dh + d.eps);
-      if (!r[u].live) continue;
-      T* o = static_cast<T*>(r[u].key ? d.k_out : d.q_out) + out_offset(d, r[u]);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int c = (n * a.G + lane) * V;
-        float f[V];
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          const float v0 = fmaf(x[u][n][i] * rs, w[n][i], bias[n][i]), v1 = fmaf(x[u][n][i + 1] * rs, w[n][i + 1], bias[n][i + 1]);
-          const int pair = (c + i) >> 1;
-          const float2 e = (r[u].in && pair < d.P) ? cs[(u * a.TS + ts) * d.P + pair] : make_float2(1.f, 0.f);
-          f[i] = r[u].in ? v0 * e.x - v1 * e.y : 0.f;
-          f[i + 1] = r[u].in ? v1 * e.x + v0 * e.y : 0.f;
-        }
-        store_cols<T, V, VEC>(o, c, d.Dh, f);
-      }
-    }
-    __syncthreads();
+  for (int i = 0; i < N; i += 2) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p + 2 * i);
+    f[i] = v.x;
+    f[i + 1] = v.y;
   }
 }
 
-// Shared memory: the angles of U * TS tokens; then (DANG) the pairs' cross products of every row, or (at the end) the
-// rows' sums for the weights. partial: [2 (weight, bias)][gridDim.x (* slices)][width], see norm_rotate_params_kernel.
+// (x, y) turned by (cos, sin) = e
+__device__ __forceinline__ f2 turn(f2 v, float2 e) {
+  float x, y;
+  unpack2(v, x, y);
+  return pack2(x * e.x - y * e.y, fmaf(y, e.x, x * e.y));
+}
+
 template <typename T, int V, bool VEC, int NV, int U>
-__global__ void __launch_bounds__(NT) norm_rotate_bwd_kernel(const NormArgs a, float* partial, float* dang, int has_bias) {
-  extern __shared__ float2 cs[];
+__global__ void __launch_bounds__(NT) norm_rotate_fwd_kernel(const NormArgs a, int w_rows) {
+  using P = Place<T, V, VEC, NV>;
+  using Raw = typename P::Raw;
+  constexpr int N = P::N;
+  extern __shared__ __align__(16) float smem[];
   const BdhNormRotateDesc& d = a.d;
-  float* rowbuf = reinterpret_cast<float*>(cs + U * a.TS * d.P);
-  const int lane = threadIdx.x % a.G, slot = threadIdx.x / a.G;
-  const int ts = slot / a.HS, head = blockIdx.y * a.HS + slot - ts * a.HS;
-  const bool slot_ok = slot < a.TS * a.HS;
-  const bool key = head >= d.Hq;
-  const float* wp = key ? d.k_weight : d.q_weight;
-  const float* bp = key ? d.k_bias : d.q_bias;
-  const long long w_at = a.shared_w ? 0 : static_cast<long long>(key ? head - d.Hq : head) * d.Dh;
-  const bool par = slot_ok && head < a.H;
-  float w[NV][V], gw[NV][V], gb[NV][V];
+  const P me(a);
+  Weights wt;
+  const int pitch = a.G * V * NV;
+  wt.fill(a, smem, pitch, w_rows, me.g0);
+  float2* cs = reinterpret_cast<float2*>(smem + 2 * w_rows * pitch);         // two sets: the tokens' now, and the next ones'
+  const int cs_set = a.TS * d.P;
+  int head[U];
 #pragma unroll
-  for (int n = 0; n < NV; ++n)
+  for (int u = 0; u < U; ++u) head[u] = me.head(a, u);
+  Raw raw[U][NV];
+  const auto load = [&](const Token& k, int u) {
+    const bool key = me.key(a, u);
+    const bool in = k.in && head[u] >= 0;
+    const T* p = key ? static_cast<const T*>(d.k) + k.b * d.k_sb + k.t * d.k_st + head[u] * d.k_sh
+                     : static_cast<const T*>(d.q) + k.b * d.q_sb + k.t * d.q_st + head[u] * d.q_sh;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (n * a.G + lane) * V + i;
-      w[n][i] = (par && wp && c < d.Dh) ? wp[w_at + c] : 1.f;
-      gw[n][i] = gb[n][i] = 0.f;
-    }
-  for (int first = blockIdx.x * a.TS * U; first < a.tokens; first += gridDim.x * a.TS * U) {
-    Row r[U];
-    float x[U][NV][V], g[U][NV][V];
+    for (int n = 0; n < NV; ++n) raw[u][n] = load_cols<T, V, VEC>(p, in ? me.column(a, n) : d.Dh, d.Dh);
+  };
+  const long long stride = static_cast<long long>(gridDim.x) * a.TS;
+  long long first = static_cast<long long>(blockIdx.x) * a.TS;
+  Token now = token_at(a, first + me.ts);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = row_of(a, first + u * a.TS + ts, head, slot_ok);
-      const T* p = static_cast<const T*>(r[u].key ? d.k : d.q) + (r[u].in ? in_offset(d, r[u]) : 0);
-      const T* pd = static_cast<const T*>(r[u].key ? d.dk_out : d.dq_out) + (r[u].in ? out_offset(d, r[u]) : 0);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int c = r[u].in ? (n * a.G + lane) * V : d.Dh;
-        load_cols<T, V, VEC>(p, c, d.Dh, x[u][n]);
-        load_cols<T, V, VEC>(pd, c, d.Dh, g[u][n]);
-      }
-    }
-    fill_angles(a, cs, first, U * a.TS);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float ss = 0.f, dot = 0.f;
-#pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          const int pair = ((n * a.G + lane) * V + i) >> 1;
-          const float2 e = (r[u].in && pair < d.P) ? cs[(u * a.TS + ts) * d.P + pair] : make_float2(1.f, 0.f);
-          const float g0 = g[u][n][i], g1 = g[u][n][i + 1];
-          g[u][n][i] = g0 * e.x + g1 * e.y;                     // dv = R^T do
-          g[u][n][i + 1] = g1 * e.x - g0 * e.y;
-#pragma unroll
-          for (int j = i; j < i + 2; ++j) {
-            ss = fmaf(x[u][n][j], x[u][n][j], ss);
-            dot = fmaf(g[u][n][j] * w[n][j], x[u][n][j], dot);
-          }
-        }
-      const float rs = rsqrtf(group_sum(ss, a.G) / d.Dh + d.eps);
-      const float m = group_sum(dot, a.G) / d.Dh * rs * rs;     // mean(w dv x r) r, per element of x
-      if (!r[u].live) continue;
-      T* o = static_cast<T*>(r[u].key ? d.dk : d.dq) + out_offset(d, r[u]);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int c = (n * a.G + lane) * V;
-        float f[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float dv = g[u][n][i], hat = x[u][n][i] * rs;
-          f[i] = rs * (dv * w[n][i] - x[u][n][i] * m);
-          gw[n][i] = fmaf(dv, hat, gw[n][i]);
-          gb[n][i] += dv;
-        }
-        store_cols<T, V, VEC>(o, c, d.Dh, f);
-        if (dang != nullptr) {
-#pragma unroll
-          for (int i = 0; i < V; i += 2) {
-            if (((c + i) >> 1) >= d.P) continue;
-            const bool hb = bp != nullptr;
-            const float v0 = fmaf(x[u][n][i] * rs, w[n][i], hb ? bp[w_at + c + i] : 0.f);
-            const float v1 = fmaf(x[u][n][i + 1] * rs, w[n][i + 1], hb ? bp[w_at + c + i + 1] : 0.f);
-            rowbuf[(u * a.rows + slot) * d.P + ((c + i) >> 1)] = r[u].in ? v0 * g[u][n][i + 1] - v1 * g[u][n][i] : 0.f;
-          }
-        }
-      }
-    }
-    __syncthreads();
-    if (dang != nullptr) {
-      const int heads = min(a.HS, a.H - static_cast<int>(blockIdx.y) * a.HS);
-      for (int s = threadIdx.x >> 5; s < U * a.TS; s += WARPS) {
-        const int token = first + s, u = s / a.TS;
-        if (token >= a.tokens) break;
-        for (int i = threadIdx.x & 31; i < d.P; i += 32) {
-          float sum = 0.f;
-          for (int h = 0; h < heads; ++h) sum += rowbuf[(u * a.rows + (s - u * a.TS) * a.HS + h) * d.P + i];
-          dang[(static_cast<long long>(blockIdx.y) * a.tokens + token) * d.P + i] = sum;
-        }
-      }
-      __syncthreads();
-    }
-  }
-  if (partial == nullptr) return;
-  // the block's sums: per head over its token slots, or (one weight for all heads) over the slice's query and key rows
-  const int width = a.shared_w ? 2 * d.Dh : a.H * d.Dh;
-  const long long lines = static_cast<long long>(gridDim.x) * (a.shared_w ? gridDim.y : 1);
-  const long long line = a.shared_w ? static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y : blockIdx.x;
-  float* buf = reinterpret_cast<float*>(cs);
-  for (int what = 0; what < (has_bias ? 2 : 1); ++what) {
-    __syncthreads();
+  for (int u = 0; u < U; ++u) load(now, u);
+  fill_angles(a, cs, first);
+  __syncthreads();
+  int set = 0;
+  for (; first < a.tokens; first += stride) {
+    const Token next = token_at(a, first + stride + me.ts);
+    float2 e[NV][N];
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = (n * a.G + lane) * V + i;
-        if (c < d.Dh) buf[slot * d.Dh + c] = what ? gb[n][i] : gw[n][i];
+      for (int i = 0; i < N; ++i) {
+        const int pair = me.column(a, n) / 2 + i;
+        e[n][i] = now.in && me.slot_ok && pair < d.P ? cs[set * cs_set + me.ts * d.P + pair] : make_float2(1.f, 0.f);
       }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= me.ng) break;                                    // (the same for the block)
+      f2 x[NV][N], ss = both(0.f);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        Pairs<T, V>::get(raw[u][n], x[n]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss = fma2(x[n][i], x[n][i], ss);
+      }
+      load(next, u);
+      const float rs = rsqrtf(group_sum(sum2(ss), a.G) / d.Dh + d.eps);
+      if (!now.live || head[u] < 0) continue;
+      const bool key = me.key(a, u);
+      T* o = key ? static_cast<T*>(d.k_out) + ((static_cast<long long>(now.b) * d.T + now.t) * d.Hk + head[u]) * d.Dh
+                 : static_cast<T*>(d.q_out) + ((static_cast<long long>(now.b) * d.T + now.t) * d.Hq + head[u]) * d.Dh;
+      const int wrow = wt.row(a, u, me.hl, key) * pitch;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        f2 w[N], b[N];
+        load_pairs(wt.w + wrow + me.column(a, n), w);
+        load_pairs(wt.b + wrow + me.column(a, n), b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x[n][i] = turn(fma2(mul2(x[n][i], both(rs)), w[i], b[i]), e[n][i]);
+          if (!now.in) x[n][i] = both(0.f);
+        }
+        store_cols<T, V, VEC>(o, me.column(a, n), d.Dh, x[n]);
+      }
+    }
+    if (first + stride < a.tokens) fill_angles(a, cs + (set ^ 1) * cs_set, first + stride);
     __syncthreads();
-    float* out = partial + (what * lines + line) * width;
-    const int heads = min(a.HS, a.H - static_cast<int>(blockIdx.y) * a.HS);
-    if (a.shared_w) {
-      for (int c = threadIdx.x; c < d.Dh; c += NT) {
-        float sq = 0.f, sk = 0.f;
-        for (int s = 0; s < a.TS; ++s)
-          for (int h = 0; h < heads; ++h) {
-            const float v = buf[(s * a.HS + h) * d.Dh + c];
-            if (static_cast<int>(blockIdx.y) * a.HS + h >= d.Hq) sk += v; else sq += v;
-          }
-        out[c] = sq;
-        out[d.Dh + c] = sk;
+    set ^= 1;
+    now = next;
+  }
+}
+
+// Shared memory: weights; two sets of angles; then (dang) the rows' cross products, or (at the end) the rows' sums for the
+// weights. PER_HEAD: a sum for each of the thread's heads; else one for q and one for k. partial: [2 (weight, bias)]
+// [lines][width], see norm_rotate_params_kernel.
+template <typename T, int V, bool VEC, int NV, int U, bool PER_HEAD>
+__global__ void __launch_bounds__(NT) norm_rotate_bwd_kernel(const NormArgs a, int w_rows, float* partial, float* dang, int has_bias) {
+  using P = Place<T, V, VEC, NV>;
+  using Raw = typename P::Raw;
+  constexpr int N = P::N, SUMS = PER_HEAD ? U : 2;
+  extern __shared__ __align__(16) float smem[];
+  const BdhNormRotateDesc& d = a.d;
+  const P me(a);
+  Weights wt;
+  const int pitch = a.G * V * NV;
+  wt.fill(a, smem, pitch, w_rows, me.g0);
+  float2* cs = reinterpret_cast<float2*>(smem + 2 * w_rows * pitch);
+  const int cs_set = a.TS * d.P, rows = a.TS * a.hr, slot = me.ts * a.hr + me.hl;
+  float* rowbuf = reinterpret_cast<float*>(cs + 2 * cs_set);
+  int head[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) head[u] = me.head(a, u);
+  Raw rx[U][NV], rg[U][NV];
+  const auto load = [&](const Token& k, int u) {
+    const bool key = me.key(a, u);
+    const bool in = k.in && head[u] >= 0;
+    const long long at = static_cast<long long>(k.b) * d.T + k.t;
+    const T* p = key ? static_cast<const T*>(d.k) + k.b * d.k_sb + k.t * d.k_st + head[u] * d.k_sh
+                     : static_cast<const T*>(d.q) + k.b * d.q_sb + k.t * d.q_st + head[u] * d.q_sh;
+    const T* g = key ? static_cast<const T*>(d.dk_out) + (at * d.Hk + head[u]) * d.Dh
+                     : static_cast<const T*>(d.dq_out) + (at * d.Hq + head[u]) * d.Dh;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = in ? me.column(a, n) : d.Dh;
+      rx[u][n] = load_cols<T, V, VEC>(p, c, d.Dh);
+      rg[u][n] = load_cols<T, V, VEC>(g, c, d.Dh);
+    }
+  };
+  f2 gw[SUMS][NV][N], gb[SUMS][NV][N];
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < N; ++i) gw[k][n][i] = gb[k][n][i] = both(0.f);
+  const long long stride = static_cast<long long>(gridDim.x) * a.TS;
+  long long first = static_cast<long long>(blockIdx.x) * a.TS;
+  Token now = token_at(a, first + me.ts);
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(now, u);
+  fill_angles(a, cs, first);
+  __syncthreads();
+  int set = 0;
+  for (; first < a.tokens; first += stride) {
+    const Token next = token_at(a, first + stride + me.ts);
+    float2 e[NV][N];
+    float cross[NV][N];
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int pair = me.column(a, n) / 2 + i;
+        e[n][i] = now.in && me.slot_ok && pair < d.P ? cs[set * cs_set + me.ts * d.P + pair] : make_float2(1.f, 0.f);
+        cross[n][i] = 0.f;
       }
-    } else {
-      for (int i = threadIdx.x; i < heads * d.Dh; i += NT) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= me.ng) break;                                    // (the same for the block)
+      const bool key = me.key(a, u);
+      const int wrow = wt.row(a, u, me.hl, key) * pitch;
+      f2 x[NV][N], g[NV][N], w[NV][N], ss = both(0.f), dot = both(0.f);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        Pairs<T, V>::get(rx[u][n], x[n]);
+        Pairs<T, V>::get(rg[u][n], g[n]);
+        if (me.slot_ok) load_pairs(wt.w + wrow + me.column(a, n), w[n]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!me.slot_ok) w[n][i] = both(0.f);
+          g[n][i] = turn(g[n][i], make_float2(e[n][i].x, -e[n][i].y));       // dv = R^T do
+          ss = fma2(x[n][i], x[n][i], ss);
+          dot = fma2(mul2(g[n][i], w[n][i]), x[n][i], dot);
+        }
+      }
+      load(next, u);
+      const float rs = rsqrtf(group_sum(sum2(ss), a.G) / d.Dh + d.eps);
+      const float m = group_sum(sum2(dot), a.G) / d.Dh * rs * rs;            // mean(w dv x r) r, per element of x
+      if (!now.live || head[u] < 0) continue;
+      T* o = key ? static_cast<T*>(d.dk) + ((static_cast<long long>(now.b) * d.T + now.t) * d.Hk + head[u]) * d.Dh
+                 : static_cast<T*>(d.dq) + ((static_cast<long long>(now.b) * d.T + now.t) * d.Hq + head[u]) * d.Dh;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        f2 out[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const f2 hat = mul2(x[n][i], both(rs));
+          out[i] = mul2(both(rs), fma2(x[n][i], both(-m), mul2(g[n][i], w[n][i])));
+          const f2 gh = mul2(g[n][i], hat);
+          if constexpr (PER_HEAD) {
+            gw[u][n][i] = add2(gw[u][n][i], gh);
+            gb[u][n][i] = add2(gb[u][n][i], g[n][i]);
+          } else if (key) {
+            gw[1][n][i] = add2(gw[1][n][i], gh);
+            gb[1][n][i] = add2(gb[1][n][i], g[n][i]);
+          } else {
+            gw[0][n][i] = add2(gw[0][n][i], gh);
+            gb[0][n][i] = add2(gb[0][n][i], g[n][i]);
+          }
+        }
+        if (dang != nullptr && now.in) {
+          f2 b[N];
+          load_pairs(wt.b + wrow + me.column(a, n), b);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            float v0, v1, g0, g1;
+            unpack2(fma2(mul2(x[n][i], both(rs)), w[n][i], b[i]), v0, v1);
+            unpack2(g[n][i], g0, g1);
+            cross[n][i] += v0 * g1 - v1 * g0;
+          }
+        }
+        store_cols<T, V, VEC>(o, me.column(a, n), d.Dh, out);
+      }
+    }
+    if (dang != nullptr) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int pair = me.column(a, n) / 2 + i;
+          if (me.slot_ok && pair < d.P) rowbuf[slot * d.P + pair] = cross[n][i];
+        }
+    }
+    if (first + stride < a.tokens) fill_angles(a, cs + (set ^ 1) * cs_set, first + stride);
+    __syncthreads();
+    if (dang != nullptr) {
+      for (int i = threadIdx.x; i < cs_set; i += NT) {
+        const int s = i / d.P, pair = i - s * d.P;
+        if (first + s >= a.tokens) break;
         float sum = 0.f;
-        for (int s = 0; s < a.TS; ++s) sum += buf[s * a.HS * d.Dh + i];
-        out[static_cast<long long>(blockIdx.y) * a.HS * d.Dh + i] = sum;
+        for (int h = 0; h < a.hr; ++h) sum += rowbuf[(s * a.hr + h) * d.P + pair];
+        dang[(static_cast<long long>(blockIdx.y) * a.tokens + first + s) * d.P + pair] = sum;
+      }
+      __syncthreads();
+    }
+    set ^= 1;
+    now = next;
+  }
+  if (partial == nullptr) return;
+  // the block's sums, over its token slots: of each head, or (one weight for all heads) of q's and of k's rows
+  const int width = d.per_head ? (d.Hq + d.Hk) * d.Dh : 2 * d.Dh;
+  const long long lines = static_cast<long long>(gridDim.x) * (d.per_head ? 1 : gridDim.y);
+  const long long line = d.per_head ? blockIdx.x : static_cast<long long>(blockIdx.x) * gridDim.y + blockIdx.y;
+  float* buf = smem;                                            // [rows][Dh]
+  for (int what = 0; what < (has_bias ? 2 : 1); ++what) {
+    float* out = partial + (what * lines + line) * width;
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) {
+      if (PER_HEAD && k >= me.ng) break;
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = me.column(a, n) + 2 * i;
+          float lo, hi;
+          unpack2(what ? gb[k][n][i] : gw[k][n][i], lo, hi);
+          if (me.slot_ok && c < d.Dh) {
+            buf[slot * d.Dh + c] = lo;
+            buf[slot * d.Dh + c + 1] = hi;
+          }
+        }
+      __syncthreads();
+      if constexpr (PER_HEAD) {
+        const bool key = me.key(a, k);
+        const int h0 = (me.g0 + k - (key ? a.q_groups : 0)) * a.hr, n_heads = min(a.hr, (key ? d.Hk : d.Hq) - h0);
+        for (int i = threadIdx.x; i < n_heads * d.Dh; i += NT) {
+          float sum = 0.f;
+          for (int s = 0; s < a.TS; ++s) sum += buf[s * a.hr * d.Dh + i];
+          out[static_cast<long long>((key ? d.Hq : 0) + h0) * d.Dh + i] = sum;
+        }
+      } else {
+        for (int c = threadIdx.x; c < d.Dh; c += NT) {
+          float sum = 0.f;
+          for (int s = 0; s < rows; ++s) sum += buf[s * d.Dh + c];
+          out[k * d.Dh + c] = sum;
+        }
       }
     }
   }
@@ -380,48 +491,59 @@ int checked(const BdhNormRotateDesc& d) {
   return BDH_OK;
 }
 
-NormArgs args_for(const BdhNormRotateDesc& d, int v, int nv) {
+NormArgs args_for(const BdhNormRotateDesc& d, int v, int nv, int groups_a_block) {
   NormArgs a;
   a.d = d;
   a.len = Lengths{d.lengths, d.lengths64};
   a.tokens = d.B * d.T;
-  a.H = d.Hq + d.Hk;
   a.G = 1;
   while (a.G * v * nv < d.Dh) a.G *= 2;
-  a.rows = NT / a.G;
-  a.slices = (a.H + a.rows - 1) / a.rows;
-  a.HS = (a.H + a.slices - 1) / a.slices;
-  a.TS = a.rows / a.HS;
-  a.shared_w = !d.per_head;
+  const int rows = NT / a.G, most = d.Hq > d.Hk ? d.Hq : d.Hk;
+  a.hr = most < rows ? most : rows;
+  a.TS = rows / a.hr;
+  a.q_groups = (d.Hq + a.hr - 1) / a.hr;
+  a.groups = a.q_groups + (d.Hk + a.hr - 1) / a.hr;
+  a.slices = (a.groups + groups_a_block - 1) / groups_a_block;
+  a.per_block = (a.groups + a.slices - 1) / a.slices;
   return a;
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? BDH_OK : BDH_ERR_LAUNCH; }
 
-// Blocks along the tokens: as many as fill the GPU about `waves` times over, so that the weights are loaded (and their
-// gradients written) a few times per SM and not once per token.
-int token_blocks(const NormArgs& a, int U, int per_sm) {
-  const long long need = (static_cast<long long>(a.tokens) + a.TS * U - 1) / (a.TS * U);
+// Blocks along the tokens: as many as run at once, so that the weights are read (and their gradients written) once per
+// block and not once per token.
+int token_blocks(const NormArgs& a, int per_sm) {
+  const long long need = (static_cast<long long>(a.tokens) + a.TS - 1) / a.TS;
   const long long most = (148LL * per_sm + a.slices - 1) / a.slices;
   return static_cast<int>(need < most ? need : most);
 }
+int weight_rows(const NormArgs& a) { return a.d.per_head ? a.per_block * a.hr : 2; }
+
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return BDH_OK;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess ? BDH_OK
+                                                                                                                          : BDH_ERR_LAUNCH;
+}
+
+constexpr int FEW = 2, MANY = 5;     // groups of heads a block: registers for their rows on the way
 
 template <typename T, int V, bool VEC, int NV, int U>
 int fwd_launch(const BdhNormRotateDesc& d, cudaStream_t s) {
-  const NormArgs a = args_for(d, V, NV);
-  const size_t smem = sizeof(float2) * U * a.TS * d.P;
-  norm_rotate_fwd_kernel<T, V, VEC, NV, U><<<dim3(token_blocks(a, U, 16), a.slices), NT, smem, s>>>(a);
+  const NormArgs a = args_for(d, V, NV, U);
+  const int w_rows = weight_rows(a);
+  const size_t smem = sizeof(float) * 2 * w_rows * a.G * V * NV + sizeof(float2) * 2 * a.TS * d.P;
+  auto kernel = norm_rotate_fwd_kernel<T, V, VEC, NV, U>;
+  if (const int rc = allow_smem(kernel, smem)) return rc;
+  kernel<<<dim3(token_blocks(a, 8), a.slices), NT, smem, s>>>(a, w_rows);
   return launched();
 }
 
-// Four tokens in flight per thread once there are enough of them to fill the GPU that way.
 template <typename T, int V, bool VEC, int NV>
-int fwd_unroll(const BdhNormRotateDesc& d, cudaStream_t s) {
-  if constexpr (NV == 1) {
-    const NormArgs a = args_for(d, V, NV);
-    if (a.tokens >= 4LL * 148 * a.TS) return fwd_launch<T, V, VEC, NV, 4>(d, s);
-  }
-  return fwd_launch<T, V, VEC, NV, 1>(d, s);
+int fwd_groups(const BdhNormRotateDesc& d, cudaStream_t s) {
+  if constexpr (NV == 1)
+    if (args_for(d, V, NV, MANY).groups > FEW) return fwd_launch<T, V, VEC, NV, MANY>(d, s);
+  return fwd_launch<T, V, VEC, NV, FEW>(d, s);
 }
 
 struct BwdOut {
@@ -434,35 +556,34 @@ struct BwdPlan {
   size_t smem;
 };
 
-BwdPlan bwd_plan(const NormArgs& a, int U, bool want_w, bool want_b, bool want_ang) {
+BwdPlan bwd_plan(const NormArgs& a, int v_nv, bool want_w, bool want_b, bool want_ang) {
   BwdPlan p;
-  p.blocks = token_blocks(a, U, 6);
-  p.width = a.shared_w ? 2 * a.d.Dh : a.H * a.d.Dh;
-  p.lines = static_cast<long long>(p.blocks) * (a.shared_w ? a.slices : 1);
+  p.blocks = token_blocks(a, 4);
+  p.width = a.d.per_head ? (a.d.Hq + a.d.Hk) * a.d.Dh : 2 * a.d.Dh;
+  p.lines = static_cast<long long>(p.blocks) * (a.d.per_head ? 1 : a.slices);
   p.partial = (want_w || want_b) ? (want_b ? 2 : 1) * p.lines * p.width : 0;
   p.angles = (want_ang && a.slices > 1) ? static_cast<long long>(a.slices) * a.tokens * a.d.P : 0;
-  const size_t cs = sizeof(float2) * U * a.TS * a.d.P;
-  const size_t rows = sizeof(float) * a.rows * (want_ang ? U * a.d.P : 0);
-  const size_t sums = sizeof(float) * a.rows * a.d.Dh;
-  p.smem = cs + rows > sums ? cs + rows : sums;
+  const size_t work = sizeof(float) * 2 * weight_rows(a) * a.G * v_nv + sizeof(float2) * 2 * a.TS * a.d.P +
+                      sizeof(float) * (want_ang ? a.TS * a.hr * a.d.P : 0);
+  const size_t sums = sizeof(float) * a.TS * a.hr * a.d.Dh;
+  p.smem = work > sums ? work : sums;
   return p;
 }
 
-template <typename T, int V, bool VEC, int NV, int U>
+template <typename T, int V, bool VEC, int NV, int U, bool PER_HEAD>
 int bwd_launch(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
-  const NormArgs a = args_for(d, V, NV);
+  const NormArgs a = args_for(d, V, NV, U);
   const bool want_b = o.dqb || o.dkb, want_w = o.dqw || o.dkw || want_b;
-  const BwdPlan p = bwd_plan(a, U, want_w, want_b, o.dang != nullptr);
+  const BwdPlan p = bwd_plan(a, V * NV, want_w, want_b, o.dang != nullptr);
   float* partial = want_w ? o.scratch : nullptr;
   float* ang = o.dang ? (p.angles ? o.scratch + p.partial : o.dang) : nullptr;
-  auto kernel = norm_rotate_bwd_kernel<T, V, VEC, NV, U>;
-  if (p.smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(p.smem)) != cudaSuccess)
-    return BDH_ERR_LAUNCH;
-  kernel<<<dim3(p.blocks, a.slices), NT, p.smem, s>>>(a, partial, ang, want_b);
+  auto kernel = norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD>;
+  if (const int rc = allow_smem(kernel, p.smem)) return rc;
+  kernel<<<dim3(p.blocks, a.slices), NT, p.smem, s>>>(a, weight_rows(a), partial, ang, want_b);
   if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
   if (want_w) {
     norm_rotate_params_kernel<<<dim3((p.width + 31) / 32, want_b ? 2 : 1), dim3(32, 16), 0, s>>>(
-        partial, p.lines, p.width, a.shared_w ? d.Dh : d.Hq * d.Dh, o.dqw, o.dkw, o.dqb, o.dkb);
+        partial, p.lines, p.width, d.per_head ? d.Hq * d.Dh : d.Dh, o.dqw, o.dkw, o.dqb, o.dkb);
     if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
   }
   if (p.angles) {
@@ -473,12 +594,11 @@ int bwd_launch(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
 }
 
 template <typename T, int V, bool VEC, int NV>
-int bwd_unroll(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
-  if constexpr (NV == 1) {
-    const NormArgs a = args_for(d, V, NV);
-    if (a.tokens >= 2LL * 148 * a.TS) return bwd_launch<T, V, VEC, NV, 2>(d, o, s);
-  }
-  return bwd_launch<T, V, VEC, NV, 1>(d, o, s);
+int bwd_groups(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
+  if (d.per_head) return bwd_launch<T, V, VEC, NV, FEW, true>(d, o, s);
+  if constexpr (NV == 1)
+    if (args_for(d, V, NV, MANY).groups > FEW) return bwd_launch<T, V, VEC, NV, MANY, false>(d, o, s);
+  return bwd_launch<T, V, VEC, NV, FEW, false>(d, o, s);
 }
 
 // The row's width decides how many packs a lane holds (at most 32 lanes a row).
@@ -497,11 +617,11 @@ int by_width(const BdhNormRotateDesc& d, const F& f) {
 
 template <typename T>
 int fwd_type(const BdhNormRotateDesc& d, cudaStream_t s) {
-  return by_width<T>(d, [&](auto v, auto vec, auto nv) { return fwd_unroll<T, decltype(v)::value, decltype(vec)::value, decltype(nv)::value>(d, s); });
+  return by_width<T>(d, [&](auto v, auto vec, auto nv) { return fwd_groups<T, decltype(v)::value, decltype(vec)::value, decltype(nv)::value>(d, s); });
 }
 template <typename T>
 int bwd_type(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
-  return by_width<T>(d, [&](auto v, auto vec, auto nv) { return bwd_unroll<T, decltype(v)::value, decltype(vec)::value, decltype(nv)::value>(d, o, s); });
+  return by_width<T>(d, [&](auto v, auto vec, auto nv) { return bwd_groups<T, decltype(v)::value, decltype(vec)::value, decltype(nv)::value>(d, o, s); });
 }
 
 }  // namespace
@@ -524,14 +644,13 @@ extern "C" long long bdh_norm_rotate_scratch(const BdhNormRotateDesc* d, int wan
   if (d->B < 1 || d->T < 1 || d->Hq < 1 || d->Dh < 2) return 0;
   long long most = 0;
   for (int v : {4, 8})
-    for (int nv : {1, 2, 4}) {
-      if (32 * v * nv < d->Dh) continue;
-      const NormArgs a = args_for(*d, v, nv);
-      for (int U : {1, 2}) {
-        const BwdPlan p = bwd_plan(a, U, want_weight, want_bias, want_angles);
+    for (int nv : {1, 2, 4})
+      for (int groups : {FEW, MANY}) {
+        if (32 * v * nv < d->Dh) continue;
+        const NormArgs a = args_for(*d, v, nv, groups);
+        const BwdPlan p = bwd_plan(a, v * nv, want_weight, want_bias, want_angles);
         most = p.partial + p.angles > most ? p.partial + p.angles : most;
       }
-    }
   return most;
 }
 
