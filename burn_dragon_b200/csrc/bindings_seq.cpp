@@ -71,15 +71,17 @@ int to_int(int64_t v, const char* name) {
 }
 
 // ---- causal convolution ------------------------------------------------------------------------------
+// x: [B, T, C], or [B, C] for one row of each
 BdhConvDesc conv_desc(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
                       bool silu) {
-  const int64_t B = x.size(0), T = x.size(1), C = x.size(2), k = w.size(1);
+  const bool one = x.dim() == 2;
+  const int64_t B = x.size(0), T = one ? 1 : x.size(1), C = x.size(-1), k = w.size(1);
   BdhConvDesc d{};
   d.dtype = elem_type(x, "x");
-  check_rows(x, x, x.scalar_type(), {B, T, C}, "x");
+  check_rows(x, x, x.scalar_type(), x.sizes(), "x");
   check_dense(w, x, at::kFloat, {C, k}, "w");
   check_f32(bias, x, {C}, "bias");
-  d.x = x.const_data_ptr(); d.x_sb = x.stride(0); d.x_st = x.stride(1);
+  d.x = x.const_data_ptr(); d.x_sb = x.stride(0); d.x_st = one ? 0 : x.stride(1);
   d.w = w.const_data_ptr<float>(); d.bias = f32_ptr(bias);
   if (given(state)) {
     check_rows(*state, x, x.scalar_type(), {B, k - 1, C}, "state");
@@ -92,7 +94,7 @@ BdhConvDesc conv_desc(const Tensor& x, const Tensor& w, const OptTensor& bias, c
 }
 
 void set_state_out(BdhConvDesc& d, const Tensor& x, const Tensor& out) {
-  check_rows(out, x, x.scalar_type(), {x.size(0), d.k - 1, x.size(2)}, "state_out");
+  check_rows(out, x, x.scalar_type(), {x.size(0), d.k - 1, x.size(-1)}, "state_out");
   d.state_out = out.data_ptr(); d.state_out_sb = out.stride(0); d.state_out_sr = out.stride(1);
 }
 
@@ -146,10 +148,10 @@ void causal_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, con
                       Tensor& y, Tensor& state_out) {
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [B, C], w: [C, k]");
-  BdhConvDesc d = conv_desc(x.unsqueeze(1), w, bias, state, c10::nullopt, silu);
+  BdhConvDesc d = conv_desc(x, w, bias, state, c10::nullopt, silu);
   check_dense(y, x, x.scalar_type(), x.sizes(), "y");
   d.y = y.data_ptr();
-  set_state_out(d, x.unsqueeze(1), state_out);
+  set_state_out(d, x, state_out);
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
 }
 
@@ -268,23 +270,26 @@ void norm_rotate_bwd(const Tensor& q, const OptTensor& k, const OptTensor& q_wei
 // ---- selective scan ----------------------------------------------------------------------------------
 BdhScanDesc scan_desc(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
                       const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths) {
-  TORCH_CHECK(u.dim() == 3 && A.dim() == 2, "u: [B, T, D], A: [D, N]");
-  const int64_t B = u.size(0), T = u.size(1), D = u.size(2), N = A.size(1);
+  TORCH_CHECK((u.dim() == 3 || u.dim() == 2) && A.dim() == 2, "u: [B, T, D] (or [B, D] for one row of each), A: [D, N]");
+  const bool one = u.dim() == 2;
+  const int64_t B = u.size(0), T = one ? 1 : u.size(1), D = u.size(-1), N = A.size(1);
   const auto type = u.scalar_type();
   BdhScanDesc d{};
   d.dtype = elem_type(u, "u");
-  check_rows(u, u, type, {B, T, D}, "u");
-  check_rows(dt, u, type, {B, T, D}, "dt");
-  check_rows(Bm, u, type, {B, T, N}, "B");
-  check_rows(Cm, u, type, {B, T, N}, "C");
+  check_rows(u, u, type, u.sizes(), "u");
+  check_rows(dt, u, type, u.sizes(), "dt");
+  for (const Tensor* t : {&Bm, &Cm}) {
+    if (one) check_rows(*t, u, type, {B, N}, "B, C");
+    else check_rows(*t, u, type, {B, T, N}, "B, C");
+  }
   check_dense(A, u, at::kFloat, {D, N}, "A");
   check_f32(skip, u, {D}, "D");
   check_f32(dt_bias, u, {D}, "dt_bias");
   check_f32(h0, u, {B, D, N}, "h0");
-  d.u = u.const_data_ptr(); d.u_sb = u.stride(0); d.u_st = u.stride(1);
-  d.dt = dt.const_data_ptr(); d.dt_sb = dt.stride(0); d.dt_st = dt.stride(1);
-  d.B_ = Bm.const_data_ptr(); d.b_sb = Bm.stride(0); d.b_st = Bm.stride(1);
-  d.C_ = Cm.const_data_ptr(); d.c_sb = Cm.stride(0); d.c_st = Cm.stride(1);
+  d.u = u.const_data_ptr(); d.u_sb = u.stride(0); d.u_st = one ? 0 : u.stride(1);
+  d.dt = dt.const_data_ptr(); d.dt_sb = dt.stride(0); d.dt_st = one ? 0 : dt.stride(1);
+  d.B_ = Bm.const_data_ptr(); d.b_sb = Bm.stride(0); d.b_st = one ? 0 : Bm.stride(1);
+  d.C_ = Cm.const_data_ptr(); d.c_sb = Cm.stride(0); d.c_st = one ? 0 : Cm.stride(1);
   d.A = A.const_data_ptr<float>(); d.skip = f32_ptr(skip); d.dt_bias = f32_ptr(dt_bias); d.h0 = f32_ptr(h0);
   set_lengths(lengths, u, B, d.lengths, d.lengths64);
   d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.D = to_int(D, "D"); d.N = to_int(N, "N");
@@ -311,6 +316,7 @@ void selective_scan_fwd(const Tensor& u, const Tensor& dt, const Tensor& A, cons
                         const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths, Tensor& y, Tensor& hT,
                         const OptTensor& marks, const OptTensor& scratch) {
   c10::cuda::CUDAGuard guard(u.device());
+  TORCH_CHECK(u.dim() == 3, "u: [B, T, D]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
   check_dense(y, u, u.scalar_type(), u.sizes(), "y");
   check_dense(hT, u, at::kFloat, {d.B, d.D, d.N}, "hT");
@@ -326,6 +332,7 @@ void selective_scan_bwd(const Tensor& u, const Tensor& dt, const Tensor& A, cons
                         const Tensor& scratch, const Tensor& dy, const OptTensor& dhT, Tensor& du, Tensor& ddt, Tensor& dA, Tensor& dB,
                         Tensor& dC, const OptTensor& dskip, const OptTensor& ddt_bias, const OptTensor& dh0) {
   c10::cuda::CUDAGuard guard(u.device());
+  TORCH_CHECK(u.dim() == 3, "u: [B, T, D]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
   const auto type = u.scalar_type();
   check_rows(dy, u, type, u.sizes(), "dy");
@@ -351,8 +358,7 @@ void selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, con
                          const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& active, Tensor& y, Tensor& out) {
   c10::cuda::CUDAGuard guard(u.device());
   TORCH_CHECK(u.dim() == 2 && dt.dim() == 2 && Bm.dim() == 2 && Cm.dim() == 2, "u, dt: [B, D], B, C: [B, N]");
-  BdhScanDesc d = scan_desc(u.unsqueeze(1), dt.unsqueeze(1), A, Bm.unsqueeze(1), Cm.unsqueeze(1), skip, dt_bias, softplus, c10::nullopt,
-                            c10::nullopt);
+  BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, c10::nullopt, c10::nullopt);
   check_dense(y, u, u.scalar_type(), u.sizes(), "y");
   d.y = y.data_ptr();
   for (const Tensor* t : {&h, static_cast<const Tensor*>(&out)}) {

@@ -55,14 +55,20 @@ struct Taps {
   static constexpr int KM = K ? K : 8, N = (V + 1) / 2;
   static_assert(KM - 1 <= R, "a window lies within two sets of rows");
   f2 w[KM][N], bias[N];
+  f2 first[K ? 1 : KM][N];             // K = 0: the taps again, from the window's start on
+  __device__ __forceinline__ f2 tap(int j, int n) const { return K ? w[j][n] : first[K ? 0 : j][n]; }
   __device__ __forceinline__ void load(const BdhConvDesc& d, int k, int c, bool live) {
-    const auto one = [&](int j, int v) { return (live && v < V && j >= KM - k) ? d.w[static_cast<long long>(c + v) * k + j - (KM - k)] : 0.f; };
+    const auto one = [&](int j, int v) { return (live && v < V && j >= KM - k && j < KM) ? d.w[static_cast<long long>(c + v) * k + j - (KM - k)] : 0.f; };
     const auto off = [&](int v) { return (live && v < V && d.bias) ? d.bias[c + v] : 0.f; };
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int j = 0; j < KM; ++j) w[j][n] = pack2(one(j, 2 * n), one(j, 2 * n + 1));
       bias[n] = pack2(off(2 * n), off(2 * n + 1));
+      if constexpr (K == 0) {
+#pragma unroll
+        for (int j = 0; j < KM; ++j) first[j][n] = pack2(one(j + KM - k, 2 * n), one(j + KM - k, 2 * n + 1));
+      }
     }
   }
   __device__ __forceinline__ f2 pre(const f2 (&before)[R][N], const f2 (&s)[R][N], int r, int n, int k) const {
@@ -202,19 +208,6 @@ struct BwdTile {
     if constexpr (RINGS) copy_close();
   }
 
-  // d pre of the row that tap j reaches back to: K known at compile time, or found among the (at most 8) rows behind
-  __device__ __forceinline__ f2 back(const f2 (&gp)[R][N], const f2 (&g)[R][N], int r, int j, int n) const {
-    if constexpr (K != 0) {
-      return W::at(gp, g, r - j, n);
-    } else {
-      f2 x = both(0.f);
-#pragma unroll
-      for (int i = 0; i < KM; ++i)
-        if (i == j - (KM - k)) x = W::at(gp, g, r - i, n);
-      return x;
-    }
-  }
-
   // One set of rows. Which of a tile's sets it is decides at compile time what INSIDE needs no test for: the first
   // completes no row before t0, the last (behind t1) gives d pre only.
   template <int SET>
@@ -265,7 +258,7 @@ struct BwdTile {
           o[n] = both(0.f);
 #pragma unroll
           for (int j = 0; j < KM; ++j)                                       // tap j of output row + (k - 1) - j
-            if (K || j >= KM - k) o[n] = fma2(w.w[j][n], back(gp, g, r, j, n), o[n]);
+            if (K || j < k) o[n] = fma2(w.tap(j, n), W::at(gp, g, r - j, n), o[n]);
         }
         const int j = row - (len - (k - 1));                                 // its place in the new state
         if (!INSIDE && d.dstate_out != nullptr && j >= 0 && j < k - 1) {

@@ -122,14 +122,17 @@ def _causal_conv_fwd(x, w, bias, state, lengths, silu):
 
 
 def _check_conv(x, w, bias, activation, dims: int) -> bool:
-    A.require(x.dim() == dims and x.is_floating_point(), f"x: expected a floating tensor of {dims} dimensions, got {x.dtype} {tuple(x.shape)}")
+    if not (x.dim() == dims and x.is_floating_point()):
+        raise ValueError(f"x: expected a floating tensor of {dims} dimensions, got {x.dtype} {tuple(x.shape)}")
     C = x.shape[-1]
-    A.require(w.dim() == 2 and w.shape[0] == C and 1 <= w.shape[1] <= 8,
-              f"w: expected [{C}, k] with k in 1..8, got {tuple(w.shape)}")
-    A.require(C >= 1, "x: expected at least one channel")
+    if not (w.dim() == 2 and w.shape[0] == C and 1 <= w.shape[1] <= 8):
+        raise ValueError(f"w: expected [{C}, k] with k in 1..8, got {tuple(w.shape)}")
+    if not (C >= 1):
+        raise ValueError("x: expected at least one channel")
     A.check_like(w, x, w.shape, "w")
     A.check_like(bias, x, (C,), "bias")
-    A.require(activation in (None, "silu"), f"activation: expected None or 'silu', got {activation!r}")
+    if not (activation in (None, "silu")):
+        raise ValueError(f"activation: expected None or 'silu', got {activation!r}")
     return activation == "silu"
 
 
@@ -163,14 +166,16 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias
     A.check_like(state, x, (B, k - 1, C), "state", x.dtype)
     active = A.check_active(active, x, B)
     A.check_out(out, state, "out")
-    A.require(not A.wants_grad(x, state, w, bias), "causal_conv_step has no gradient: call it under torch.no_grad(), or use causal_conv")
+    if A.wants_grad(x, state, w, bias):
+        raise ValueError("causal_conv_step has no gradient: call it under torch.no_grad(), or use causal_conv")
     if not A.on_kernels(x):
         y, new = causal_conv_reference(x.unsqueeze(1), w, bias, state, None, activation)
         y = y[:, 0]
         if active is not None:
             y, new = torch.where(active[:, None], y, 0.0), torch.where(active[:, None, None], new, state)
         return y, (new if out is None else out.copy_(new))
-    A.require(out is None or C == 1 or out.stride(-1) == 1, "out: its channels must be adjacent")
+    if not (out is None or C == 1 or out.stride(-1) == 1):
+        raise ValueError("out: its channels must be adjacent")
     y = torch.empty(B, C, device=x.device, dtype=x.dtype)
     new = torch.empty(B, k - 1, C, device=x.device, dtype=x.dtype) if out is None else out
     native.ops.causal_conv_step(A.adjacent(x), A.adjacent(state), A.dense_f32(w), A.dense_f32(bias), active, silu, y, new)

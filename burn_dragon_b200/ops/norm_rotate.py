@@ -110,41 +110,57 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     Rotation, if any: `angles` [B, T, pairs] in radians, or `freqs` [2 * pairs] in cycles per position with `positions`
     - the first token's (an int), or [T] or [B, T] integers (the single-token form has T = 1 and one position a stream).
     `lengths` [B]: rows behind a sequence's length give 0 and take no part in any gradient."""
-    A.require(q.dim() == 4 and q.is_floating_point(), f"q: expected a floating [B, T, heads, Dh] tensor, got {q.dtype} {tuple(q.shape)}")
+    if not (q.dim() == 4 and q.is_floating_point()):
+        raise ValueError(f"q: expected a floating [B, T, heads, Dh] tensor, got {q.dtype} {tuple(q.shape)}")
     B, T, Hq, Dh = q.shape
-    A.require(Hq >= 1 and Dh >= 2 and Dh % 2 == 0 and Dh <= 512, f"q: expected at least one head and an even Dh up to 512, got {tuple(q.shape)}")
-    A.require(k is None or (k.dim() == 4 and k.shape[2] >= 1), "k: expected [B, T, heads, Dh]")
+    if not (Hq >= 1 and Dh >= 2 and Dh % 2 == 0 and Dh <= 512):
+        raise ValueError(f"q: expected at least one head and an even Dh up to 512, got {tuple(q.shape)}")
+    if not (k is None or (k.dim() == 4 and k.shape[2] >= 1)):
+        raise ValueError("k: expected [B, T, heads, Dh]")
     Hk = k.shape[2] if k is not None else 0
     A.check_like(k, q, (B, T, Hk, Dh), "k", q.dtype)
-    A.require(k is not None or (k_weight is None and k_bias is None), "k_weight and k_bias come with k")
+    if not (k is not None or (k_weight is None and k_bias is None)):
+        raise ValueError("k_weight and k_bias come with k")
     params = ((q_weight, Hq, "q_weight"), (k_weight, Hk, "k_weight"), (q_bias, Hq, "q_bias"), (k_bias, Hk, "k_bias"))
     per_head = any(t is not None and t.dim() == 2 for t, _, _ in params)
     for t, H, name in params:
         A.check_like(t, q, (H, Dh) if per_head else (Dh,), name)
-    A.require(angles is None or freqs is None, "angles and freqs: one of the two at most")
+    if not (angles is None or freqs is None):
+        raise ValueError("angles and freqs: one of the two at most")
     pos0 = 0
     if angles is not None:
-        A.require(angles.dim() == 3 and 2 * angles.shape[2] <= Dh, f"angles: expected [B, T, pairs] with pairs up to {Dh // 2}, got {tuple(angles.shape)}")
+        if not (angles.dim() == 3 and 2 * angles.shape[2] <= Dh):
+            raise ValueError(f"angles: expected [B, T, pairs] with pairs up to {Dh // 2}, got {tuple(angles.shape)}")
         A.check_like(angles, q, (B, T, angles.shape[2]), "angles")
-        A.require(isinstance(positions, int) and positions == 0, "positions come with freqs")
+        if not (isinstance(positions, int) and positions == 0):
+            raise ValueError("positions come with freqs")
     elif freqs is not None:
-        A.require(freqs.dim() == 1 and freqs.shape[0] % 2 == 0 and freqs.shape[0] <= Dh, f"freqs: expected an even number up to {Dh}, got {tuple(freqs.shape)}")
+        if not (freqs.dim() == 1 and freqs.shape[0] % 2 == 0 and freqs.shape[0] <= Dh):
+            raise ValueError(f"freqs: expected an even number up to {Dh}, got {tuple(freqs.shape)}")
         A.check_like(freqs, q, freqs.shape, "freqs")
-        A.require(not A.wants_grad(freqs), "freqs has no gradient; pass angles")
+        if A.wants_grad(freqs):
+            raise ValueError("freqs has no gradient; pass angles")
         if isinstance(positions, torch.Tensor):
-            A.require(positions.dtype in (torch.int32, torch.int64), f"positions: expected int32 or int64, got {positions.dtype}")
-            A.require(tuple(positions.shape) in ((T,), (B, T)), f"positions: expected {(T,)} or {(B, T)}, got {tuple(positions.shape)}")
-            A.require(positions.device == q.device, f"positions is on {positions.device}, expected {q.device}")
+            if not (positions.dtype in (torch.int32, torch.int64)):
+                raise ValueError(f"positions: expected int32 or int64, got {positions.dtype}")
+            if not (tuple(positions.shape) in ((T,), (B, T))):
+                raise ValueError(f"positions: expected {(T,)} or {(B, T)}, got {tuple(positions.shape)}")
+            if not (positions.device == q.device):
+                raise ValueError(f"positions is on {positions.device}, expected {q.device}")
         else:
             pos0 = int(positions)
     else:
-        A.require(isinstance(positions, int) and positions == 0, "positions come with freqs")
+        if not (isinstance(positions, int) and positions == 0):
+            raise ValueError("positions come with freqs")
     lengths = A.check_lengths(lengths, q, B)
     if not A.on_kernels(q):
         return norm_rotate_reference(q, k, q_weight, k_weight, q_bias, k_bias, angles=angles, freqs=freqs, positions=positions,
                                      lengths=lengths, eps=eps)
-    A.require(B * T <= 1 << 30, "more than 2^30 tokens")
-    pos = positions.expand(B, T) if isinstance(positions, torch.Tensor) else None
+    if not (B * T <= 1 << 30):
+        raise ValueError("more than 2^30 tokens")
+    pos = None
+    if isinstance(positions, torch.Tensor):
+        pos = positions if positions.dim() == 2 else positions.expand(B, T)
     args = (A.adjacent(q), A.adjacent(k), A.dense_f32(q_weight), A.dense_f32(k_weight), A.dense_f32(q_bias), A.dense_f32(k_bias),
             A.adjacent(angles.float()) if angles is not None else None, A.dense_f32(freqs), pos, pos0, lengths, float(eps))
     if A.wants_grad(q, k, q_weight, k_weight, q_bias, k_bias, angles):

@@ -91,10 +91,13 @@ class _SelectiveScan(torch.autograd.Function):
 
 
 def _check(u, dt, A, Bm, Cm, D, dt_bias, dims: int) -> Tuple[int, int, int]:
-    A_.require(u.dim() == dims and u.is_floating_point(), f"u: expected a floating tensor of {dims} dimensions, got {u.dtype} {tuple(u.shape)}")
+    if not (u.dim() == dims and u.is_floating_point()):
+        raise ValueError(f"u: expected a floating tensor of {dims} dimensions, got {u.dtype} {tuple(u.shape)}")
     Dn = u.shape[-1]
-    A_.require(Dn >= 1, "u: expected at least one channel")
-    A_.require(A.dim() == 2 and A.shape[0] == Dn and 1 <= A.shape[1] <= 64, f"A: expected [{Dn}, N] with N in 1..64, got {tuple(A.shape)}")
+    if not (Dn >= 1):
+        raise ValueError("u: expected at least one channel")
+    if not (A.dim() == 2 and A.shape[0] == Dn and 1 <= A.shape[1] <= 64):
+        raise ValueError(f"A: expected [{Dn}, N] with N in 1..64, got {tuple(A.shape)}")
     rows, N = u.shape[:-1], A.shape[1]
     A_.check_like(A, u, A.shape, "A")
     A_.check_like(dt, u, u.shape, "dt", u.dtype)
@@ -141,8 +144,8 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
     A_.check_like(h, u, (B, Dn, N), "h", _state_type(u))
     active = A_.check_active(active, u, B)
     A_.check_out(out, h, "out")
-    A_.require(not A_.wants_grad(u, dt, A, Bm, Cm, h, D, dt_bias),
-               "selective_scan_step has no gradient: call it under torch.no_grad(), or use selective_scan")
+    if A_.wants_grad(u, dt, A, Bm, Cm, h, D, dt_bias):
+        raise ValueError("selective_scan_step has no gradient: call it under torch.no_grad(), or use selective_scan")
     if not A_.on_kernels(u):
         row = lambda t: t.unsqueeze(1)                                                                   # noqa: E731
         y, new = selective_scan_reference(row(u), row(dt), A, row(Bm), row(Cm), D, dt_bias=dt_bias, dt_softplus=dt_softplus, h0=h)
@@ -151,7 +154,8 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
             y, new = torch.where(active[:, None], y, 0.0), torch.where(active[:, None, None], new, h)
         return y, (new if out is None else out.copy_(new))
     dense = lambda t: (N == 1 or t.stride(2) == 1) and (Dn == 1 or t.stride(1) == N)                     # noqa: E731
-    A_.require(out is None or dense(out), "out: each stream's [D, N] must be dense")
+    if not (out is None or dense(out)):
+        raise ValueError("out: each stream's [D, N] must be dense")
     h = h if dense(h) else h.contiguous()
     y = torch.empty(B, Dn, device=u.device, dtype=u.dtype)
     new = torch.empty(B, Dn, N, device=u.device, dtype=torch.float32) if out is None else out

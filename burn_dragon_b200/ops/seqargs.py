@@ -10,11 +10,6 @@ from . import native
 KERNEL_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def require(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def on_kernels(t: torch.Tensor) -> bool:
     """Do calls with this tensor run on the CUDA kernels? (float64 and CPU tensors take the torch statement.)"""
     return t.is_cuda and t.dtype in KERNEL_TYPES and native.load()
@@ -80,11 +75,13 @@ def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None
     if out is None:
         return
     check_like(out, src, src.shape, name, src.dtype)
-    require(not (torch.is_grad_enabled() and out.requires_grad), f"{name} requires a gradient; a step form has none")
+    if not (not (torch.is_grad_enabled() and out.requires_grad)):
+        raise ValueError(f"{name} requires a gradient; a step form has none")
     same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
-    require(all(st > 0 or n <= 1 for st, n in zip(out.stride(), out.shape)), f"{name}: its rows overlap one another")
+    if not (all(st > 0 or n <= 1 for st, n in zip(out.stride(), out.shape))):
+        raise ValueError(f"{name}: its rows overlap one another")
     if not same and out.numel():
         span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
         (a0, a1), (b0, b1) = span(out), span(src)
-        require(a1 <= b0 or b1 <= a0 or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr(),
-                f"{name} overlaps the state without being it")
+        if not (a1 <= b0 or b1 <= a0 or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr()):
+            raise ValueError(f"{name} overlaps the state without being it")
