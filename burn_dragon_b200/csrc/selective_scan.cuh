@@ -195,8 +195,14 @@ struct Tile {
   __device__ __forceinline__ Pack<T, S::V> u(int i) const { return bits<S::V>(ru[i]); }
   __device__ __forceinline__ Pack<T, S::V> dt(int i) const { return bits<S::V>(rdt[i]); }
   __device__ __forceinline__ Pack<T, S::V> dy(int i) const { return bits<S::V>(rdy[i]); }
-  __device__ __forceinline__ Pack<T, 4> B(int i) const { return bits<4>(rB[i]); }
-  __device__ __forceinline__ Pack<T, 4> C(int i) const { return bits<4>(rC[i]); }
+  __device__ __forceinline__ void put_bc(T* B, T* C) const {
+    const int at = (threadIdx.x & 31) * (S::NP / 2);
+#pragma unroll
+    for (int i = 0; i < S::NB; ++i) {
+      *reinterpret_cast<Raw4*>(B + at + 4 * i) = rB[i];
+      *reinterpret_cast<Raw4*>(C + at + 4 * i) = rC[i];
+    }
+  }
 };
 
 // The same in shared memory, fetched by asynchronous copies RING - 1 tiles ahead: a warp alone on its scheduler takes less
@@ -256,18 +262,17 @@ struct Ring {
     __device__ __forceinline__ Pack<T, S::V> u(int i) const { return get<S::V>(s.u + lane() * S::E + i * S::V); }
     __device__ __forceinline__ Pack<T, S::V> dt(int i) const { return get<S::V>(s.dt + lane() * S::E + i * S::V); }
     __device__ __forceinline__ Pack<T, S::V> dy(int i) const { return get<S::V>(s.dy + lane() * S::E + i * S::V); }
-    __device__ __forceinline__ Pack<T, 4> B(int i) const { return get<4>(s.B + lane() * (S::NP / 2) + 4 * i); }
-    __device__ __forceinline__ Pack<T, 4> C(int i) const { return get<4>(s.C + lane() * (S::NP / 2) + 4 * i); }
   };
   __device__ __forceinline__ View at(int tile) const { return View{stage[tile % RING]}; }
 };
 
 // What a warp's compute loop reads. Rows are padded by 16 bytes, so that eight lanes that store four rows meet no bank twice.
+// (B and C are read as they came: made fp32 beside this they cost more shared memory and stores than the conversions,
+// 16 states 5 %, 64 states 2.7 times.)
 template <int G, int CT, bool DY>
 struct alignas(16) WarpMem {
   static constexpr int NP = 4 * G, CW = 32 / G * CT;
   float2 step[LT][CW + 2];                             // dt', dt' u
-  float B[LT][NP], C[LT][NP];
   float dy[DY ? LT : 1][CW + 4];
   float bias[CW], skip[CW];
 
@@ -279,10 +284,10 @@ struct alignas(16) WarpMem {
   }
   // Rows behind `len` get dt' = 0: the states stay as they are. (Channels behind D need nothing: their u, dy and A
   // read as 0.)
-  template <typename T, bool WANT_B, bool WANT_C, typename Source>
+  template <typename T, typename Source>
   __device__ __forceinline__ void put(const BdhScanDesc& d, const Source& x, int t0, int len) {
     using S = Shape<T, G, CT>;
-    const int lane = threadIdx.x & 31, t = lane / 2, c = (lane & 1) * S::E, n = (lane & 1) * (NP / 2);
+    const int lane = threadIdx.x & 31, t = lane / 2, c = (lane & 1) * S::E;
     const float keep = t0 + t < len ? 1.f : 0.f;
     float dt[S::E + 1], uu[S::E + 1];
     dt[S::E] = uu[S::E] = 0.f;
@@ -314,17 +319,6 @@ struct alignas(16) WarpMem {
         const Pack<T, S::V> p = x.dy(i);
 #pragma unroll
         for (int j = 0; j < S::V; ++j) dy[t][c + i * S::V + j] = p[j];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < S::NB; ++i) {
-      if constexpr (WANT_B) {
-        const Pack<T, 4> p = x.B(i);
-        *reinterpret_cast<float4*>(&B[t][n + 4 * i]) = make_float4(p[0], p[1], p[2], p[3]);
-      }
-      if constexpr (WANT_C) {
-        const Pack<T, 4> p = x.C(i);
-        *reinterpret_cast<float4*>(&C[t][n + 4 * i]) = make_float4(p[0], p[1], p[2], p[3]);
       }
     }
   }
@@ -398,27 +392,37 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
 
 // The factors of a few steps, made ahead of the chain through h: its loads must not stand behind the stores of the steps
 // before, which the compiler cannot tell from them.
-template <int G, int CT, bool DY, bool WANT_C>
+template <int G, int CT, bool WANT_C>
 struct Steps {
   static constexpr int N = 4 / CT;
   f2 e[N][CT][2], in[N][CT][2], k[WANT_C ? N : 1][2];
-  __device__ __forceinline__ void make(const WarpMem<G, CT, DY>& sh, int t, int cl, int n0, const f2 (&A2)[CT][2]) {
+  template <typename Mem, typename Rows>
+  __device__ __forceinline__ void make(const Mem& sh, const Rows& rows, int t, int cl, int n0, const f2 (&A2)[CT][2]) {
 #pragma unroll
     for (int s = 0; s < N; ++s) {
       float dt[CT], du[CT];
-      f2 b0, b1;
+      f2 b[2];
       sh.steps(t + s, cl, dt, du);
-      load4(&sh.B[t + s][n0], b0, b1);
-      if constexpr (WANT_C) load4(&sh.C[t + s][n0], k[s][0], k[s][1]);
+      rows.B(t + s, n0, b);
+      if constexpr (WANT_C) rows.C(t + s, n0, k[s]);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         e[s][c][0] = ex2x2(mul1(dt[c], A2[c][0]));
         e[s][c][1] = ex2x2(mul1(dt[c], A2[c][1]));
-        in[s][c][0] = mul1(du[c], b0);
-        in[s][c][1] = mul1(du[c], b1);
+        in[s][c][0] = mul1(du[c], b[0]);
+        in[s][c][1] = mul1(du[c], b[1]);
       }
     }
   }
+};
+
+// This lane's states of B and C at a step of rows [LT][NP]
+template <typename T, int NP>
+struct RowsOf {
+  const T *b, *c;
+  static __device__ __forceinline__ void get(const T* p, f2 (&f)[2]) { Pairs<T, 4>::get(*reinterpret_cast<const typename Pack<T, 4>::Raw*>(p), f); }
+  __device__ __forceinline__ void B(int t, int n0, f2 (&f)[2]) const { get(b + t * NP + n0, f); }
+  __device__ __forceinline__ void C(int t, int n0, f2 (&f)[2]) const { get(c + t * NP + n0, f); }
 };
 
 struct Where {
@@ -471,8 +475,9 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
     const int t0 = tile * LT;
     if (tile < end) {
       copy_wait<RING - 2>();
-      sh.in.template put<T, true, true>(d, sh.ring.at(tile), t0, len);
+      sh.in.template put<T>(d, sh.ring.at(tile), t0, len);
       __syncwarp();
+      const RowsOf<T, S::NP> bc{sh.ring.at(tile).s.B, sh.ring.at(tile).s.C};
       sh.ring.template load<true, true>(d, tile + RING - 1, end, w.b, c0, len);
       if (marks != nullptr)
 #pragma unroll
@@ -480,12 +485,12 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
           if (c + k < d.D)
             *reinterpret_cast<ulonglong2*>(marks + ((static_cast<long long>(w.b) * a.tiles + tile) * d.D + c + k) * S::NP + n0) =
                 make_ulonglong2(h[k][0], h[k][1]);
-      using Group = Steps<G, CT, false, true>;
+      using Group = Steps<G, CT, true>;
       Group now, next;
-      now.make(sh.in, 0, cl, n0, A2);
+      now.make(sh.in, bc, 0, cl, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, s0 + Group::N, cl, n0, A2);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
@@ -572,8 +577,9 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
   for (int i = 0; i < n; ++i) {
     const int tile = tile_of(i);
     copy_wait<RING - 2>();
-    sh.in.template put<T, !REV, REV>(d, sh.ring.at(tile), tile * LT, len);
+    sh.in.template put<T>(d, sh.ring.at(tile), tile * LT, len);
     __syncwarp();
+    const RowsOf<T, S::NP> bc{sh.ring.at(tile).s.B, sh.ring.at(tile).s.C};
     sh.ring.template load<!REV, REV>(d, i + RING - 1 < n ? tile_of(i + RING - 1) : -1, end, w.b, c0, len);
     constexpr int GS = 8 / CT;
 #pragma unroll
@@ -583,16 +589,20 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
       for (int s = 0; s < GS; ++s) {
         const int t = REV ? LT - 1 - s0 - s : s0 + s;
         float dt[CT], du[CT];
-        f2 b0, b1;
+        f2 b[2];
         sh.in.steps(t, cl, dt, du);
-        load4(REV ? &sh.in.C[t][n0] : &sh.in.B[t][n0], b0, b1);
-        if constexpr (REV) sh.in.dys(t, cl, du);
+        if constexpr (REV) {
+          bc.C(t, n0, b);
+          sh.in.dys(t, cl, du);
+        } else {
+          bc.B(t, n0, b);
+        }
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
           e[s][k][0] = ex2x2(mul1(dt[k], A2[k][0]));
           e[s][k][1] = ex2x2(mul1(dt[k], A2[k][1]));
-          in[s][k][0] = mul1(du[k], b0);
-          in[s][k][1] = mul1(du[k], b1);
+          in[s][k][0] = mul1(du[k], b[0]);
+          in[s][k][1] = mul1(du[k], b[1]);
           total[k] += dt[k];
         }
       }
@@ -623,28 +633,30 @@ struct ScanGrads {
   float* per_channel;                  // [2][B][segs][D]: partial dD, dbias
 };
 
-template <int G, int CT>
+template <typename T, int G, int CT>
 struct BwdMem {
   static constexpr int NP = 4 * G, CW = 32 / G * CT;
   struct PerWarp {
     WarpMem<G, CT, true> in;
+    alignas(16) T B[LT * NP], C[LT * NP];
     float2 out[LT][CW + 2];            // sum g B, sum A2 q
     ulonglong2 h[LT][CT][32];          // h_{t-1}, each lane its own
+    __device__ __forceinline__ RowsOf<T, NP> bc() const { return {B, C}; }
   } warp[BWD_WARPS];
   alignas(16) float bc[BWD_WARPS][LT][2 * NP];     // the warps' sums over their channels
 };
 
 // What a step of the reverse walk reads
-template <int G, int CT>
+template <typename T, int G, int CT>
 struct BwdStep {
   float dt[CT], du[CT], gy[CT];
   f2 b[2], c[2];
   ulonglong2 h[CT];
-  __device__ __forceinline__ void load(const typename BwdMem<G, CT>::PerWarp& sh, int t, int lane, int cl, int n0) {
+  __device__ __forceinline__ void load(const typename BwdMem<T, G, CT>::PerWarp& sh, int t, int lane, int cl, int n0) {
     sh.in.steps(t, cl, dt, du);
     sh.in.dys(t, cl, gy);
-    load4(&sh.in.B[t][n0], b[0], b[1]);
-    load4(&sh.in.C[t][n0], c[0], c[1]);
+    sh.bc().B(t, n0, b);
+    sh.bc().C(t, n0, c);
 #pragma unroll
     for (int k = 0; k < CT; ++k) h[k] = sh.h[t][k][lane];
   }
@@ -654,9 +666,9 @@ template <typename T, int G, int CT, bool VEC>
 __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd_kernel(const ScanArgs a, const ScanGrads o) {
   using S = Shape<T, G, CT>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  BwdMem<G, CT>& all = *reinterpret_cast<BwdMem<G, CT>*>(smem_raw);
+  BwdMem<T, G, CT>& all = *reinterpret_cast<BwdMem<T, G, CT>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  typename BwdMem<G, CT>::PerWarp& sh = all.warp[warp];
+  typename BwdMem<T, G, CT>::PerWarp& sh = all.warp[warp];
   const BdhScanDesc& d = a.d;
   const Where w = where(a, blockIdx.x);
   const int n0 = lane % G * 4, cl = lane / G * CT, c0 = (w.part * BWD_WARPS + warp) * S::CW, c = c0 + cl;
@@ -700,7 +712,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
     }
     if (any) {
       f2 h[CT][2], dat[CT][2];
-      sh.in.template put<T, true, true>(d, x, t0, len);
+      sh.in.template put<T>(d, x, t0, len);
+      x.put_bc(sh.B, sh.C);
 #pragma unroll
       for (int k = 0; k < CT; ++k) {
         h[k][0] = mark[k][0];
@@ -712,12 +725,13 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
         x.load(d, w.b, c0, t0 - LT, len);
         load_marks(tile - 1);
       }
-      using Group = Steps<G, CT, true, false>;
+      using Group = Steps<G, CT, false>;
+      const RowsOf<T, S::NP> bc = sh.bc();
       Group now, next;
-      now.make(sh.in, 0, cl, n0, A2);
+      now.make(sh.in, bc, 0, cl, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, s0 + Group::N, cl, n0, A2);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
@@ -728,7 +742,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           }
         now = next;
       }
-      BwdStep<G, CT> at_t, before;
+      BwdStep<T, G, CT> at_t, before;
       at_t.load(sh, LT - 1, lane, cl, n0);
 #pragma unroll 4
       for (int t = LT - 1; t >= 0; --t) {
@@ -893,56 +907,80 @@ __global__ void __launch_bounds__(256) selective_scan_params_kernel(const float*
 }
 
 // ---- one token ---------------------------------------------------------------------------------------
-// Bound by the states: 4 B N D read and written per stream.
-template <typename T, int G>
-__global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const BdhScanDesc d, const float* h, long long h_sb, float* out, long long out_sb,
-                                                                 const unsigned char* active, int vec4) {
+// Bound by the states: 4 B N D read and written per stream. A lane group takes R streams of one channel: A, bias and
+// skip are read once, and each lane makes the steps (a softplus each) of its share of the streams for the others.
+template <typename T, int G, int R>
+__global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const BdhScanDesc d, const float* h, long long h_sb, float* out,
+                                                                           long long out_sb, const unsigned char* active, int vec) {
+  constexpr int OWN = (R + G - 1) / G;                 // streams whose steps this lane makes
   const int lane = threadIdx.x & 31, ng = lane % G, n0 = 4 * ng;
   const long long i = (static_cast<long long>(blockIdx.x) * STEP_THREADS + threadIdx.x) / G;
-  const int b = static_cast<int>(i / d.D), c = static_cast<int>(i % d.D);
-  const bool live = b < d.B, on = live && (active == nullptr || active[b] != 0);
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, y = 0.f, u = 0.f;
+  const int c = static_cast<int>(i % d.D);
+  const long long b0 = i / d.D * R;
+  const bool live = b0 < d.B;
   const long long at = static_cast<long long>(c) * d.N + n0;
-  if (live) {
-    const float* hp = h + b * h_sb + at;
-    if (vec4 && n0 < d.N) {
-      const float4 t = *reinterpret_cast<const float4*>(hp);
-      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  float v[R][4], a[4], y[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float* p = h + (b0 + r) * h_sb + at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[r][j] = 0.f;
+    if (!live || b0 + r >= d.B) continue;
+    if (vec) {
+      if (n0 < d.N) *reinterpret_cast<float4*>(v[r]) = *reinterpret_cast<const float4*>(p);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = n0 + j < d.N ? hp[j] : 0.f;
+      for (int j = 0; j < 4; ++j)
+        if (n0 + j < d.N) v[r][j] = p[j];
     }
-    if (on) {
-      u = elem_to_float<T>(static_cast<const T*>(d.u)[b * d.u_sb + c]);
-      const float raw = elem_to_float<T>(static_cast<const T*>(d.dt)[b * d.dt_sb + c]) + (d.dt_bias ? d.dt_bias[c] : 0.f);
-      float dt = raw, same;
-      if (d.softplus) unpack2(softplus2(both(raw)), dt, same);
-      const float du = dt * u;
-      const T* bp = static_cast<const T*>(d.B_) + b * d.b_sb + n0;
-      const T* cp = static_cast<const T*>(d.C_) + b * d.c_sb + n0;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a[j] = live && n0 + j < d.N ? d.A[at + j] * LOG2E : 0.f;
+  const float bias = live && d.dt_bias ? d.dt_bias[c] : 0.f, skip = live && d.skip ? d.skip[c] : 0.f;
+  float step[OWN], input[OWN];
+#pragma unroll
+  for (int k = 0; k < OWN; ++k) {
+    const long long b = b0 + k * G + ng;
+    const bool on = live && k * G + ng < R && b < d.B && (active == nullptr || active[b] != 0);
+    input[k] = on ? elem_to_float<T>(static_cast<const T*>(d.u)[b * d.u_sb + c]) : 0.f;
+    step[k] = on ? elem_to_float<T>(static_cast<const T*>(d.dt)[b * d.dt_sb + c]) + bias : 0.f;
+    float same;
+    if (d.softplus) unpack2(softplus2(both(step[k])), step[k], same);
+    if (!on) step[k] = 0.f;
+  }
+  const int first = lane - ng;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long b = b0 + r;
+    const float dt = __shfl_sync(0xffffffffu, step[r / G], first + r % G), u = __shfl_sync(0xffffffffu, input[r / G], first + r % G);
+    const bool on = live && b < d.B && (active == nullptr || active[b] != 0);
+    float sum = 0.f;
+    if (on && n0 < d.N) {
+      const T* pb = static_cast<const T*>(d.B_) + b * d.b_sb + n0;
+      const T* pc = static_cast<const T*>(d.C_) + b * d.c_sb + n0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n0 + j < d.N) {
-          v[j] = fmaf(ex2(dt * (d.A[at + j] * LOG2E)), v[j], du * elem_to_float<T>(bp[j]));
-          y = fmaf(elem_to_float<T>(cp[j]), v[j], y);
+          v[r][j] = fmaf(ex2(dt * a[j]), v[r][j], dt * u * elem_to_float<T>(pb[j]));
+          sum = fmaf(elem_to_float<T>(pc[j]), v[r][j], sum);
         }
     }
-  }
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (!live) return;
-  float* op = out + b * out_sb + at;
-  if (on || op != h + b * h_sb + at) {
-    if (vec4 && n0 < d.N) {
-      *reinterpret_cast<float4*>(op) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
+    for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    y[r] = on ? fmaf(skip, u, sum) : 0.f;
+    if (!live || b >= d.B) continue;
+    float* p = out + b * out_sb + at;
+    if (on || p != h + b * h_sb + at) {
+      if (vec) {
+        if (n0 < d.N) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v[r]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + j < d.N) op[j] = v[j];
+        for (int j = 0; j < 4; ++j)
+          if (n0 + j < d.N) p[j] = v[r][j];
+      }
     }
+    if (ng == r % G) static_cast<T*>(d.y)[b * d.D + c] = elem_from_float<T>(y[r]);
   }
-  if (ng == 0)
-    static_cast<T*>(d.y)[static_cast<long long>(b) * d.D + c] = elem_from_float<T>(on ? fmaf(d.skip ? d.skip[c] : 0.f, u, y) : 0.f);
 }
 
 // ---- host --------------------------------------------------------------------------------------------
@@ -979,16 +1017,16 @@ constexpr int MOST_SEGS = 64;          // so that combining the segments stays c
 // (which cost the exponentials a second time), by a model of the time of a tile: what a warp alone on its scheduler
 // takes and what a busy scheduler (592 of them) takes for one, joined as the root of the sum of squares; and what the
 // segments before each segment cost it, which grows with their number squared.
-// Measured for 16 states (clocks): one channel 1890 and 1355, two 2640 and 1885; a sweep is 0.76 of a pass.
+// Measured for 16 states (clocks): one channel 1600 and 1230, two 2350 and 1650; a sweep is 0.8 of a pass.
 Plan fwd_plan(const BdhScanDesc& d) {
   Plan best = plan(d, 2, 1, 1);
   double least = 0;
   for (int CT = 1; CT <= 2; ++CT)
     for (int segs = 1; segs <= MOST_SEGS; segs += segs < 8 ? 1 : 4) {
       const Plan p = plan(d, CT, 1, segs);
-      const double alone = CT == 2 ? 2640 : 1890, busy = (CT == 2 ? 1885 : 1355) * (static_cast<double>(d.B) * p.segs * p.parts / 592);
+      const double alone = CT == 2 ? 2350 : 1600, busy = (CT == 2 ? 1650 : 1230) * (static_cast<double>(d.B) * p.segs * p.parts / 592);
       const double carry = 5000 + 150.0 * p.segs + 55.0 * p.segs * p.segs * d.B * p.parts / 592;
-      const double t = p.per_seg * sqrt(alone * alone + busy * busy) * (p.segs > 1 ? 1.76 : 1) + (p.segs > 1 ? carry : 0);
+      const double t = p.per_seg * sqrt(alone * alone + busy * busy) * (p.segs > 1 ? 1.8 : 1) + (p.segs > 1 ? carry : 0);
       if (least == 0 || t < least) {
         least = t;
         best = p;
@@ -1101,7 +1139,7 @@ int bwd_launch(const BdhScanDesc& d, const Plan& p, const ScanGrads& o, float* s
   const long long grid = static_cast<long long>(d.B) * p.segs * p.parts;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
   auto kernel = selective_scan_bwd_kernel<T, G, CT, VEC>;
-  constexpr int smem = sizeof(BwdMem<G, CT>);
+  constexpr int smem = sizeof(BwdMem<T, G, CT>);
   static PerDeviceOnce once;
   if (const int rc = allow_smem(once, kernel, smem)) return rc;
   kernel<<<static_cast<unsigned>(grid), 32 * BWD_WARPS, smem, s>>>(a, o);
@@ -1167,10 +1205,15 @@ int selective_scan_step_of(const BdhScanDesc& d, const float* h, long long h_sb,
   const int vec4 = d.N % 4 == 0 && h_sb % 4 == 0 && out_sb % 4 == 0 && multiple(h, 16) && multiple(out, 16);
   return by_lanes(lanes_for(d.N), [&](auto g) {
     constexpr int G = decltype(g)::value;
-    const long long blocks = (static_cast<long long>(d.B) * d.D * G + STEP_THREADS - 1) / STEP_THREADS;
-    if (blocks > 0x7fffffffLL) return static_cast<int>(BDH_ERR_TOO_LARGE);
-    selective_scan_step_kernel<T, G><<<static_cast<unsigned>(blocks), STEP_THREADS, 0, s>>>(d, h, h_sb, out, out_sb, active, vec4);
-    return launched();
+    const auto launch = [&](auto kernel, int R) {
+      const long long blocks = (static_cast<long long>((d.B + R - 1) / R) * d.D * G + STEP_THREADS - 1) / STEP_THREADS;
+      if (blocks > 0x7fffffffLL) return static_cast<int>(BDH_ERR_TOO_LARGE);
+      kernel<<<static_cast<unsigned>(blocks), STEP_THREADS, 0, s>>>(d, h, h_sb, out, out_sb, active, vec4);
+      return launched();
+    };
+    // four streams a lane group while that still gives every SM a few blocks
+    if (static_cast<long long>(d.B) * d.D * G >= 4LL * 148 * 4 * STEP_THREADS) return launch(selective_scan_step_kernel<T, G, 4>, 4);
+    return launch(selective_scan_step_kernel<T, G, 1>, 1);
   });
 }
 

@@ -115,8 +115,8 @@ class _CausalConv(torch.autograd.Function):
 
 def _causal_conv_fwd(x, w, bias, state, lengths, silu):
     B, T, C = x.shape
-    y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
-    tail = torch.empty(B, w.shape[1] - 1, C, device=x.device, dtype=x.dtype)
+    y = x.new_empty((B, T, C))
+    tail = x.new_empty((B, w.shape[1] - 1, C))
     native.ops.causal_conv_fwd(x, w, bias, state, lengths, silu, y, tail)
     return y, tail
 
@@ -176,8 +176,8 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias
         return y, (new if out is None else out.copy_(new))
     if not (out is None or C == 1 or out.stride(-1) == 1):
         raise ValueError("out: its channels must be adjacent")
-    y = torch.empty(B, C, device=x.device, dtype=x.dtype)
-    new = torch.empty(B, k - 1, C, device=x.device, dtype=x.dtype) if out is None else out
+    y = x.new_empty((B, C))
+    new = x.new_empty((B, k - 1, C)) if out is None else out
     native.ops.causal_conv_step(A.adjacent(x), A.adjacent(state), A.dense_f32(w), A.dense_f32(bias), active, silu, y, new)
     return y, new
 

@@ -53,8 +53,8 @@ def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, 
 
 
 def _forward(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps):
-    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    ko = torch.empty(k.shape, device=q.device, dtype=q.dtype) if k is not None else None
+    qo = q.new_empty(q.shape)
+    ko = k.new_empty(k.shape) if k is not None else None
     native.ops.norm_rotate_fwd(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps, qo, ko)
     return qo, ko
 

@@ -48,11 +48,10 @@ def _forward(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, train):
     B, T, Dn = u.shape
     N = A.shape[1]
     n_marks, n_scratch, _ = native.ops.selective_scan_sizes(B, T, Dn, N)
-    f32 = dict(device=u.device, dtype=torch.float32)
-    y = torch.empty(B, T, Dn, device=u.device, dtype=u.dtype)
-    hT = torch.empty(B, Dn, N, **f32)
-    marks = torch.empty(n_marks, **f32) if train else None
-    scratch = torch.empty(n_scratch, **f32) if n_scratch else None
+    y = u.new_empty((B, T, Dn))
+    hT = A.new_empty((B, Dn, N))
+    marks = A.new_empty((n_marks,)) if train else None
+    scratch = A.new_empty((n_scratch,)) if n_scratch else None
     native.ops.selective_scan_fwd(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, y, hT, marks, scratch)
     return y, hT, marks
 
@@ -157,8 +156,8 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
     if not (out is None or dense(out)):
         raise ValueError("out: each stream's [D, N] must be dense")
     h = h if dense(h) else h.contiguous()
-    y = torch.empty(B, Dn, device=u.device, dtype=u.dtype)
-    new = torch.empty(B, Dn, N, device=u.device, dtype=torch.float32) if out is None else out
+    y = u.new_empty((B, Dn))
+    new = h.new_empty((B, Dn, N)) if out is None else out
     native.ops.selective_scan_step(A_.adjacent(u), A_.adjacent(dt), A_.dense_f32(A), A_.adjacent(Bm), A_.adjacent(Cm), h, A_.dense_f32(D),
                                    A_.dense_f32(dt_bias), bool(dt_softplus), active, y, new)
     return y, new

@@ -23,7 +23,7 @@ def check_like(t: Optional[torch.Tensor], ref: torch.Tensor, shape: tuple, name:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != ref.device:
         raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
-    if t.dtype != dtype if dtype is not None else not t.is_floating_point():
+    if (t.dtype is not dtype) if dtype is not None else not t.is_floating_point():
         raise ValueError(f"{name}: expected {dtype if dtype is not None else 'a floating type'}, got {t.dtype}")
 
 
@@ -62,11 +62,17 @@ def adjacent(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def dense_f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """A parameter as the kernels read it."""
-    return None if t is None else t.float().contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.float().contiguous()
 
 
 def wants_grad(*ts: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None:
@@ -78,8 +84,11 @@ def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None
     if not (not (torch.is_grad_enabled() and out.requires_grad)):
         raise ValueError(f"{name} requires a gradient; a step form has none")
     same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
-    if not (all(st > 0 or n <= 1 for st, n in zip(out.stride(), out.shape))):
-        raise ValueError(f"{name}: its rows overlap one another")
+    reach = 1                                            # elements that the dimensions of smaller stride span
+    for st, n in sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1):
+        if st < reach:
+            raise ValueError(f"{name}: its rows overlap one another")
+        reach = st * (n - 1) + reach
     if not same and out.numel():
         span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
         (a0, a1), (b0, b1) = span(out), span(src)

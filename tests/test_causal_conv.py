@@ -69,6 +69,9 @@ SHAPES = [
     (2, 67, 48, 8, True, True, True, False),
     (1, 40, 8, 1, True, False, False, False),
     (4, 1, 264, 5, True, True, True, False),
+    (3, 300, 64, 4, True, True, True, True),              # tiles with nothing to test inside, and ragged ends
+    (2, 260, 130, 3, True, False, False, False),
+    (1, 250, 36, 2, True, True, False, False),
 ]
 
 
@@ -194,7 +197,8 @@ def test_refusals(device):
             MO.causal_conv(args.pop("x"), args.pop("w"), args.pop("bias", None), **args)
     st = torch.zeros(2, 3, 8, device=device)
     for change, message in [(dict(state=st[:1]), "state"), (dict(active=torch.ones(2, device=device)), "active"),
-                            (dict(out=st.half()), "out"), (dict(out=st[:, :1].expand(2, 3, 8)), "out")]:
+                            (dict(out=st.half()), "out"), (dict(out=st[:, :1].expand(2, 3, 8)), "out"),
+                            (dict(out=torch.zeros(64, device=device).as_strided((2, 3, 8), (12, 4, 1))), "overlap")]:
         args = {**dict(state=st), **change}
         with pytest.raises(ValueError, match=message):
             MO.causal_conv_step(x[:, 0], args.pop("state"), w, **args)

@@ -123,6 +123,7 @@ CASES = [
     (1, 47, 48, 64, True, True, True, True, False),
     (4, 18, 136, 33, True, True, False, True, False),
     (6, 20, 4000, 16, False, False, True, True, False),     # enough channels for two a lane
+    (9, 50, 1200, 16, True, False, True, True, True),       # many warps, the sequence whole
 ]
 
 
@@ -131,7 +132,7 @@ CASES = [
 @pytest.mark.parametrize("case", CASES)
 def test_outputs_and_gradients(device, dtype, case):
     B, T, D, N, ragged, carry, softplus, extras, view = case
-    if device == "cpu" and D > 1000 and dtype != torch.float32:
+    if device == "cpu" and D >= 1000 and dtype != torch.float32:
         pytest.skip("once is enough for the torch statement at this size")
     p, n, dy, dhT = make(device, dtype, *case)
     leaves = {k: t.detach().requires_grad_() if t is not None else None for k, t in p.items()}
@@ -226,6 +227,27 @@ def test_segments_and_single_tokens_continue_a_prompt(device, N):
     assert torch.equal(yt[active], ref[active]) and (yt[~active] == 0).all()
     assert torch.equal(new[active], moved[active]) and torch.equal(new[~active], st[~active])
     assert torch.equal(pool[:3, 1], new) and (pool[:, 0] == 0).all() and (pool[3] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,B,D,N", [(torch.bfloat16, 79, 1030, 16), (torch.float32, 82, 2048, 5), (torch.float16, 21, 1000, 61)])
+def test_single_tokens_of_many_streams(dtype, B, D, N):
+    """Enough streams that a lane group takes four of them; one row of the recurrence, with and without its extras."""
+    for extras in (True, False):
+        p, _, _, _ = make("cuda", dtype, B, 1, D, N, False, True, True, extras, True)
+        want = definition({k: t.double() if t is not None else None for k, t in p.items()}, None, True, torch.zeros(B, 1, D, device="cuda").double(),
+                          None)
+        active = torch.rand(B, device="cuda") < 0.7
+        with torch.no_grad():
+            row = [p["u"][:, 0], p["dt"][:, 0], p["A"], p["B"][:, 0], p["C"][:, 0]]
+            y, h = S.selective_scan_step(*row, p["h0"], p["D"], dt_bias=p["dt_bias"], dt_softplus=True)
+            some, kept = S.selective_scan_step(*row, p["h0"], p["D"], dt_bias=p["dt_bias"], dt_softplus=True, active=active)
+            inplace = p["h0"].clone()
+            S.selective_scan_step(*row, inplace, p["D"], dt_bias=p["dt_bias"], dt_softplus=True, active=active, out=inplace)
+        within(y[:, None], *want["y"], "y")
+        within(h, *want["h"], "h")
+        assert torch.equal(some[active], y[active]) and (some[~active] == 0).all()
+        assert torch.equal(kept[active], h[active]) and torch.equal(kept[~active], p["h0"][~active]) and torch.equal(inplace, kept)
 
 
 @pytest.mark.parametrize("device", DEVICES)
