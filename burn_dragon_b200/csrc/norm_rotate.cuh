@@ -22,6 +22,10 @@ namespace bdh {
 namespace {
 
 constexpr int NT = 128;
+// Blocks an SM: as many as run at once, in one round over the tokens. Registers for five and three (forward 87 us, backward
+// 156 us at 4 x 4096 tokens, 32 + 8 heads of 128, bf16; for four and two 90 and 191 us, for six and four, which spill, 125 and
+// 203 us; two rounds of blocks 89 and 171 us). Rows of several packs a lane need more.
+constexpr int FWD_BLOCKS = 5, BWD_BLOCKS = 3;
 
 struct NormArgs {
   BdhNormRotateDesc d;
@@ -206,7 +210,7 @@ __device__ __forceinline__ f2 turn(f2 v, float2 e) {
 }
 
 template <typename T, int V, bool VEC, int NV, int U>
-__global__ void __launch_bounds__(NT) norm_rotate_fwd_kernel(const NormArgs a, int w_rows) {
+__global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_kernel(const NormArgs a, int w_rows) {
   using P = Place<T, V, VEC, NV>;
   using Raw = typename P::Raw;
   constexpr int N = P::N;
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(NT) norm_rotate_fwd_kernel(const NormArgs a, i
 // weights. PER_HEAD: a sum for each of the thread's heads; else one for q and one for k. partial: [2 (weight, bias)]
 // [lines][width], see norm_rotate_params_kernel.
 template <typename T, int V, bool VEC, int NV, int U, bool PER_HEAD, bool BIAS>
-__global__ void __launch_bounds__(NT) norm_rotate_bwd_kernel(const NormArgs a, int w_rows, float* partial, float* dang) {
+__global__ void __launch_bounds__(NT, NV == 1 ? BWD_BLOCKS : 2) norm_rotate_bwd_kernel(const NormArgs a, int w_rows, float* partial, float* dang) {
   using P = Place<T, V, VEC, NV>;
   using Raw = typename P::Raw;
   constexpr int N = P::N, SUMS = PER_HEAD ? U : 2;
@@ -568,7 +572,7 @@ int fwd_launch(const BdhNormRotateDesc& d, cudaStream_t s) {
   const size_t smem = sizeof(float) * 2 * w_rows * a.G * V * NV + sizeof(float2) * 2 * a.TS * d.P;
   auto kernel = norm_rotate_fwd_kernel<T, V, VEC, NV, U>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
-  kernel<<<dim3(token_blocks(a, 8), a.slices), NT, smem, s>>>(a, w_rows);
+  kernel<<<dim3(token_blocks(a, FWD_BLOCKS), a.slices), NT, smem, s>>>(a, w_rows);
   return launched();
 }
 
@@ -591,7 +595,7 @@ struct BwdPlan {
 
 BwdPlan bwd_plan(const NormArgs& a, int v_nv, bool want_w, bool want_b, bool want_ang) {
   BwdPlan p;
-  p.blocks = token_blocks(a, 4);
+  p.blocks = token_blocks(a, BWD_BLOCKS);
   p.width = a.d.per_head ? (a.d.Hq + a.d.Hk) * a.d.Dh : 2 * a.d.Dh;
   p.lines = static_cast<long long>(p.blocks) * (a.d.per_head ? 1 : a.slices);
   p.partial = (want_w || want_b) ? (want_b ? 2 : 1) * p.lines * p.width : 0;
