@@ -307,7 +307,7 @@ int bdh_causal_conv_bwd(const BdhConvDesc* d, float* dw, float* db, float* parti
 // byte is 0 gives y = 0 and keeps its state.
 int bdh_causal_conv_step(const BdhConvDesc* d, const unsigned char* active, cudaStream_t s);
 
-// RMS norm of every head of q and k, then the rotation of its channel pairs (2i, 2i + 1), i < P (norm_rotate.cu):
+// RMS norm of every head of q and k, then the rotation of its channel pairs (2i, 2i + 1), i < P (norm_rotate.cuh):
 // v = x / sqrt(mean x^2 + eps) * w + b; (o0, o1) = (v0 cos - v1 sin, v1 cos + v0 sin). q, k: strides in elements of the
 // batch, a token and a head; q_out, k_out and the backward tensors: contiguous [B, T, heads, Dh]. Weights and biases
 // fp32 [Dh], or [heads, Dh] with per_head (null: ones, zeros). Angles: `angles` (radians, P adjacent), or
@@ -345,7 +345,7 @@ long long bdh_norm_rotate_scratch(const BdhNormRotateDesc* d, int want_weight, i
 int bdh_norm_rotate_bwd(const BdhNormRotateDesc* d, float* dq_weight, float* dk_weight, float* dq_bias, float* dk_bias,
                         float* dangles, float* scratch, cudaStream_t s);
 
-// Selective scan (selective_scan.cu): dt' = softplus(dt + dt_bias) or dt + dt_bias; h_t = exp(dt'_t A) h_{t-1} + dt'_t u_t B_t;
+// Selective scan (selective_scan.cuh): dt' = softplus(dt + dt_bias) or dt + dt_bias; h_t = exp(dt'_t A) h_{t-1} + dt'_t u_t B_t;
 // y_t = C_t . h_t + skip u_t, for channels d < D with N <= 64 states each. u, dt, dy [B, T, D] and B, C [B, T, N]: strides
 // in elements of the batch and of a row; A [D, N], dt_bias, skip [D], h0, hT, dhT, dh0 [B, D, N] fp32 contiguous; y, du,
 // ddt contiguous. lengths as above: behind a length the state stays, y and all gradients are 0.

@@ -8,7 +8,11 @@
 // walks down a tile of the time axis with the k - 1 rows behind it in registers, so that each element of x is read
 // once and k - 1 rows per tile twice (the second time from L2). fp32 throughout; the parameter gradients are summed
 // in registers over every tile that a block walks, then over the block, then over the blocks in a fixed order (no
-// atomics: two runs give the same bits).
+// atomics: two runs give the same bits). Channels go in pairs (one instruction for two), rows in sets that change
+// places instead of moving, and the next set is on its way while one is worked on.
+//
+// Measured, 8 x 2048 x 4096 bf16: forward 57 us (0.73 of the copy rate), backward 110 us (0.57: about 30 instructions an
+// element pair and row, at three warps a scheduler) and 7 us for the parameters' sums; one token of 64 streams 4.6 us.
 #include "bdh_kernels.h"
 #include "pair_math.cuh"
 

@@ -1,4 +1,4 @@
-"""RMS norm of every query and key head together with its rotation, in one pass (`csrc/norm_rotate.cu`).
+"""RMS norm of every query and key head together with its rotation, in one pass (`csrc/norm_rotate.cuh`).
 
     v = x / sqrt(mean x^2 + eps) * weight + bias          over the Dh channels of a head
     (o_2i, o_2i+1) = (v_2i cos - v_2i+1 sin, v_2i+1 cos + v_2i sin)     for the first pairs; the other channels stay

@@ -1,4 +1,4 @@
-"""Selective scan: a diagonal recurrence whose step is an input of its own for every channel (`csrc/selective_scan.cu`).
+"""Selective scan: a diagonal recurrence whose step is an input of its own for every channel (`csrc/selective_scan.cuh`).
 
     dt'_t = softplus(dt_t + dt_bias)                       (dt_softplus; else dt_t + dt_bias)
     h_t = exp(dt'_t A) h_{t-1} + (dt'_t u_t) (x) B_t        h: [D, N] per sequence
