@@ -1,10 +1,13 @@
 // torch.ops.bdh.* of the parts of a state-space layer (causal convolution, per-head norm + rotation, selective
-// scan). As in bindings.cpp the caller allocates every output and all scratch; shapes that the kernels rely on are
-// checked here once more, so that a direct call cannot make them read or write out of range.
+// scan). Shapes that the kernels rely on are checked here once more, so that a direct call cannot make them read or
+// write out of range. Unlike in bindings.cpp, results and scratch are allocated here, from torch's allocator on the
+// current stream: a call of one token is as long as its way through Python, and every tensor made there adds to it.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
+
+#include <vector>
 
 #include "bdh_kernels.h"
 
@@ -46,7 +49,6 @@ void check_f32(const OptTensor& t, const Tensor& on, at::IntArrayRef sizes, cons
 }
 
 const float* f32_ptr(const OptTensor& t) { return given(t) ? t->const_data_ptr<float>() : nullptr; }
-float* f32_out(const OptTensor& t) { return given(t) ? t->data_ptr<float>() : nullptr; }
 
 void set_lengths(const OptTensor& t, const Tensor& on, int64_t B, const void*& ptr, int& is64) {
   ptr = nullptr;
@@ -64,6 +66,9 @@ const unsigned char* active_ptr(const OptTensor& t, const Tensor& on, int64_t B)
   check_dense(*t, on, at::kBool, {B}, "active");
   return reinterpret_cast<const unsigned char*>(t->const_data_ptr());
 }
+
+Tensor new_f32(const Tensor& on, at::IntArrayRef sizes) { return at::empty(sizes, on.options().dtype(at::kFloat)); }
+Tensor new_rows(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options()); }
 
 int to_int(int64_t v, const char* name) {
   TORCH_CHECK(v >= 0 && v <= 0x7fffffff - 4096, name, ": too large");
@@ -98,61 +103,57 @@ void set_state_out(BdhConvDesc& d, const Tensor& x, const Tensor& out) {
   d.state_out = out.data_ptr(); d.state_out_sb = out.stride(0); d.state_out_sr = out.stride(1);
 }
 
-void causal_conv_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
-                     bool silu, Tensor& y, Tensor& state_out) {
+std::vector<Tensor> causal_conv_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state,
+                                    const OptTensor& lengths, bool silu) {
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.dim() == 3 && w.dim() == 2, "x: [B, T, C], w: [C, k]");
   BdhConvDesc d = conv_desc(x, w, bias, state, lengths, silu);
-  check_dense(y, x, x.scalar_type(), x.sizes(), "y");
+  Tensor y = new_rows(x, x.sizes()), end = new_rows(x, {d.B, d.k - 1, d.C});
   d.y = y.data_ptr();
-  set_state_out(d, x, state_out);
+  set_state_out(d, x, end);
   check_rc(bdh_causal_conv_fwd(&d, cur_stream()), "causal_conv_fwd");
+  return {y, end};
 }
 
-int64_t causal_conv_partials(int64_t B, int64_t T, int64_t C, int64_t k) {
-  BdhConvDesc d{};
-  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.C = to_int(C, "C"); d.k = to_int(k, "k");
-  return bdh_causal_conv_partials(&d);
-}
-
-void causal_conv_bwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
-                     bool silu, const Tensor& dy, const OptTensor& dstate_out, Tensor& dx, const OptTensor& dstate,
-                     const OptTensor& dw, const OptTensor& db, const OptTensor& partial) {
+// dx, then those of dw, db, dstate that are wanted
+std::vector<Tensor> causal_conv_bwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
+                                    bool silu, const OptTensor& dy, const OptTensor& dstate_out, bool want_w, bool want_bias,
+                                    bool want_state) {
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.dim() == 3 && w.dim() == 2, "x: [B, T, C], w: [C, k]");
   BdhConvDesc d = conv_desc(x, w, bias, state, lengths, silu);
-  const int64_t B = x.size(0), C = x.size(2);
-  check_rows(dy, x, x.scalar_type(), x.sizes(), "dy");
-  d.dy = dy.const_data_ptr(); d.dy_sb = dy.stride(0); d.dy_st = dy.stride(1);
-  check_dense(dx, x, x.scalar_type(), x.sizes(), "dx");
-  d.dx = dx.data_ptr();
+  TORCH_CHECK(d.B > 0 && d.T > 0, "no rows");
+  TORCH_CHECK(!want_state || given(state), "state: needed for its gradient");
+  const Tensor g = given(dy) ? *dy : at::zeros(x.sizes(), x.options());
+  check_rows(g, x, x.scalar_type(), x.sizes(), "dy");
+  d.dy = g.const_data_ptr(); d.dy_sb = g.stride(0); d.dy_st = g.stride(1);
   if (given(dstate_out)) {
-    check_dense(*dstate_out, x, x.scalar_type(), {B, d.k - 1, C}, "dstate_out");
+    check_dense(*dstate_out, x, x.scalar_type(), {d.B, d.k - 1, d.C}, "dstate_out");
     d.dstate_out = dstate_out->const_data_ptr();
   }
-  if (given(dstate)) {
-    check_dense(*dstate, x, x.scalar_type(), {B, d.k - 1, C}, "dstate");
-    d.dstate = dstate->data_ptr();
-  }
-  check_f32(dw, x, {C, d.k}, "dw");
-  check_f32(db, x, {C}, "db");
-  if (given(dw) || given(db)) {
-    TORCH_CHECK(given(partial), "partial: needed for dw and db");
-    check_f32(partial, x, {partial->size(0)}, "partial");
-    TORCH_CHECK(partial->size(0) >= bdh_causal_conv_partials(&d), "partial: too small");
-  }
-  check_rc(bdh_causal_conv_bwd(&d, f32_out(dw), f32_out(db), f32_out(partial), cur_stream()), "causal_conv_bwd");
+  std::vector<Tensor> out{new_rows(x, x.sizes())};
+  d.dx = out[0].data_ptr();
+  float *dw = nullptr, *db = nullptr;
+  if (want_w) dw = out.emplace_back(new_f32(x, w.sizes())).data_ptr<float>();
+  if (want_bias) db = out.emplace_back(new_f32(x, {d.C})).data_ptr<float>();
+  if (want_state) d.dstate = out.emplace_back(new_rows(x, {d.B, d.k - 1, d.C})).data_ptr();
+  Tensor partial;
+  if (want_w || want_bias) partial = new_f32(x, {bdh_causal_conv_partials(&d)});
+  check_rc(bdh_causal_conv_bwd(&d, dw, db, partial.defined() ? partial.data_ptr<float>() : nullptr, cur_stream()), "causal_conv_bwd");
+  return out;
 }
 
-void causal_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, const OptTensor& bias, const OptTensor& active, bool silu,
-                      Tensor& y, Tensor& state_out) {
+// y, and the new state unless it goes to `out`
+std::vector<Tensor> causal_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, const OptTensor& bias, const OptTensor& active,
+                                     bool silu, const OptTensor& out) {
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [B, C], w: [C, k]");
   BdhConvDesc d = conv_desc(x, w, bias, state, c10::nullopt, silu);
-  check_dense(y, x, x.scalar_type(), x.sizes(), "y");
-  d.y = y.data_ptr();
-  set_state_out(d, x, state_out);
+  std::vector<Tensor> result{new_rows(x, x.sizes())};
+  d.y = result[0].data_ptr();
+  set_state_out(d, x, given(out) ? *out : result.emplace_back(new_rows(x, state.sizes())));
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
+  return result;
 }
 
 // ---- per-head norm + rotation ------------------------------------------------------------------------
@@ -209,62 +210,53 @@ BdhNormRotateDesc norm_desc(const Tensor& q, const OptTensor& k, const OptTensor
   return d;
 }
 
-void norm_rotate_fwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& q_bias,
-                     const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs, const OptTensor& positions,
-                     int64_t pos0, const OptTensor& lengths, double eps, Tensor& q_out, const OptTensor& k_out) {
+std::vector<Tensor> norm_rotate_fwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                                    const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
+                                    const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
   c10::cuda::CUDAGuard guard(q.device());
   BdhNormRotateDesc d = norm_desc(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
-  check_dense(q_out, q, q.scalar_type(), q.sizes(), "q_out");
-  d.q_out = q_out.data_ptr();
-  if (given(k)) {
-    TORCH_CHECK(given(k_out), "k_out: needed");
-    check_dense(*k_out, q, q.scalar_type(), k->sizes(), "k_out");
-    d.k_out = k_out->data_ptr();
-  }
+  std::vector<Tensor> out{new_rows(q, q.sizes())};
+  d.q_out = out[0].data_ptr();
+  if (given(k)) d.k_out = out.emplace_back(new_rows(q, k->sizes())).data_ptr();
   check_rc(bdh_norm_rotate_fwd(&d, cur_stream()), "norm_rotate_fwd");
+  return out;
 }
 
-int64_t norm_rotate_scratch(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t Dh, int64_t P, bool per_head, bool want_weight,
-                            bool want_bias, bool want_angles) {
-  BdhNormRotateDesc d{};
-  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.Hq = to_int(Hq, "heads"); d.Hk = to_int(Hk, "heads"); d.Dh = to_int(Dh, "Dh");
-  d.P = to_int(P, "pairs"); d.per_head = per_head;
-  return bdh_norm_rotate_scratch(&d, want_weight, want_bias, want_angles);
-}
-
-void norm_rotate_bwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& q_bias,
-                     const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs, const OptTensor& positions,
-                     int64_t pos0, const OptTensor& lengths, double eps, const Tensor& dq_out, const OptTensor& dk_out, Tensor& dq,
-                     const OptTensor& dk, const OptTensor& dq_weight, const OptTensor& dk_weight, const OptTensor& dq_bias,
-                     const OptTensor& dk_bias, const OptTensor& dangles, const OptTensor& scratch) {
+// dq, dk (with k), then those of q_weight, k_weight, q_bias, k_bias and angles that `want` has a bit for
+std::vector<Tensor> norm_rotate_bwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                                    const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
+                                    const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps,
+                                    const OptTensor& dq_out, const OptTensor& dk_out, int64_t want) {
   c10::cuda::CUDAGuard guard(q.device());
   BdhNormRotateDesc d = norm_desc(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+  TORCH_CHECK(d.B > 0 && d.T > 0, "no rows");
   const auto type = q.scalar_type();
-  check_dense(dq_out, q, type, q.sizes(), "dq_out");
-  check_dense(dq, q, type, q.sizes(), "dq");
-  d.dq_out = dq_out.const_data_ptr(); d.dq = dq.data_ptr();
+  std::vector<Tensor> out{new_rows(q, q.sizes())};
+  d.dq = out[0].data_ptr();
+  const Tensor gq = given(dq_out) ? *dq_out : at::zeros(q.sizes(), q.options());
+  check_dense(gq, q, type, q.sizes(), "dq_out");
+  d.dq_out = gq.const_data_ptr();
+  Tensor gk;
   if (given(k)) {
-    TORCH_CHECK(given(dk_out) && given(dk), "dk_out, dk: needed");
-    check_dense(*dk_out, q, type, k->sizes(), "dk_out");
-    check_dense(*dk, q, type, k->sizes(), "dk");
-    d.dk_out = dk_out->const_data_ptr(); d.dk = dk->data_ptr();
+    gk = given(dk_out) ? *dk_out : at::zeros(k->sizes(), q.options());
+    check_dense(gk, q, type, k->sizes(), "dk_out");
+    d.dk_out = gk.const_data_ptr();
+    d.dk = out.emplace_back(new_rows(q, k->sizes())).data_ptr();
   }
-  const auto check_grad = [&](const OptTensor& t, int64_t heads, const char* name) {
-    if (d.per_head) check_f32(t, q, {heads, d.Dh}, name);
-    else check_f32(t, q, {d.Dh}, name);
-    return f32_out(t);
-  };
-  float* gqw = check_grad(dq_weight, d.Hq, "dq_weight");
-  float* gkw = check_grad(dk_weight, d.Hk, "dk_weight");
-  float* gqb = check_grad(dq_bias, d.Hq, "dq_bias");
-  float* gkb = check_grad(dk_bias, d.Hk, "dk_bias");
-  check_f32(dangles, q, {d.B, d.T, d.P}, "dangles");
-  const long long need = bdh_norm_rotate_scratch(&d, gqw || gkw || gqb || gkb, gqb || gkb, given(dangles));
-  if (need > 0) {
-    TORCH_CHECK(given(scratch) && scratch->numel() >= need, "scratch: too small");
-    check_f32(scratch, q, {scratch->numel()}, "scratch");
-  }
-  check_rc(bdh_norm_rotate_bwd(&d, gqw, gkw, gqb, gkb, f32_out(dangles), f32_out(scratch), cur_stream()), "norm_rotate_bwd");
+  const OptTensor* params[5] = {&q_weight, &k_weight, &q_bias, &k_bias, &angles};
+  float* grads[5] = {};
+  for (int i = 0; i < 5; ++i)
+    if (want >> i & 1) {
+      TORCH_CHECK(given(*params[i]), "a gradient is wanted of something that was not given");
+      grads[i] = out.emplace_back(new_f32(q, (*params[i])->sizes())).data_ptr<float>();
+    }
+  const bool bias = grads[2] || grads[3];
+  const long long need = bdh_norm_rotate_scratch(&d, bias || grads[0] || grads[1], bias, grads[4] != nullptr);
+  Tensor scratch;
+  if (need > 0) scratch = new_f32(q, {need});
+  check_rc(bdh_norm_rotate_bwd(&d, grads[0], grads[1], grads[2], grads[3], grads[4], need > 0 ? scratch.data_ptr<float>() : nullptr,
+                               cur_stream()), "norm_rotate_bwd");
+  return out;
 }
 
 // ---- selective scan ----------------------------------------------------------------------------------
@@ -297,118 +289,97 @@ BdhScanDesc scan_desc(const Tensor& u, const Tensor& dt, const Tensor& A, const 
   return d;
 }
 
-std::tuple<int64_t, int64_t, int64_t> selective_scan_sizes(int64_t B, int64_t T, int64_t D, int64_t N) {
-  BdhScanDesc d{};
-  d.B = to_int(B, "B"); d.T = to_int(T, "T"); d.D = to_int(D, "D"); d.N = to_int(N, "N");
-  long long marks, fwd, bwd;
-  bdh_selective_scan_sizes(&d, &marks, &fwd, &bwd);
-  return {marks, fwd, bwd};
-}
-
-float* scratch_of(const OptTensor& t, const Tensor& on, long long need, const char* name) {
-  if (need <= 0) return nullptr;
-  TORCH_CHECK(given(t) && t->numel() >= need, name, ": too small");
-  check_f32(t, on, {t->numel()}, name);
-  return t->data_ptr<float>();
-}
-
-void selective_scan_fwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
-                        const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths, Tensor& y, Tensor& hT,
-                        const OptTensor& marks, const OptTensor& scratch) {
+// y, hT and, for a backward pass (train), the states at the tiles' starts
+std::vector<Tensor> selective_scan_fwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                                       const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0,
+                                       const OptTensor& lengths, bool train) {
   c10::cuda::CUDAGuard guard(u.device());
   TORCH_CHECK(u.dim() == 3, "u: [B, T, D]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
-  check_dense(y, u, u.scalar_type(), u.sizes(), "y");
-  check_dense(hT, u, at::kFloat, {d.B, d.D, d.N}, "hT");
-  d.y = y.data_ptr(); d.hT = hT.data_ptr<float>();
   long long n_marks, n_fwd, n_bwd;
   bdh_selective_scan_sizes(&d, &n_marks, &n_fwd, &n_bwd);
-  float* m = given(marks) ? scratch_of(marks, u, n_marks, "marks") : nullptr;
-  check_rc(bdh_selective_scan_fwd(&d, m, scratch_of(scratch, u, n_fwd, "scratch"), cur_stream()), "selective_scan_fwd");
+  std::vector<Tensor> out{new_rows(u, u.sizes()), new_f32(u, {d.B, d.D, d.N})};
+  d.y = out[0].data_ptr(); d.hT = out[1].data_ptr<float>();
+  float* marks = train ? out.emplace_back(new_f32(u, {n_marks})).data_ptr<float>() : nullptr;
+  Tensor scratch;
+  if (n_fwd > 0) scratch = new_f32(u, {n_fwd});
+  check_rc(bdh_selective_scan_fwd(&d, marks, n_fwd > 0 ? scratch.data_ptr<float>() : nullptr, cur_stream()), "selective_scan_fwd");
+  return out;
 }
 
-void selective_scan_bwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
-                        const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths, const Tensor& marks,
-                        const Tensor& scratch, const Tensor& dy, const OptTensor& dhT, Tensor& du, Tensor& ddt, Tensor& dA, Tensor& dB,
-                        Tensor& dC, const OptTensor& dskip, const OptTensor& ddt_bias, const OptTensor& dh0) {
+// du, ddt, dA, dB, dC, then dD and ddt_bias where these were given and dh0 where it is wanted
+std::vector<Tensor> selective_scan_bwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                                       const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0,
+                                       const OptTensor& lengths, const Tensor& marks, const OptTensor& dy, const OptTensor& dhT,
+                                       bool want_h0) {
   c10::cuda::CUDAGuard guard(u.device());
   TORCH_CHECK(u.dim() == 3, "u: [B, T, D]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
+  TORCH_CHECK(d.B > 0 && d.T > 0, "no rows");
   const auto type = u.scalar_type();
-  check_rows(dy, u, type, u.sizes(), "dy");
-  check_dense(du, u, type, u.sizes(), "du");
-  check_dense(ddt, u, type, u.sizes(), "ddt");
-  check_dense(dA, u, at::kFloat, A.sizes(), "dA");
-  check_dense(dB, u, type, Bm.sizes(), "dB");
-  check_dense(dC, u, type, Cm.sizes(), "dC");
-  check_f32(dskip, u, {d.D}, "dD");
-  check_f32(ddt_bias, u, {d.D}, "ddt_bias");
+  const Tensor g = given(dy) ? *dy : at::zeros(u.sizes(), u.options());
+  check_rows(g, u, type, u.sizes(), "dy");
   check_f32(dhT, u, {d.B, d.D, d.N}, "dhT");
-  check_f32(dh0, u, {d.B, d.D, d.N}, "dh0");
-  d.dy = dy.const_data_ptr(); d.dy_sb = dy.stride(0); d.dy_st = dy.stride(1);
-  d.du = du.data_ptr(); d.ddt = ddt.data_ptr(); d.dhT = f32_ptr(dhT); d.dh0 = f32_out(dh0);
   long long n_marks, n_fwd, n_bwd;
   bdh_selective_scan_sizes(&d, &n_marks, &n_fwd, &n_bwd);
-  const float* m = scratch_of(marks, u, n_marks, "marks");
-  check_rc(bdh_selective_scan_bwd(&d, m, scratch_of(scratch, u, n_bwd, "scratch"), dA.data_ptr<float>(), f32_out(dskip), f32_out(ddt_bias),
-                                  dB.data_ptr(), dC.data_ptr(), cur_stream()), "selective_scan_bwd");
+  check_dense(marks, u, at::kFloat, {n_marks}, "marks");
+  std::vector<Tensor> out{new_rows(u, u.sizes()), new_rows(u, u.sizes()), new_f32(u, A.sizes()), new_rows(u, Bm.sizes()), new_rows(u, Cm.sizes())};
+  float* dD = given(skip) ? out.emplace_back(new_f32(u, {d.D})).data_ptr<float>() : nullptr;
+  float* dbias = given(dt_bias) ? out.emplace_back(new_f32(u, {d.D})).data_ptr<float>() : nullptr;
+  d.dh0 = want_h0 ? out.emplace_back(new_f32(u, {d.B, d.D, d.N})).data_ptr<float>() : nullptr;
+  d.dy = g.const_data_ptr(); d.dy_sb = g.stride(0); d.dy_st = g.stride(1);
+  d.du = out[0].data_ptr(); d.ddt = out[1].data_ptr(); d.dhT = f32_ptr(dhT);
+  Tensor scratch = new_f32(u, {n_bwd});
+  check_rc(bdh_selective_scan_bwd(&d, marks.const_data_ptr<float>(), scratch.data_ptr<float>(), out[2].data_ptr<float>(), dD, dbias,
+                                  out[3].data_ptr(), out[4].data_ptr(), cur_stream()), "selective_scan_bwd");
+  return out;
 }
 
-void selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const Tensor& h,
-                         const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& active, Tensor& y, Tensor& out) {
+// y, and the new state unless it goes to `out`
+std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const Tensor& h,
+                                        const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& active,
+                                        const OptTensor& out) {
   c10::cuda::CUDAGuard guard(u.device());
   TORCH_CHECK(u.dim() == 2 && dt.dim() == 2 && Bm.dim() == 2 && Cm.dim() == 2, "u, dt: [B, D], B, C: [B, N]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, c10::nullopt, c10::nullopt);
-  check_dense(y, u, u.scalar_type(), u.sizes(), "y");
-  d.y = y.data_ptr();
-  for (const Tensor* t : {&h, static_cast<const Tensor*>(&out)}) {
+  std::vector<Tensor> result{new_rows(u, u.sizes())};
+  d.y = result[0].data_ptr();
+  const Tensor to = given(out) ? *out : result.emplace_back(new_f32(u, {d.B, d.D, d.N}));
+  for (const Tensor* t : {&h, &to}) {
     check_rows(*t, u, at::kFloat, {d.B, d.D, d.N}, "h");
     TORCH_CHECK(d.D == 1 || t->stride(1) == d.N, "h: expected dense [D, N] states");
   }
-  check_rc(bdh_selective_scan_step(&d, h.const_data_ptr<float>(), h.stride(0), out.data_ptr<float>(), out.stride(0),
+  check_rc(bdh_selective_scan_step(&d, h.const_data_ptr<float>(), h.stride(0), to.data_ptr<float>(), to.stride(0),
                                    active_ptr(active, u, d.B), cur_stream()), "selective_scan_step");
+  return result;
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(bdh, m) {
-  m.def("causal_conv_fwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor(a!) y, "
-        "Tensor(b!) state_out) -> ()");
-  m.def("causal_conv_partials(int B, int T, int C, int k) -> int");
-  m.def("causal_conv_bwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor dy, "
-        "Tensor? dstate_out, Tensor(a!) dx, Tensor(b!)? dstate, Tensor(c!)? dw, Tensor(d!)? db, Tensor(e!)? partial) -> ()");
-  m.def("causal_conv_step(Tensor x, Tensor state, Tensor w, Tensor? bias, Tensor? active, bool silu, Tensor(a!) y, "
-        "Tensor(b!) state_out) -> ()");
+  m.def("causal_conv_fwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> Tensor[]");
+  m.def("causal_conv_bwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor? dy, "
+        "Tensor? dstate_out, bool want_w, bool want_bias, bool want_state) -> Tensor[]");
+  m.def("causal_conv_step(Tensor x, Tensor state, Tensor w, Tensor? bias, Tensor? active, bool silu, Tensor(a!)? out) -> Tensor[]");
   m.def("norm_rotate_fwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
-        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor(a!) q_out, Tensor(b!)? k_out) -> ()");
-  m.def("norm_rotate_scratch(int B, int T, int Hq, int Hk, int Dh, int P, bool per_head, bool want_weight, bool want_bias, "
-        "bool want_angles) -> int");
+        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps) -> Tensor[]");
   m.def("norm_rotate_bwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
-        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor dq_out, Tensor? dk_out, Tensor(a!) dq, "
-        "Tensor(b!)? dk, Tensor(c!)? dq_weight, Tensor(d!)? dk_weight, Tensor(e!)? dq_bias, Tensor(f!)? dk_bias, "
-        "Tensor(g!)? dangles, Tensor(h!)? scratch) -> ()");
-  m.def("selective_scan_sizes(int B, int T, int D, int N) -> (int, int, int)");
+        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor? dq_out, Tensor? dk_out, int want) -> Tensor[]");
   m.def("selective_scan_fwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
-        "Tensor? lengths, Tensor(a!) y, Tensor(b!) hT, Tensor(c!)? marks, Tensor(d!)? scratch) -> ()");
+        "Tensor? lengths, bool train) -> Tensor[]");
   m.def("selective_scan_bwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
-        "Tensor? lengths, Tensor marks, Tensor(a!) scratch, Tensor dy, Tensor? dhT, Tensor(b!) du, Tensor(c!) ddt, Tensor(d!) dA, "
-        "Tensor(e!) dB, Tensor(f!) dC, Tensor(g!)? dD, Tensor(h!)? ddt_bias, Tensor(i!)? dh0) -> ()");
+        "Tensor? lengths, Tensor marks, Tensor? dy, Tensor? dhT, bool want_h0) -> Tensor[]");
   m.def("selective_scan_step(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor h, Tensor? D, Tensor? dt_bias, bool softplus, "
-        "Tensor? active, Tensor(a!) y, Tensor(b!) out) -> ()");
+        "Tensor? active, Tensor(a!)? out) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
-  m.impl("selective_scan_fwd", &selective_scan_fwd);
-  m.impl("selective_scan_bwd", &selective_scan_bwd);
-  m.impl("selective_scan_step", &selective_scan_step);
-  m.impl("norm_rotate_fwd", &norm_rotate_fwd);
-  m.impl("norm_rotate_bwd", &norm_rotate_bwd);
   m.impl("causal_conv_fwd", &causal_conv_fwd);
   m.impl("causal_conv_bwd", &causal_conv_bwd);
   m.impl("causal_conv_step", &causal_conv_step);
-}
-TORCH_LIBRARY_IMPL(bdh, CompositeExplicitAutograd, m) {
-  m.impl("causal_conv_partials", &causal_conv_partials);
-  m.impl("norm_rotate_scratch", &norm_rotate_scratch);
-  m.impl("selective_scan_sizes", &selective_scan_sizes);
+  m.impl("norm_rotate_fwd", &norm_rotate_fwd);
+  m.impl("norm_rotate_bwd", &norm_rotate_bwd);
+  m.impl("selective_scan_fwd", &selective_scan_fwd);
+  m.impl("selective_scan_bwd", &selective_scan_bwd);
+  m.impl("selective_scan_step", &selective_scan_step);
 }

@@ -86,7 +86,8 @@ class _CausalConv(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, w, bias, state, lengths)
         ctx.silu = silu
-        return _causal_conv_fwd(x, w, bias, state, lengths, silu)
+        y, tail = native.ops.causal_conv_fwd(x, w, bias, state, lengths, silu)
+        return y, tail
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -94,31 +95,15 @@ class _CausalConv(torch.autograd.Function):
         x, w, bias, state, lengths = ctx.saved_tensors
         if dy is None and dtail is None:
             return (None,) * 6
-        B, T, C = x.shape
-        k = w.shape[1]
-        dy = A.adjacent(dy) if dy is not None else torch.zeros_like(x)
-        dtail = dtail.contiguous() if dtail is not None else None
-        need = ctx.needs_input_grad
-        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
-        dw = torch.empty_like(w) if need[1] else None
-        db = torch.empty_like(bias) if bias is not None and need[2] else None
-        dstate = torch.empty(B, k - 1, C, device=x.device, dtype=x.dtype) if state is not None and need[3] else None
-        if B * T == 0:                                                         # no rows: the state went through unchanged
-            zero = lambda t: t.zero_() if t is not None else None
-            return dx, zero(dw), zero(db), dtail if dstate is not None and dtail is not None else zero(dstate), None, None
-        part = None
-        if dw is not None or db is not None:
-            part = torch.empty(native.ops.causal_conv_partials(B, T, C, k), device=x.device, dtype=torch.float32)
-        native.ops.causal_conv_bwd(x, w, bias, state, lengths, ctx.silu, dy, dtail, dx, dstate, dw, db, part)
-        return dx, dw, db, dstate, None, None
-
-
-def _causal_conv_fwd(x, w, bias, state, lengths, silu):
-    B, T, C = x.shape
-    y = x.new_empty((B, T, C))
-    tail = x.new_empty((B, w.shape[1] - 1, C))
-    native.ops.causal_conv_fwd(x, w, bias, state, lengths, silu, y, tail)
-    return y, tail
+        want_w, want_b, want_state = ctx.needs_input_grad[1:4]
+        if x.shape[0] * x.shape[1] == 0:                                       # no rows: the state went through unchanged
+            dstate = None if not want_state else dtail if dtail is not None else torch.zeros_like(state)
+            return (torch.empty_like(x), torch.zeros_like(w) if want_w else None, torch.zeros_like(bias) if want_b else None, dstate,
+                    None, None)
+        dx, *rest = native.ops.causal_conv_bwd(x, w, bias, state, lengths, ctx.silu, A.adjacent(dy),
+                                               dtail.contiguous() if dtail is not None else None, want_w, want_b, want_state)
+        rest = iter(rest)
+        return (dx, *(next(rest) if want else None for want in (want_w, want_b, want_state)), None, None)
 
 
 def _check_conv(x, w, bias, activation, dims: int) -> bool:
@@ -151,7 +136,10 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     if not A.on_kernels(x):
         return causal_conv_reference(x, w, bias, state, lengths, activation)
     args = (A.adjacent(x), A.dense_f32(w), A.dense_f32(bias), A.adjacent(state), lengths, silu)
-    return _CausalConv.apply(*args) if A.wants_grad(x, w, bias, state) else _causal_conv_fwd(*args)
+    if A.wants_grad(x, w, bias, state):
+        return _CausalConv.apply(*args)
+    y, tail = native.ops.causal_conv_fwd(*args)
+    return y, tail
 
 
 def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -176,10 +164,8 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias
         return y, (new if out is None else out.copy_(new))
     if not (out is None or C == 1 or out.stride(-1) == 1):
         raise ValueError("out: its channels must be adjacent")
-    y = x.new_empty((B, C))
-    new = x.new_empty((B, k - 1, C)) if out is None else out
-    native.ops.causal_conv_step(A.adjacent(x), A.adjacent(state), A.dense_f32(w), A.dense_f32(bias), active, silu, y, new)
-    return y, new
+    y, *new = native.ops.causal_conv_step(A.adjacent(x), A.adjacent(state), A.dense_f32(w), A.dense_f32(bias), active, silu, out)
+    return y, (new[0] if out is None else out)
 
 
 # ---- gated RMSNorm -----------------------------------------------------------------------------------

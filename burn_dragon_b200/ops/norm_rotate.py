@@ -52,11 +52,9 @@ def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, 
     return tuple(outs)
 
 
-def _forward(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps):
-    qo = q.new_empty(q.shape)
-    ko = k.new_empty(k.shape) if k is not None else None
-    native.ops.norm_rotate_fwd(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps, qo, ko)
-    return qo, ko
+def _forward(*args):
+    out = native.ops.norm_rotate_fwd(*args)
+    return out[0], (out[1] if len(out) > 1 else None)
 
 
 class _NormRotate(torch.autograd.Function):
@@ -73,30 +71,14 @@ class _NormRotate(torch.autograd.Function):
         q, k, qw, kw, qb, kb, angles, freqs, positions, lengths = ctx.saved_tensors
         if dqo is None and dko is None:
             return (None,) * 12
-        need = ctx.needs_input_grad
-        like = lambda t, want: torch.empty_like(t) if t is not None and want else None                    # noqa: E731
-        gqw, gkw, gqb, gkb = (like(t, w) for t, w in zip((qw, kw, qb, kb), need[2:6]))
-        gan = torch.empty(angles.shape, device=q.device, dtype=torch.float32) if angles is not None and need[6] else None
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if k is not None else None
-        B, T, Hq, Dh = q.shape
-        if B * T == 0:
-            for t in (gqw, gkw, gqb, gkb):
-                if t is not None:
-                    t.zero_()
-            return dq, dk, gqw, gkw, gqb, gkb, gan, None, None, None, None, None
-        dqo = dqo.contiguous() if dqo is not None else torch.zeros(q.shape, device=q.device, dtype=q.dtype)
-        if k is not None:
-            dko = dko.contiguous() if dko is not None else torch.zeros(k.shape, device=q.device, dtype=q.dtype)
-        bias = gqb is not None or gkb is not None
-        weight = bias or gqw is not None or gkw is not None
-        P = angles.shape[-1] if angles is not None else freqs.shape[0] // 2 if freqs is not None else 0
-        per_head = any(t is not None and t.dim() == 2 for t in (qw, kw, qb, kb))
-        n = native.ops.norm_rotate_scratch(B, T, Hq, k.shape[2] if k is not None else 0, Dh, P, per_head, weight, bias, gan is not None)
-        scratch = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-        native.ops.norm_rotate_bwd(q, k, qw, kw, qb, kb, angles, freqs, positions, ctx.pos0, lengths, ctx.eps, dqo, dko, dq, dk,
-                                   gqw, gkw, gqb, gkb, gan, scratch)
-        return dq, dk, gqw, gkw, gqb, gkb, gan, None, None, None, None, None
+        want = ctx.needs_input_grad[2:7]
+        if q.shape[0] * q.shape[1] == 0:
+            zeros = [torch.zeros_like(t) if w else None for t, w in zip((qw, kw, qb, kb, angles), want)]
+            return (torch.empty_like(q), torch.empty_like(k) if k is not None else None, *zeros, None, None, None, None, None)
+        grads = iter(native.ops.norm_rotate_bwd(
+            q, k, qw, kw, qb, kb, angles, freqs, positions, ctx.pos0, lengths, ctx.eps, dqo.contiguous() if dqo is not None else None,
+            dko.contiguous() if dko is not None else None, sum(1 << i for i, w in enumerate(want) if w)))
+        return (next(grads), next(grads) if k is not None else None, *(next(grads) if w else None for w in want), None, None, None, None, None)
 
 
 def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,

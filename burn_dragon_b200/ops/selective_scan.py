@@ -44,25 +44,13 @@ def selective_scan_reference(u, dt, A, Bm, Cm, D=None, *, dt_bias=None, dt_softp
     return y.to(u.dtype), h
 
 
-def _forward(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, train):
-    B, T, Dn = u.shape
-    N = A.shape[1]
-    n_marks, n_scratch, _ = native.ops.selective_scan_sizes(B, T, Dn, N)
-    y = u.new_empty((B, T, Dn))
-    hT = A.new_empty((B, Dn, N))
-    marks = A.new_empty((n_marks,)) if train else None
-    scratch = A.new_empty((n_scratch,)) if n_scratch else None
-    native.ops.selective_scan_fwd(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, y, hT, marks, scratch)
-    return y, hT, marks
-
-
 class _SelectiveScan(torch.autograd.Function):
     """Kept for the backward pass: the inputs and the states at every 16th step (fp32)."""
 
     @staticmethod
     def forward(ctx, u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths):
         ctx.set_materialize_grads(False)
-        y, hT, marks = _forward(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, True)
+        y, hT, marks = native.ops.selective_scan_fwd(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, True)
         ctx.save_for_backward(u, dt, A, Bm, Cm, D, dt_bias, h0, lengths, marks)
         ctx.softplus = softplus
         return y, hT
@@ -73,20 +61,13 @@ class _SelectiveScan(torch.autograd.Function):
         u, dt, A, Bm, Cm, D, dt_bias, h0, lengths, marks = ctx.saved_tensors
         if dy is None and dhT is None:
             return (None,) * 10
-        B, T, Dn = u.shape
-        N = A.shape[1]
-        f32 = dict(device=u.device, dtype=torch.float32)
-        dy = A_.adjacent(dy) if dy is not None else torch.zeros(B, T, Dn, device=u.device, dtype=u.dtype)
-        dhT = dhT.contiguous() if dhT is not None else None
-        du, ddt = (torch.empty(B, T, Dn, device=u.device, dtype=u.dtype) for _ in range(2))
-        dB, dC = (torch.empty(B, T, N, device=u.device, dtype=u.dtype) for _ in range(2))
-        dA = torch.empty(Dn, N, **f32)
-        dD, dbias = (torch.empty(Dn, **f32) if t is not None else None for t in (D, dt_bias))
-        dh0 = torch.empty(B, Dn, N, **f32) if h0 is not None and ctx.needs_input_grad[8] else None
-        scratch = torch.empty(native.ops.selective_scan_sizes(B, T, Dn, N)[2], **f32)
-        native.ops.selective_scan_bwd(u, dt, A, Bm, Cm, D, dt_bias, ctx.softplus, h0, lengths, marks, scratch, dy, dhT, du, ddt, dA, dB,
-                                      dC, dD, dbias, dh0)
-        return du, ddt, dA, dB, dC, dD, dbias, None, dh0, None
+        want_h0 = ctx.needs_input_grad[8]
+        du, ddt, dA, dB, dC, *rest = native.ops.selective_scan_bwd(
+            u, dt, A, Bm, Cm, D, dt_bias, ctx.softplus, h0, lengths, marks, A_.adjacent(dy), dhT.contiguous() if dhT is not None else None,
+            want_h0)
+        rest = iter(rest)
+        dD, dbias = (next(rest) if t is not None else None for t in (D, dt_bias))
+        return du, ddt, dA, dB, dC, dD, dbias, None, next(rest) if want_h0 else None, None
 
 
 def _check(u, dt, A, Bm, Cm, D, dt_bias, dims: int) -> Tuple[int, int, int]:
@@ -129,7 +110,8 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
             bool(dt_softplus), A_.dense_f32(h0), lengths)
     if A_.wants_grad(u, dt, A, Bm, Cm, D, dt_bias, h0):
         return _SelectiveScan.apply(*args)
-    return _forward(*args, False)[:2]
+    y, hT = native.ops.selective_scan_fwd(*args, False)
+    return y, hT
 
 
 def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, h: torch.Tensor,
@@ -156,8 +138,6 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
     if not (out is None or dense(out)):
         raise ValueError("out: each stream's [D, N] must be dense")
     h = h if dense(h) else h.contiguous()
-    y = u.new_empty((B, Dn))
-    new = h.new_empty((B, Dn, N)) if out is None else out
-    native.ops.selective_scan_step(A_.adjacent(u), A_.adjacent(dt), A_.dense_f32(A), A_.adjacent(Bm), A_.adjacent(Cm), h, A_.dense_f32(D),
-                                   A_.dense_f32(dt_bias), bool(dt_softplus), active, y, new)
-    return y, new
+    y, *new = native.ops.selective_scan_step(A_.adjacent(u), A_.adjacent(dt), A_.dense_f32(A), A_.adjacent(Bm), A_.adjacent(Cm), h,
+                                             A_.dense_f32(D), A_.dense_f32(dt_bias), bool(dt_softplus), active, out)
+    return y, (new[0] if out is None else out)
