@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <vector>
 
 #include "bdh_kernels.h"
@@ -65,6 +66,19 @@ const unsigned char* active_ptr(const OptTensor& t, const Tensor& on, int64_t B)
   if (!given(t)) return nullptr;
   check_dense(*t, on, at::kBool, {B}, "active");
   return reinterpret_cast<const unsigned char*>(t->const_data_ptr());
+}
+
+// A step writes its states while other threads still read their inputs.
+void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs) {
+  const auto end = [](const Tensor& t) {
+    int64_t reach = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.const_data_ptr()) + reach * static_cast<int64_t>(t.element_size());
+  };
+  if (out.numel() == 0) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(t->numel() == 0 || end(*t) <= static_cast<const char*>(out.const_data_ptr()) ||
+                end(out) <= static_cast<const char*>(t->const_data_ptr()), "out overlaps an input other than the state");
 }
 
 Tensor new_f32(const Tensor& on, at::IntArrayRef sizes) { return at::empty(sizes, on.options().dtype(at::kFloat)); }
@@ -151,6 +165,7 @@ std::vector<Tensor> causal_conv_step(const Tensor& x, const Tensor& state, const
   BdhConvDesc d = conv_desc(x, w, bias, state, c10::nullopt, silu);
   std::vector<Tensor> result{new_rows(x, x.sizes())};
   d.y = result[0].data_ptr();
+  if (given(out)) check_apart(*out, {&x, &w});
   set_state_out(d, x, given(out) ? *out : result.emplace_back(new_rows(x, state.sizes())));
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
   return result;
@@ -344,6 +359,7 @@ std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, c10::nullopt, c10::nullopt);
   std::vector<Tensor> result{new_rows(u, u.sizes())};
   d.y = result[0].data_ptr();
+  if (given(out)) check_apart(*out, {&u, &dt, &A, &Bm, &Cm});
   const Tensor to = given(out) ? *out : result.emplace_back(new_f32(u, {d.B, d.D, d.N}));
   for (const Tensor* t : {&h, &to}) {
     check_rows(*t, u, at::kFloat, {d.B, d.D, d.N}, "h");

@@ -75,22 +75,38 @@ def wants_grad(*ts: Optional[torch.Tensor]) -> bool:
     return False
 
 
+def _meet(delta: int, dims: list) -> bool:
+    """Do two tensors of these (stride, size) meet, `delta` elements apart? Strides fall and no row overlaps another."""
+    if not dims:
+        return delta == 0
+    (st, n), rest = dims[0], dims[1:]
+    return any(abs(k) < n and _meet(delta - k * st, rest) for k in (delta // st, delta // st + 1))
+
+
 def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None:
     """`out` of a single-token step: shaped like the state, which it may be; memory it shares with the state otherwise would
     be overwritten before it is read."""
     if out is None:
         return
     check_like(out, src, src.shape, name, src.dtype)
-    if not (not (torch.is_grad_enabled() and out.requires_grad)):
+    if torch.is_grad_enabled() and out.requires_grad:
         raise ValueError(f"{name} requires a gradient; a step form has none")
-    same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
+    strides = out.stride()
+    same = out.data_ptr() == src.data_ptr() and strides == src.stride()
+    dims = sorted((st, n) for st, n in zip(strides, out.shape) if n > 1)
     reach = 1                                            # elements that the dimensions of smaller stride span
-    for st, n in sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1):
+    for st, n in dims:
         if st < reach:
             raise ValueError(f"{name}: its rows overlap one another")
         reach = st * (n - 1) + reach
-    if not same and out.numel():
+    if same or not out.numel() or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr():
+        return
+    if strides == src.stride():                          # slices of one buffer, which may interleave
+        delta, odd = divmod(out.data_ptr() - src.data_ptr(), out.element_size())
+        meet = odd or _meet(delta, dims[::-1])
+    else:
         span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
         (a0, a1), (b0, b1) = span(out), span(src)
-        if not (a1 <= b0 or b1 <= a0 or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr()):
-            raise ValueError(f"{name} overlaps the state without being it")
+        meet = a0 < b1 and b0 < a1
+    if meet:
+        raise ValueError(f"{name} overlaps the state without being it")

@@ -422,3 +422,66 @@ def test_long_sequences_and_other_streams():
     within(y, *want["y"], "y")
     within(torch.cat(ys, 1), *want["y"], "y in pieces")
     within(h, *want["h"], "h")
+
+
+@pytest.mark.gpu
+def test_a_training_step_replays_from_a_graph():
+    """Forward and backward of the whole layer in one captured graph: the bits of the eager step, on new inputs as well."""
+    D, N = 40, 16
+    w = layer_weights("cuda", D, N)
+    x = torch.randn(2, 50, 2 * D + 2 * N + N // 2, device="cuda")
+    n = torch.tensor([50, 21], device="cuda")
+    dy = torch.randn(2, 50, D, device="cuda")
+
+    def step():
+        leaves = {k: t.detach().requires_grad_() for k, t in w.items()}
+        xs = x.detach().requires_grad_()
+        y, _ = layer(xs, leaves, n, (None, None, None))
+        return [y.detach(), *torch.autograd.grad(y, [xs, *leaves.values()], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.mul_(0.5)
+    n.clamp_(max=37)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_in_slices_of_one_buffer(device):
+    """Old and new states interleaved in one buffer, which do not meet, are taken; shifted by a stream, they are refused."""
+    B, D, N = 3, 8, 4
+    g = torch.Generator().manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g).to(device)                                               # noqa: E731
+    row = dict(u=r(B, D), dt=r(B, D).abs(), A=-r(D, N).abs(), Bm=r(B, N), Cm=r(B, N))
+    pair = r(B, 2, D, N)
+    y, h = S.selective_scan_step(**row, h=pair[:, 0].clone())
+    old = pair[:, 0].clone()
+    y2, h2 = S.selective_scan_step(**row, h=pair[:, 0], out=pair[:, 1])
+    assert torch.equal(y, y2) and torch.equal(h, pair[:, 1]) and torch.equal(old, pair[:, 0]) and h2.data_ptr() == pair[:, 1].data_ptr()
+    both = r(2, B + 1, D, N)
+    with pytest.raises(ValueError, match="overlaps"):
+        S.selective_scan_step(**row, h=both[0, 1:], out=both[0, :B])
+    x, w = r(B, D), r(D, 4)
+    rows = r(B, 2, 3, D)
+    _, new = MO.causal_conv_step(x, rows[:, 0].clone(), w)
+    MO.causal_conv_step(x, rows[:, 0], w, out=rows[:, 1])
+    assert torch.equal(new, rows[:, 1])
+
+
+@pytest.mark.gpu
+def test_states_that_overlap_other_inputs_are_refused():
+    """A step reads its inputs while other threads already write states."""
+    w, buf = torch.randn(8, 4, device="cuda"), torch.zeros(2, 4, 8, device="cuda")
+    with pytest.raises(RuntimeError, match="overlaps an input"):
+        MO.causal_conv_step(buf[:, 3], torch.zeros(2, 3, 8, device="cuda"), w, out=buf[:, 1:])
+    z = lambda *s: torch.zeros(*s, device="cuda")                                                        # noqa: E731
+    pool = z(2, 8, 4)
+    with pytest.raises(RuntimeError, match="overlaps an input"):
+        S.selective_scan_step(z(2, 8), z(2, 8), z(8, 4), pool[0, :2], z(2, 4), z(2, 8, 4), out=pool)
