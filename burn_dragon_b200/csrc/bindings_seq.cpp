@@ -1,13 +1,18 @@
 // torch.ops.bdh.* of the parts of a state-space layer (causal convolution, per-head norm + rotation, selective
 // scan). Shapes that the kernels rely on are checked here once more, so that a direct call cannot make them read or
 // write out of range. Unlike in bindings.cpp, results and scratch are allocated here, from torch's allocator on the
-// current stream: a call of one token is as long as its way through Python, and every tensor made there adds to it.
+// current stream, and the derivatives of the sequence forms are autograd nodes of C++: a small call is as long as its
+// way through Python, and every tensor and node made there adds to it.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <initializer_list>
+#include <memory>
+#include <string>
 #include <vector>
 
 #include "bdh_kernels.h"
@@ -16,6 +21,9 @@ namespace {
 
 using at::Tensor;
 using OptTensor = c10::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
 
 void check_rc(int rc, const char* what) { TORCH_CHECK(rc == BDH_OK, "bdh kernel '", what, "' failed with code ", rc); }
 
@@ -84,6 +92,43 @@ void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs)
 Tensor new_f32(const Tensor& on, at::IntArrayRef sizes) { return at::empty(sizes, on.options().dtype(at::kFloat)); }
 Tensor new_rows(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options()); }
 
+// ---- autograd ----------------------------------------------------------------------------------------
+Tensor tensor_of(const OptTensor& t) { return given(t) ? *t : Tensor(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
+OptTensor dense(const Tensor& t) { return t.defined() ? OptTensor(t.contiguous()) : c10::nullopt; }
+OptTensor adjacent(const Tensor& t) {
+  if (!t.defined()) return c10::nullopt;
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A call records a node only if one of these has a gradient.
+bool records(std::initializer_list<const Tensor*> tensors, std::initializer_list<const OptTensor*> others) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (wants(*t)) return true;
+  for (const OptTensor* t : others)
+    if (given(*t) && wants(**t)) return true;
+  return false;
+}
+
+// Gradients are not differentiable again: a second derivative that reaches them ends in an error.
+variable_list first_derivative(variable_list grads, const variable_list& incoming, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  bool recorded = false;
+  for (const Tensor& t : incoming) recorded = recorded || wants(t);
+  if (!recorded) return grads;
+  variable_list in;
+  for (const Tensor& t : grads)
+    if (t.defined()) in.push_back(t.detach().requires_grad_(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", static_cast<int64_t>(in.size()));
+  const variable_list out = (*error)(variable_list(in));
+  size_t i = 0;
+  for (Tensor& t : grads)
+    if (t.defined()) t = out[i++];
+  return grads;
+}
+
 int to_int(int64_t v, const char* name) {
   TORCH_CHECK(v >= 0 && v <= 0x7fffffff - 4096, name, ": too large");
   return static_cast<int>(v);
@@ -119,8 +164,8 @@ void set_state_out(BdhConvDesc& d, const Tensor& x, const Tensor& out) {
 
 std::vector<Tensor> causal_conv_fwd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state,
                                     const OptTensor& lengths, bool silu) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 3 && w.dim() == 2, "x: [B, T, C] on a GPU, w: [C, k]");
   c10::cuda::CUDAGuard guard(x.device());
-  TORCH_CHECK(x.dim() == 3 && w.dim() == 2, "x: [B, T, C], w: [C, k]");
   BdhConvDesc d = conv_desc(x, w, bias, state, lengths, silu);
   Tensor y = new_rows(x, x.sizes()), end = new_rows(x, {d.B, d.k - 1, d.C});
   d.y = y.data_ptr();
@@ -155,6 +200,45 @@ std::vector<Tensor> causal_conv_bwd(const Tensor& x, const Tensor& w, const OptT
   if (want_w || want_bias) partial = new_f32(x, {bdh_causal_conv_partials(&d)});
   check_rc(bdh_causal_conv_bwd(&d, dw, db, partial.defined() ? partial.data_ptr<float>() : nullptr, cur_stream()), "causal_conv_bwd");
   return out;
+}
+
+struct CausalConv : Function<CausalConv> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state,
+                               const OptTensor& lengths, bool silu) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w, tensor_of(bias), tensor_of(state), tensor_of(lengths)});
+    ctx->saved_data["silu"] = silu;
+    ctx->saved_data["want"] = int64_t{wants(w)} | int64_t{wants(tensor_of(bias))} << 1 | int64_t{wants(tensor_of(state))} << 2;
+    return causal_conv_fwd(x, w, bias, state, lengths, silu);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);                              // x, w, bias, state, lengths, silu
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list in = ctx->get_saved_variables();
+      const int64_t want = ctx->saved_data["want"].toInt();
+      if (in[0].size(0) * in[0].size(1) == 0) {        // no rows: the state went through unchanged
+        out[0] = at::empty_like(in[0]);
+        for (int i = 1; i < 4; ++i)
+          if (want >> (i - 1) & 1) out[i] = i == 3 && grads[1].defined() ? grads[1] : at::zeros_like(in[i]);
+      } else {
+        const std::vector<Tensor> made = causal_conv_bwd(in[0], in[1], opt(in[2]), opt(in[3]), opt(in[4]), ctx->saved_data["silu"].toBool(),
+                                                         adjacent(grads[0]), dense(grads[1]), want & 1, want & 2, want & 4);
+        size_t at = 0;
+        out[0] = made[at++];
+        for (int i = 1; i < 4; ++i)
+          if (want >> (i - 1) & 1) out[i] = made[at++];
+      }
+    }
+    return first_derivative(std::move(out), grads, "causal_conv");
+  }
+};
+
+std::vector<Tensor> causal_conv(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
+                                bool silu) {
+  if (!records({&x, &w}, {&bias, &state})) return causal_conv_fwd(x, w, bias, state, lengths, silu);
+  return CausalConv::apply(x, w, bias, state, lengths, silu);
 }
 
 // y, and the new state unless it goes to `out`
@@ -228,6 +312,7 @@ BdhNormRotateDesc norm_desc(const Tensor& q, const OptTensor& k, const OptTensor
 std::vector<Tensor> norm_rotate_fwd(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                     const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
                                     const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
+  TORCH_CHECK(q.is_cuda(), "q: expected a tensor on a GPU");
   c10::cuda::CUDAGuard guard(q.device());
   BdhNormRotateDesc d = norm_desc(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
   std::vector<Tensor> out{new_rows(q, q.sizes())};
@@ -274,6 +359,52 @@ std::vector<Tensor> norm_rotate_bwd(const Tensor& q, const OptTensor& k, const O
   return out;
 }
 
+struct NormRotate : Function<NormRotate> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                               const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
+                               const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, tensor_of(k), tensor_of(q_weight), tensor_of(k_weight), tensor_of(q_bias), tensor_of(k_bias), tensor_of(angles),
+                            tensor_of(freqs), tensor_of(positions), tensor_of(lengths)});
+    int64_t want = 0, i = 0;
+    for (const OptTensor* t : {&q_weight, &k_weight, &q_bias, &k_bias, &angles}) want |= int64_t{wants(tensor_of(*t))} << i++;
+    ctx->saved_data["want"] = want;
+    ctx->saved_data["pos0"] = pos0;
+    ctx->saved_data["eps"] = eps;
+    return norm_rotate_fwd(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(12);                             // in the order of the arguments
+    const Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : Tensor();
+    if (!dq.defined() && !dk.defined()) return out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list in = ctx->get_saved_variables();
+      const int64_t want = ctx->saved_data["want"].toInt();
+      if (in[0].size(0) * in[0].size(1) == 0) {
+        for (int i = 0; i < 7; ++i)
+          if (in[i].defined() && (i < 2 || (want >> (i - 2) & 1))) out[i] = at::zeros_like(in[i]);
+      } else {
+        const std::vector<Tensor> made =
+            norm_rotate_bwd(in[0], opt(in[1]), opt(in[2]), opt(in[3]), opt(in[4]), opt(in[5]), opt(in[6]), opt(in[7]), opt(in[8]),
+                            ctx->saved_data["pos0"].toInt(), opt(in[9]), ctx->saved_data["eps"].toDouble(), dense(dq), dense(dk), want);
+        size_t at = 0;
+        for (int i = 0; i < 7; ++i)
+          if (i == 0 || (i == 1 && in[1].defined()) || (i > 1 && (want >> (i - 2) & 1))) out[i] = made[at++];
+      }
+    }
+    return first_derivative(std::move(out), grads, "norm_rotate");
+  }
+};
+
+std::vector<Tensor> norm_rotate(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                                const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
+                                const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
+  if (!records({&q}, {&k, &q_weight, &k_weight, &q_bias, &k_bias, &angles}))
+    return norm_rotate_fwd(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+  return NormRotate::apply(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
+}
+
 // ---- selective scan ----------------------------------------------------------------------------------
 BdhScanDesc scan_desc(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const OptTensor& skip,
                       const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths) {
@@ -308,8 +439,8 @@ BdhScanDesc scan_desc(const Tensor& u, const Tensor& dt, const Tensor& A, const 
 std::vector<Tensor> selective_scan_fwd(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
                                        const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0,
                                        const OptTensor& lengths, bool train) {
+  TORCH_CHECK(u.is_cuda() && u.dim() == 3, "u: [B, T, D] on a GPU");
   c10::cuda::CUDAGuard guard(u.device());
-  TORCH_CHECK(u.dim() == 3, "u: [B, T, D]");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
   long long n_marks, n_fwd, n_bwd;
   bdh_selective_scan_sizes(&d, &n_marks, &n_fwd, &n_bwd);
@@ -350,6 +481,45 @@ std::vector<Tensor> selective_scan_bwd(const Tensor& u, const Tensor& dt, const 
   return out;
 }
 
+// Kept for the backward pass: the inputs and the states at every 16th step (fp32).
+struct SelectiveScan : Function<SelectiveScan> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                               const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0, const OptTensor& lengths) {
+    ctx->set_materialize_grads(false);
+    std::vector<Tensor> made = selective_scan_fwd(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths, true);
+    ctx->save_for_backward({u, dt, A, Bm, Cm, tensor_of(skip), tensor_of(dt_bias), tensor_of(h0), tensor_of(lengths), made[2]});
+    ctx->saved_data["softplus"] = softplus;
+    ctx->saved_data["want_h0"] = wants(tensor_of(h0));
+    made.pop_back();
+    return made;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(10);                             // in the order of the arguments
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    {
+      at::AutoGradMode off(false);
+      const variable_list in = ctx->get_saved_variables();
+      const bool want_h0 = ctx->saved_data["want_h0"].toBool();
+      const std::vector<Tensor> made =
+          selective_scan_bwd(in[0], in[1], in[2], in[3], in[4], opt(in[5]), opt(in[6]), ctx->saved_data["softplus"].toBool(), opt(in[7]),
+                             opt(in[8]), in[9], adjacent(grads[0]), dense(grads[1]), want_h0);
+      size_t at = 0;
+      for (int i = 0; i < 7; ++i)
+        if (in[i].defined()) out[i] = made[at++];
+      if (want_h0) out[8] = made[at];
+    }
+    return first_derivative(std::move(out), grads, "selective_scan");
+  }
+};
+
+std::vector<Tensor> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                                   const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0,
+                                   const OptTensor& lengths) {
+  if (!records({&u, &dt, &A, &Bm, &Cm}, {&skip, &dt_bias, &h0}))
+    return selective_scan_fwd(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths, false);
+  return SelectiveScan::apply(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
+}
+
 // y, and the new state unless it goes to `out`
 std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm, const Tensor& h,
                                         const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& active,
@@ -373,29 +543,24 @@ std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(bdh, m) {
-  m.def("causal_conv_fwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> Tensor[]");
-  m.def("causal_conv_bwd(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu, Tensor? dy, "
-        "Tensor? dstate_out, bool want_w, bool want_bias, bool want_state) -> Tensor[]");
+  m.def("causal_conv(Tensor x, Tensor w, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> Tensor[]");
   m.def("causal_conv_step(Tensor x, Tensor state, Tensor w, Tensor? bias, Tensor? active, bool silu, Tensor(a!)? out) -> Tensor[]");
-  m.def("norm_rotate_fwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
+  m.def("norm_rotate(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
         "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps) -> Tensor[]");
-  m.def("norm_rotate_bwd(Tensor q, Tensor? k, Tensor? q_weight, Tensor? k_weight, Tensor? q_bias, Tensor? k_bias, Tensor? angles, "
-        "Tensor? freqs, Tensor? positions, int pos0, Tensor? lengths, float eps, Tensor? dq_out, Tensor? dk_out, int want) -> Tensor[]");
-  m.def("selective_scan_fwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
-        "Tensor? lengths, bool train) -> Tensor[]");
-  m.def("selective_scan_bwd(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
-        "Tensor? lengths, Tensor marks, Tensor? dy, Tensor? dhT, bool want_h0) -> Tensor[]");
+  m.def("selective_scan(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? dt_bias, bool softplus, Tensor? h0, "
+        "Tensor? lengths) -> Tensor[]");
   m.def("selective_scan_step(Tensor u, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor h, Tensor? D, Tensor? dt_bias, bool softplus, "
         "Tensor? active, Tensor(a!)? out) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(bdh, CUDA, m) {
-  m.impl("causal_conv_fwd", &causal_conv_fwd);
-  m.impl("causal_conv_bwd", &causal_conv_bwd);
   m.impl("causal_conv_step", &causal_conv_step);
-  m.impl("norm_rotate_fwd", &norm_rotate_fwd);
-  m.impl("norm_rotate_bwd", &norm_rotate_bwd);
-  m.impl("selective_scan_fwd", &selective_scan_fwd);
-  m.impl("selective_scan_bwd", &selective_scan_bwd);
   m.impl("selective_scan_step", &selective_scan_step);
+}
+
+// (these record their own nodes)
+TORCH_LIBRARY_IMPL(bdh, CompositeImplicitAutograd, m) {
+  m.impl("causal_conv", &causal_conv);
+  m.impl("norm_rotate", &norm_rotate);
+  m.impl("selective_scan", &selective_scan);
 }

@@ -80,32 +80,6 @@ def causal_conv_reference(x, w, bias=None, state=None, lengths=None, activation:
     return torch.where(keep[..., None], y, 0.0).to(x.dtype), tail.to(x.dtype)
 
 
-class _CausalConv(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, bias, state, lengths, silu):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, w, bias, state, lengths)
-        ctx.silu = silu
-        y, tail = native.ops.causal_conv_fwd(x, w, bias, state, lengths, silu)
-        return y, tail
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dtail):
-        x, w, bias, state, lengths = ctx.saved_tensors
-        if dy is None and dtail is None:
-            return (None,) * 6
-        want_w, want_b, want_state = ctx.needs_input_grad[1:4]
-        if x.shape[0] * x.shape[1] == 0:                                       # no rows: the state went through unchanged
-            dstate = None if not want_state else dtail if dtail is not None else torch.zeros_like(state)
-            return (torch.empty_like(x), torch.zeros_like(w) if want_w else None, torch.zeros_like(bias) if want_b else None, dstate,
-                    None, None)
-        dx, *rest = native.ops.causal_conv_bwd(x, w, bias, state, lengths, ctx.silu, A.adjacent(dy),
-                                               dtail.contiguous() if dtail is not None else None, want_w, want_b, want_state)
-        rest = iter(rest)
-        return (dx, *(next(rest) if want else None for want in (want_w, want_b, want_state)), None, None)
-
-
 def _check_conv(x, w, bias, activation, dims: int) -> bool:
     if not (x.dim() == dims and x.is_floating_point()):
         raise ValueError(f"x: expected a floating tensor of {dims} dimensions, got {x.dtype} {tuple(x.shape)}")
@@ -135,10 +109,7 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     lengths = A.check_lengths(lengths, x, B)
     if not A.on_kernels(x):
         return causal_conv_reference(x, w, bias, state, lengths, activation)
-    args = (A.adjacent(x), A.dense_f32(w), A.dense_f32(bias), A.adjacent(state), lengths, silu)
-    if A.wants_grad(x, w, bias, state):
-        return _CausalConv.apply(*args)
-    y, tail = native.ops.causal_conv_fwd(*args)
+    y, tail = native.ops.causal_conv(A.adjacent(x), A.dense_f32(w), A.dense_f32(bias), A.adjacent(state), lengths, silu)
     return y, tail
 
 

@@ -52,35 +52,6 @@ def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, 
     return tuple(outs)
 
 
-def _forward(*args):
-    out = native.ops.norm_rotate_fwd(*args)
-    return out[0], (out[1] if len(out) > 1 else None)
-
-
-class _NormRotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, qw, kw, qb, kb, angles, freqs, positions, lengths)
-        ctx.pos0, ctx.eps = pos0, eps
-        return _forward(q, k, qw, kw, qb, kb, angles, freqs, positions, pos0, lengths, eps)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dqo, dko):
-        q, k, qw, kw, qb, kb, angles, freqs, positions, lengths = ctx.saved_tensors
-        if dqo is None and dko is None:
-            return (None,) * 12
-        want = ctx.needs_input_grad[2:7]
-        if q.shape[0] * q.shape[1] == 0:
-            zeros = [torch.zeros_like(t) if w else None for t, w in zip((qw, kw, qb, kb, angles), want)]
-            return (torch.empty_like(q), torch.empty_like(k) if k is not None else None, *zeros, None, None, None, None, None)
-        grads = iter(native.ops.norm_rotate_bwd(
-            q, k, qw, kw, qb, kb, angles, freqs, positions, ctx.pos0, lengths, ctx.eps, dqo.contiguous() if dqo is not None else None,
-            dko.contiguous() if dko is not None else None, sum(1 << i for i, w in enumerate(want) if w)))
-        return (next(grads), next(grads) if k is not None else None, *(next(grads) if w else None for w in want), None, None, None, None, None)
-
-
 def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
                 k_weight: Optional[torch.Tensor] = None, q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, *,
                 angles: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
@@ -143,8 +114,7 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     pos = None
     if isinstance(positions, torch.Tensor):
         pos = positions if positions.dim() == 2 else positions.expand(B, T)
-    args = (A.adjacent(q), A.adjacent(k), A.dense_f32(q_weight), A.dense_f32(k_weight), A.dense_f32(q_bias), A.dense_f32(k_bias),
-            A.adjacent(angles.float()) if angles is not None else None, A.dense_f32(freqs), pos, pos0, lengths, float(eps))
-    if A.wants_grad(q, k, q_weight, k_weight, q_bias, k_bias, angles):
-        return _NormRotate.apply(*args)
-    return _forward(*args)
+    out = native.ops.norm_rotate(
+        A.adjacent(q), A.adjacent(k), A.dense_f32(q_weight), A.dense_f32(k_weight), A.dense_f32(q_bias), A.dense_f32(k_bias),
+        A.adjacent(angles.float()) if angles is not None else None, A.dense_f32(freqs), pos, pos0, lengths, float(eps))
+    return out[0], (out[1] if k is not None else None)

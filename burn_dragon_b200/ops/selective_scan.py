@@ -44,32 +44,6 @@ def selective_scan_reference(u, dt, A, Bm, Cm, D=None, *, dt_bias=None, dt_softp
     return y.to(u.dtype), h
 
 
-class _SelectiveScan(torch.autograd.Function):
-    """Kept for the backward pass: the inputs and the states at every 16th step (fp32)."""
-
-    @staticmethod
-    def forward(ctx, u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths):
-        ctx.set_materialize_grads(False)
-        y, hT, marks = native.ops.selective_scan_fwd(u, dt, A, Bm, Cm, D, dt_bias, softplus, h0, lengths, True)
-        ctx.save_for_backward(u, dt, A, Bm, Cm, D, dt_bias, h0, lengths, marks)
-        ctx.softplus = softplus
-        return y, hT
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dhT):
-        u, dt, A, Bm, Cm, D, dt_bias, h0, lengths, marks = ctx.saved_tensors
-        if dy is None and dhT is None:
-            return (None,) * 10
-        want_h0 = ctx.needs_input_grad[8]
-        du, ddt, dA, dB, dC, *rest = native.ops.selective_scan_bwd(
-            u, dt, A, Bm, Cm, D, dt_bias, ctx.softplus, h0, lengths, marks, A_.adjacent(dy), dhT.contiguous() if dhT is not None else None,
-            want_h0)
-        rest = iter(rest)
-        dD, dbias = (next(rest) if t is not None else None for t in (D, dt_bias))
-        return du, ddt, dA, dB, dC, dD, dbias, None, next(rest) if want_h0 else None, None
-
-
 def _check(u, dt, A, Bm, Cm, D, dt_bias, dims: int) -> Tuple[int, int, int]:
     if not (u.dim() == dims and u.is_floating_point()):
         raise ValueError(f"u: expected a floating tensor of {dims} dimensions, got {u.dtype} {tuple(u.shape)}")
@@ -106,11 +80,8 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
     lengths = A_.check_lengths(lengths, u, B)
     if not A_.on_kernels(u) or u.shape[0] * u.shape[1] == 0:
         return selective_scan_reference(u, dt, A, Bm, Cm, D, dt_bias=dt_bias, dt_softplus=dt_softplus, h0=h0, lengths=lengths)
-    args = (A_.adjacent(u), A_.adjacent(dt), A_.dense_f32(A), A_.adjacent(Bm), A_.adjacent(Cm), A_.dense_f32(D), A_.dense_f32(dt_bias),
-            bool(dt_softplus), A_.dense_f32(h0), lengths)
-    if A_.wants_grad(u, dt, A, Bm, Cm, D, dt_bias, h0):
-        return _SelectiveScan.apply(*args)
-    y, hT = native.ops.selective_scan_fwd(*args, False)
+    y, hT = native.ops.selective_scan(A_.adjacent(u), A_.adjacent(dt), A_.dense_f32(A), A_.adjacent(Bm), A_.adjacent(Cm), A_.dense_f32(D),
+                                      A_.dense_f32(dt_bias), bool(dt_softplus), A_.dense_f32(h0), lengths)
     return y, hT
 
 

@@ -485,3 +485,55 @@ def test_states_that_overlap_other_inputs_are_refused():
     pool = z(2, 8, 4)
     with pytest.raises(RuntimeError, match="overlaps an input"):
         S.selective_scan_step(z(2, 8), z(2, 8), z(8, 4), pool[0, :2], z(2, 4), z(2, 8, 4), out=pool)
+
+
+def _calls(device):
+    """{operator: (call of its tensors, those tensors)}, every one of which has a gradient."""
+    g = torch.Generator().manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=g).to(device)                                               # noqa: E731
+    B, T, D, N = 2, 9, 8, 4
+    return {
+        "conv": (lambda x, w, b, st: MO.causal_conv(x, w, b, state=st), [r(B, T, D), r(D, 4), r(D), r(B, 3, D)]),
+        "norm_rotate": (lambda q, k, qw, kw, qb, kb, an: NR.norm_rotate(q, k, qw, kw, qb, kb, angles=an),
+                        [r(B, T, 3, D), r(B, T, 2, D), r(D), r(D), r(D), r(D), r(B, T, 3)]),
+        "scan": (lambda u, dt, A, Bm, Cm, Dk, db, h0: S.selective_scan(u, dt, A, Bm, Cm, Dk, dt_bias=db, dt_softplus=True, h0=h0),
+                 [r(B, T, D), r(B, T, D), -r(D, N).abs(), r(B, T, N), r(B, T, N), r(D), r(D), r(B, D, N)]),
+    }
+
+
+@pytest.mark.parametrize("name", ["conv", "norm_rotate", "scan"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_each_gradient_alone_and_each_result_alone(device, name):
+    """One input with a gradient at a time, and one result used at a time, give what all of them together give. A gradient
+    is a sum of at most 144 terms, each off by at most 24 u: two ways to it differ by 2 (144 + 24) u = 2e-5 of the
+    terms' magnitudes, which are at most 50 times the largest gradient here; a gradient of another input is off by all of it."""
+    fn, tensors = _calls(device)[name]
+    leaves = [t.clone().requires_grad_() for t in tensors]
+    outs = fn(*leaves)
+    seeds = [torch.randn(o.shape, generator=torch.Generator().manual_seed(2)).to(device) for o in outs]
+    together = torch.autograd.grad(outs, leaves, seeds)
+    parts = [torch.autograd.grad(fn(*leaves)[i], leaves, seeds[i], allow_unused=True) for i in range(2)]
+    for i, want in enumerate(together):
+        leaf = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(tensors)]
+        used = [(o, s) for o, s in zip(fn(*leaf), seeds) if o.requires_grad]
+        got, = torch.autograd.grad([o for o, _ in used], leaf[i], [s for _, s in used])
+        both = sum(p[i] for p in parts if p[i] is not None)
+        scale = want.abs().max() + sum(p[i].abs().max() for p in parts if p[i] is not None)
+        assert (got - want).abs().max() <= 1e-3 * scale and (both - want).abs().max() <= 1e-3 * scale, i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["conv", "norm_rotate", "scan"])
+def test_a_second_derivative_is_refused(name):
+    fn, tensors = _calls("cuda")[name]
+    leaves = [t.clone().requires_grad_() for t in tensors]
+    out = fn(*leaves)[0]
+    seed = torch.ones_like(out).requires_grad_()
+    first = torch.autograd.grad(out, leaves[0], seed, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        first.sum().backward()
+    with pytest.raises(RuntimeError):                                        # no way from it to the input, which grad() refuses
+        torch.autograd.grad(first.sum(), leaves[0])
+    out = fn(*leaves)[0]
+    plain, = torch.autograd.grad(out, leaves[0], seed.detach())
+    assert torch.equal(first.detach(), plain)
