@@ -55,7 +55,7 @@ struct ScanArgs {
   int tiles, per_seg, segs;            // tiles per sequence, per segment; segments
   int parts;                           // warps (forward) or blocks (backward) across the channels
   const float* seg_state;              // [B][segs][D][NP]: states of the segments from zero (forward or reverse)
-  const float* seg_dt;                 // [B][segs][D]: their total steps (times log2(e), as every step here)
+  const float* seg_dt;                 // [B][segs][D]: their total steps
 };
 
 __device__ __forceinline__ void load4(const float* p, f2& x, f2& y) {
@@ -75,14 +75,13 @@ __device__ __forceinline__ f2 exp_minus_abs(f2 x) {
   return fma2(t, mul2(lo, both(LN2)), t);
 }
 
-// softplus(x) log2(e) = max(x, 0) log2(e) + log2(1 + exp(-|x|)) for two steps at once: the steps are kept in this unit, so
-// that the exponent of a decay is one product, rounded once. log2(1 + t) / t on [0, 1] is the polynomial of degree 9
-// through its values at the Chebyshev nodes: off by at most 5.4e-9 of itself (the nearest singularity, t = -1, makes the
-// error fall by 3 + 2 sqrt(2) a degree), so the result is off by the 32-bit rounding.
+// softplus(x) = max(x, 0) + log1p(exp(-|x|)) for two steps at once. log1p(t) / t on [0, 1] is the polynomial of degree 9
+// through its values at the Chebyshev nodes: off by at most 5.4e-9 of itself (the nearest singularity, t = -1,
+// makes the error fall by 3 + 2 sqrt(2) a degree), so the result is off by the 32-bit rounding.
 __device__ __forceinline__ f2 softplus2(f2 x) {
-  constexpr float P[10] = {1.4426950216293335f, -0.7213459610939026f, 0.4808460772037506f, -0.3599757254123688f,
-                           0.28368109464645386f, -0.22029472887516022f, 0.15211233496665955f, -0.08132993429899216f,
-                           0.02819390781223774f, -0.00458208192139864f};
+  constexpr float P[10] = {1.0f, -0.49999892711639404f, 0.33329710364341736f, -0.24951615929603577f, 0.1966327428817749f,
+                           -0.1526966691017151f, 0.10543623566627502f, -0.056373611092567444f, 0.019542526453733444f,
+                           -0.0031760570127516985f};
   const f2 t = exp_minus_abs(x);
   f2 p = both(P[9]);
 #pragma unroll
@@ -91,7 +90,7 @@ __device__ __forceinline__ f2 softplus2(f2 x) {
   unpack2(x, a, b);
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(ma) : "f"(a));
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(mb) : "f"(b));
-  return fma2(pack2(ma, mb), both(LOG2E), mul2(p, t));
+  return fma2(p, t, pack2(ma, mb));
 }
 // its derivative, 1 / (1 + exp(-x))
 __device__ __forceinline__ f2 sigmoid2(f2 x) {
@@ -280,7 +279,7 @@ struct Ring {
 template <int G, int CT, bool DY>
 struct alignas(16) WarpMem {
   static constexpr int NP = 4 * G, CW = 32 / G * CT;
-  float2 step[LT][CW + 2];                             // dt' log2(e), dt' u
+  float2 step[LT][CW + 2];                             // dt', dt' u
   float dy[DY ? LT : 1][CW + 4];
   float bias[CW], skip[CW];
 
@@ -311,11 +310,11 @@ struct alignas(16) WarpMem {
 #pragma unroll
     for (int j = 0; j < S::E; j += 2) {
       f2 s = pack2(dt[j], dt[j + 1]);
-      s = d.softplus ? softplus2(s) : mul2(s, both(LOG2E));
+      if (d.softplus) s = softplus2(s);
       s = mul2(s, both(keep));
       float s0, s1, v0, v1;
       unpack2(s, s0, s1);
-      unpack2(mul2(mul2(s, both(LN2)), pack2(uu[j], uu[j + 1])), v0, v1);
+      unpack2(mul2(s, pack2(uu[j], uu[j + 1])), v0, v1);
       if constexpr (S::E > 1)
         *reinterpret_cast<float4*>(&step[t][c + j]) = make_float4(s0, v0, s1, v1);
       else
@@ -369,17 +368,21 @@ __device__ __forceinline__ void store_state(float* p, int c, int n0, const BdhSc
     if (c < d.D && n0 + j < d.N) p[static_cast<long long>(c) * d.N + n0 + j] = v[j];
 }
 
-// A; 0 for padding
+// A2 = A log2(e); 0 for padding
 template <int CT>
-__device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (&rate)[CT][2]) {
+__device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (&A2)[CT][2]) {
 #pragma unroll
-  for (int k = 0; k < CT; ++k) load_state(d.A, c + k, n0, d, rate[k]);
+  for (int k = 0; k < CT; ++k) {
+    load_state(d.A, c + k, n0, d, A2[k]);
+    A2[k][0] = mul2(A2[k][0], both(LOG2E));
+    A2[k][1] = mul2(A2[k][1], both(LOG2E));
+  }
 }
 
 // The state a segment starts from: `h` (the sequence's own) carried through the segments before it, in order; in reverse
 // through those behind it.
 template <int CT, int NP>
-__device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to, int by, int c, int n0, const f2 (&rate)[CT][2], f2 (&h)[CT][2]) {
+__device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to, int by, int c, int n0, const f2 (&A2)[CT][2], f2 (&h)[CT][2]) {
   for (int s = from; s != to; s += by) {
 #pragma unroll
     for (int k = 0; k < CT; ++k) {
@@ -388,8 +391,8 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
       const f2 dt = both(a.seg_dt[at]);
       f2 s0, s1;
       load4(a.seg_state + at * NP + n0, s0, s1);
-      h[k][0] = fma2(ex2x2(mul2(dt, rate[k][0])), h[k][0], s0);
-      h[k][1] = fma2(ex2x2(mul2(dt, rate[k][1])), h[k][1], s1);
+      h[k][0] = fma2(ex2x2(mul2(dt, A2[k][0])), h[k][0], s0);
+      h[k][1] = fma2(ex2x2(mul2(dt, A2[k][1])), h[k][1], s1);
     }
   }
 }
@@ -401,7 +404,7 @@ struct Steps {
   static constexpr int N = 4 / CT;
   f2 e[N][CT][2], in[N][CT][2], k[WANT_C ? N : 1][2];
   template <typename Mem, typename Rows>
-  __device__ __forceinline__ void make(const Mem& sh, const Rows& rows, int t, int cl, int n0, const f2 (&rate)[CT][2]) {
+  __device__ __forceinline__ void make(const Mem& sh, const Rows& rows, int t, int cl, int n0, const f2 (&A2)[CT][2]) {
 #pragma unroll
     for (int s = 0; s < N; ++s) {
       float dt[CT], du[CT];
@@ -411,8 +414,8 @@ struct Steps {
       if constexpr (WANT_C) rows.C(t + s, n0, k[s]);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        e[s][c][0] = ex2x2(mul1(dt[c], rate[c][0]));
-        e[s][c][1] = ex2x2(mul1(dt[c], rate[c][1]));
+        e[s][c][0] = ex2x2(mul1(dt[c], A2[c][0]));
+        e[s][c][1] = ex2x2(mul1(dt[c], A2[c][1]));
         in[s][c][0] = mul1(du[c], b[0]);
         in[s][c][1] = mul1(du[c], b[1]);
       }
@@ -466,12 +469,12 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
   const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles), end = min(last, (len + LT - 1) / LT);
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) sh.ring.template load<true, true>(d, first + i, end, w.b, c0, len);
-  f2 rate[CT][2], h[CT][2];
-  load_a<CT>(d, c, n0, rate);
+  f2 A2[CT][2], h[CT][2];
+  load_a<CT>(d, c, n0, A2);
 #pragma unroll
   for (int k = 0; k < CT; ++k)
     load_state(d.h0 ? d.h0 + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, h[k]);
-  carry<CT, S::NP>(a, w.b, 0, w.seg, 1, c, n0, rate, h);
+  carry<CT, S::NP>(a, w.b, 0, w.seg, 1, c, n0, A2, h);
   sh.in.params(d, c0);
   __syncwarp();
   const int row = lane / 2, col = (lane & 1) * S::E;
@@ -491,10 +494,10 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
                 make_ulonglong2(h[k][0], h[k][1]);
       using Group = Steps<G, CT, true>;
       Group now, next;
-      now.make(sh.in, bc, 0, cl, n0, rate);
+      now.make(sh.in, bc, 0, cl, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, rate);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
@@ -568,9 +571,9 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
   const auto tile_of = [&](int i) { return REV ? end - 1 - i : first + i; };
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) sh.ring.template load<!REV, REV>(d, i < n ? tile_of(i) : -1, end, w.b, c0, len);
-  f2 rate[CT][2], h[CT][2];
+  f2 A2[CT][2], h[CT][2];
   float total[CT];
-  load_a<CT>(d, c, n0, rate);
+  load_a<CT>(d, c, n0, A2);
 #pragma unroll
   for (int k = 0; k < CT; ++k) {
     h[k][0] = h[k][1] = both(0.f);
@@ -603,8 +606,8 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
         }
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
-          e[s][k][0] = ex2x2(mul1(dt[k], rate[k][0]));
-          e[s][k][1] = ex2x2(mul1(dt[k], rate[k][1]));
+          e[s][k][0] = ex2x2(mul1(dt[k], A2[k][0]));
+          e[s][k][1] = ex2x2(mul1(dt[k], A2[k][1]));
           in[s][k][0] = mul1(du[k], b[0]);
           in[s][k][1] = mul1(du[k], b[1]);
           total[k] += dt[k];
@@ -643,7 +646,7 @@ struct BwdMem {
   struct PerWarp {
     WarpMem<G, CT, true> in;
     alignas(16) T B[LT * NP], C[LT * NP];
-    float2 out[LT][CW + 2];            // sum g B, sum A q
+    float2 out[LT][CW + 2];            // sum g B, sum A2 q
     ulonglong2 h[LT][CT][32];          // h_{t-1}, each lane its own
     __device__ __forceinline__ RowsOf<T, NP> bc() const { return {B, C}; }
   } warp[BWD_WARPS];
@@ -677,14 +680,14 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
   const Where w = where(a, blockIdx.x);
   const int n0 = lane % G * 4, cl = lane / G * CT, c0 = (w.part * BWD_WARPS + warp) * S::CW, c = c0 + cl;
   const int len = a.len.get(w.b, d.T);
-  f2 rate[CT][2], r[CT][2], da[CT][2];
-  load_a<CT>(d, c, n0, rate);
+  f2 A2[CT][2], r[CT][2], da[CT][2];
+  load_a<CT>(d, c, n0, A2);
 #pragma unroll
   for (int k = 0; k < CT; ++k) {
     load_state(d.dhT ? d.dhT + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, r[k]);
     da[k][0] = da[k][1] = both(0.f);
   }
-  carry<CT, S::NP>(a, w.b, a.segs - 1, w.seg, -1, c, n0, rate, r);
+  carry<CT, S::NP>(a, w.b, a.segs - 1, w.seg, -1, c, n0, A2, r);
   sh.in.params(d, c0);
   float sum_skip[S::E], sum_bias[S::E];                // of this lane's channels, over its rows
 #pragma unroll
@@ -732,10 +735,10 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
       using Group = Steps<G, CT, false>;
       const RowsOf<T, S::NP> bc = sh.bc();
       Group now, next;
-      now.make(sh.in, bc, 0, cl, n0, rate);
+      now.make(sh.in, bc, 0, cl, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, rate);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
         for (int k = 0; k < CT; ++k) {
           const float dt = at_t.dt[k], du = at_t.du[k], gy = at_t.gy[k];
           const f2 g0 = fma1(gy, at_t.c[0], r[k][0]), g1 = fma1(gy, at_t.c[1], r[k][1]);
-          const f2 e0 = ex2x2(mul1(dt, rate[k][0])), e1 = ex2x2(mul1(dt, rate[k][1]));
+          const f2 e0 = ex2x2(mul1(dt, A2[k][0])), e1 = ex2x2(mul1(dt, A2[k][1]));
           if (k == 0) {
             sb0 = mul1(du, g0); sb1 = mul1(du, g1);
             sc0 = mul1(gy, h[k][0]); sc1 = mul1(gy, h[k][1]);
@@ -773,7 +776,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           dat[k][0] = fma1(dt, q0, dat[k][0]);
           dat[k][1] = fma1(dt, q1, dat[k][1]);
           nv[2 * k] = sum2(fma2(g1, at_t.b[1], mul2(g0, at_t.b[0])));
-          nv[2 * k + 1] = sum2(fma2(rate[k][1], q1, mul2(rate[k][0], q0)));
+          nv[2 * k + 1] = sum2(fma2(A2[k][1], q1, mul2(A2[k][0], q0)));
         }
         int at;
         bool once;
@@ -820,8 +823,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           dd[j] = 0.f;
           if (in) {
             const float2 s = sh.out[row][cc];
-            du = fmaf(LN2 * sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
-            dd[j] = fmaf(u[i][j], s.x, s.y);
+            du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
+            dd[j] = fmaf(u[i][j], s.x, LN2 * s.y);
             sum_skip[i * S::V + j] = fmaf(dy[i][j], u[i][j], sum_skip[i * S::V + j]);
           }
           pu.set(j, du);
@@ -860,9 +863,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
   const long long seg = static_cast<long long>(w.b) * a.segs + w.seg;
 #pragma unroll
   for (int k = 0; k < CT; ++k) {
-    if (c + k < d.D)
-      *reinterpret_cast<ulonglong2*>(o.da + (seg * d.D + c + k) * S::NP + n0) =
-          make_ulonglong2(mul2(da[k][0], both(LN2)), mul2(da[k][1], both(LN2)));
+    if (c + k < d.D) *reinterpret_cast<ulonglong2*>(o.da + (seg * d.D + c + k) * S::NP + n0) = make_ulonglong2(da[k][0], da[k][1]);
     if (w.seg == 0 && d.dh0 != nullptr) store_state(d.dh0 + static_cast<long long>(w.b) * d.D * d.N, c + k, n0, d, r[k]);
   }
   // the 16 lanes of a warp that share channels add their sums up
@@ -941,7 +942,7 @@ __global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = live && n0 + j < d.N ? d.A[at + j] : 0.f;
+  for (int j = 0; j < 4; ++j) a[j] = live && n0 + j < d.N ? d.A[at + j] * LOG2E : 0.f;
   const float bias = live && d.dt_bias ? d.dt_bias[c] : 0.f, skip = live && d.skip ? d.skip[c] : 0.f;
   float step[OWN], input[OWN];
 #pragma unroll
@@ -952,7 +953,6 @@ __global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const
     step[k] = on ? elem_to_float<T>(static_cast<const T*>(d.dt)[b * d.dt_sb + c]) + bias : 0.f;
     float same;
     if (d.softplus) unpack2(softplus2(both(step[k])), step[k], same);
-    else step[k] *= LOG2E;
     if (!on) step[k] = 0.f;
   }
   const int first = lane - ng;
@@ -968,7 +968,7 @@ __global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n0 + j < d.N) {
-          v[r][j] = fmaf(ex2(dt * a[j]), v[r][j], dt * LN2 * u * elem_to_float<T>(pb[j]));
+          v[r][j] = fmaf(ex2(dt * a[j]), v[r][j], dt * u * elem_to_float<T>(pb[j]));
           sum = fmaf(elem_to_float<T>(pc[j]), v[r][j], sum);
         }
     }
