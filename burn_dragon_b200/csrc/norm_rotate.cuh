@@ -13,7 +13,7 @@
 // groups of hr rows, each of q or of k alone, so that a weight's gradient stays in registers over all rows that share
 // it. Sums are fp32, in a fixed order.
 //
-// Measured, 4 x 4096 tokens, 32 + 8 heads of 128, bf16: forward 87 us (0.60 of the copy rate), backward 156 us (0.50): the
+// Measured, 4 x 4096 tokens, 32 + 8 heads of 128, bf16: forward 89 us (0.60 of the copy rate), backward 158 us (0.50): the
 // pairs' turns and conversions issue about 20 instructions a pair of elements. 64 tokens alone: 5 us.
 #pragma once
 #include "bdh_kernels.h"
