@@ -102,7 +102,7 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     passed as `state` with the sequence's next rows (None: zeros). Rows are fp32, fp16 or bf16 (y and the states are of
     their type), sums fp32; x and the state may be views whose channels are adjacent. `lengths` [B]: the rows of each sequence that
     count; y is 0 behind them, the state ends there, and whatever x holds there is not read. Differentiable in x, w,
-    bias and both states; the sums over rows are made in a fixed order."""
+    bias and both states, once (no second derivative); the sums over rows are made in a fixed order."""
     silu = _check_conv(x, w, bias, activation, 3)
     B, T, C = x.shape
     A.check_like(state, x, (B, w.shape[1] - 1, C), "state", x.dtype)
@@ -117,8 +117,9 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, w: torch.Tensor, bias
                      activation: Optional[str] = "silu", active: Optional[torch.Tensor] = None,
                      out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`causal_conv` for one row of every stream: x [B, C], state [B, k-1, C] -> (y [B, C], state'). The state is left
-    as it was unless `out=state` asks for the update in place (`out`: where state' goes). `active` [B] (bool): a stream
-    marked false gives y = 0 and keeps its state. No gradients (a decoding form)."""
+    as it was unless `out=state` asks for the update in place (`out`: where state' goes, which is the state itself or
+    shares no memory with an input). `active` [B] (bool): a stream marked false gives y = 0 and keeps its state. No
+    gradients (a decoding form)."""
     silu = _check_conv(x, w, bias, activation, 2)
     B, C = x.shape
     k = w.shape[1]

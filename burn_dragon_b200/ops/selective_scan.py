@@ -72,7 +72,7 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
     """u, dt [B, T, D], A [D, N] (N <= 64, finite), Bm, Cm [B, T, N], D and dt_bias [D], h0 [B, D, N] (fp32; None: zeros)
     -> (y [B, T, D] in the rows' type, hT [B, D, N] fp32). Rows are fp32, fp16 or bf16, all alike, and may be views into a
     wider projection (elements of a row adjacent). `lengths` [B]: behind a sequence's length the state stays as it
-    is, y is 0, and the inputs are not read. Differentiable in everything but `lengths`, the carried states included;
+    is, y is 0, and the inputs are not read. Differentiable once in everything but `lengths`, the carried states included;
     a forward pass under autograd keeps the fp32 states of every 16th step (B T D N / 4 bytes, N rounded up to 8, 16, 32
     or 64). All states and sums are fp32, sums over rows and channels in a fixed order."""
     B, Dn, N = _check(u, dt, A, Bm, Cm, D, dt_bias, 3)
@@ -90,7 +90,7 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: 
                         active: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`selective_scan` for one row of every stream: u, dt [B, D], Bm, Cm [B, N], h [B, D, N] (fp32) -> (y [B, D], h'). The
     state is left as it was unless `out=h` asks for the update in place (`out`: where h' goes; like h it may be a
-    slice of a larger tensor as long as each stream's [D, N] is dense). `active` [B] (bool): a stream marked false gives
+    slice of a larger tensor as long as each stream's [D, N] is dense; it is h itself or shares no memory with an input). `active` [B] (bool): a stream marked false gives
     y = 0 and keeps its state. No gradients (a decoding form)."""
     B, Dn, N = _check(u, dt, A, Bm, Cm, D, dt_bias, 2)
     A_.check_like(h, u, (B, Dn, N), "h", _state_type(u))
