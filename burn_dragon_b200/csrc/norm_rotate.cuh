@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_
   for (; first < a.tokens; first += stride) {
     const Token next = token_at(a, first + stride + me.ts);
     const Rows<T, P> next_rows(a, me, next.b, next.t);
+    const float eps = now.in ? d.eps : 1.f;                     // (behind a length the row is 0, and d.eps may be)
     float2 e[NV][N];                                            // (0, 0) for a token behind its length: its rows become 0
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_
         for (int i = 0; i < N; ++i) ss = fma2(x[n][i], x[n][i], ss);
       }
       load(next, next_rows, u);
-      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, d.eps));
+      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
       if (!now.live || !me.has(a, u)) continue;
       const bool key = me.key(a, u);
       T* o = static_cast<T*>(key ? d.k_out : d.q_out) + rows.dense(a, me, u);
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? BWD_BLOCKS : 2) norm_rotate_bwd_
   for (; first < a.tokens; first += stride) {
     const Token next = token_at(a, first + stride + me.ts);
     const Rows<T, P> next_at(a, me, next.b, next.t);
+    const float eps = now.in ? d.eps : 1.f;
     float2 e[NV][N];
     float cross[NV][N];
 #pragma unroll
@@ -367,7 +369,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? BWD_BLOCKS : 2) norm_rotate_bwd_
         }
       }
       load(next, next_at, u);
-      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, d.eps));
+      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
       const float m = group_sum(sum2(dot), a.G) * a.per_column * rs * rs;            // mean(w dv x r) r, per element of x
       if (!now.live || !me.has(a, u)) continue;
       T* o = static_cast<T*>(key ? d.dk : d.dq) + at.dense(a, me, u);

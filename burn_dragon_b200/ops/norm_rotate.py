@@ -41,7 +41,7 @@ def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, 
         if x is None:
             outs.append(None)
             continue
-        xs = x.to(ct) if keep is None else torch.where(keep, x.to(ct), 0.0)
+        xs = x.to(ct) if keep is None else torch.where(keep, x.to(ct), 1.0)     # (1: a norm that exists without eps too)
         v = xs * torch.rsqrt(xs.square().mean(-1, keepdim=True) + eps)
         v = v * w.to(ct) if w is not None else v
         v = v + b.to(ct) if b is not None else v

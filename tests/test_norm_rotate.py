@@ -263,3 +263,27 @@ def test_two_runs_give_the_same_bits_and_replay_from_a_graph():
     with torch.no_grad():
         a2, b2 = NR.norm_rotate(*tensors, lengths=n, **how)
     assert torch.equal(a, a2) and torch.equal(b, b2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_behind_a_length_without_eps(device):
+    """eps = 0: the norm of a row behind a length, which reads as 0, must not reach a result (0 / 0 there). Against the
+    sequences by themselves in float64. A term is off by about (16 + 8) u, a sum of 14 of them by 14 u more, together 3e-6 of
+    the terms' magnitudes, and these are at most 14 times the largest: 1e-4 of the largest result holds them."""
+    g = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(*s, generator=g).to(device)                                               # noqa: E731
+    q, w, b, an, dy = r(2, 5, 2, 16), r(16), r(16), r(2, 5, 8), r(2, 5, 2, 16)
+    n = torch.tensor([5, 2], device=device)
+    leaves = [t.clone().requires_grad_() for t in (q, w, b, an)]
+    out, _ = NR.norm_rotate(leaves[0], None, leaves[1], None, leaves[2], angles=leaves[3], lengths=n, eps=0.0)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, dy)]
+    exact = [t.double().requires_grad_() for t in (q, w, b, an)]
+    want = []
+    for i, m in enumerate((5, 2)):
+        o, _ = NR.norm_rotate(exact[0][i:i + 1, :m], None, exact[1], None, exact[2], angles=exact[3][i:i + 1, :m], eps=0.0)
+        want.append(torch.cat((o, o.new_zeros(1, 5 - m, 2, 16)), 1))
+    want = torch.cat(want)
+    want = [want.detach(), *torch.autograd.grad(want, exact, dy.double())]
+    for a, e in zip(got, want):
+        assert (a.double() - e).abs().max() <= 1e-4 * e.abs().max()
+    assert (got[0][1, 2:] == 0).all() and (got[1][1, 2:] == 0).all()
