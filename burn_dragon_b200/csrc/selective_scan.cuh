@@ -24,7 +24,7 @@
 // Exponentials are the hardware's (2 units in the last place): exact ones would halve the error of the gradient of A
 // (1.8e-6 of its norm over 2048 steps) and take a third more time.
 //
-// Measured (bf16 rows, 16 states): a prompt of 8192 x 4096 361 us, of 6 x 777 x 1000 with 64 states (fp16) 107 us; forward
+// Measured (bf16 rows, 16 states): a prompt of 8192 x 4096 361 us, of 6 x 777 x 1000 with 64 states (fp16, lengths drawn) 107 to 134 us; forward
 // 4 x 2048 x 2048 160 us, backward 450 us. At full occupancy a pass runs at 0.7 of the exponentials' rate; the backward
 // kernel issues ~190 instructions for 8 states of a lane and step, at two warps a scheduler.
 #pragma once
