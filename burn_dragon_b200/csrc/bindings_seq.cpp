@@ -89,6 +89,12 @@ void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs)
                 end(out) <= static_cast<const char*>(t->const_data_ptr()), "out overlaps an input other than the state");
 }
 
+// What a kernel wrote through a pointer counts as a change of the tensor for autograd too: a backward pass that kept `out`
+// as a sequence's state refuses it. (The alias mark of the schema alone does not count.)
+void changed(const OptTensor& out) {
+  if (given(out)) torch::autograd::impl::bump_version(*out);
+}
+
 Tensor new_f32(const Tensor& on, at::IntArrayRef sizes) { return at::empty(sizes, on.options().dtype(at::kFloat)); }
 Tensor new_rows(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options()); }
 
@@ -252,6 +258,7 @@ std::vector<Tensor> causal_conv_step(const Tensor& x, const Tensor& state, const
   if (given(out)) check_apart(*out, {&x, &w});
   set_state_out(d, x, given(out) ? *out : result.emplace_back(new_rows(x, state.sizes())));
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
+  changed(out);
   return result;
 }
 
@@ -537,6 +544,7 @@ std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const
   }
   check_rc(bdh_selective_scan_step(&d, h.const_data_ptr<float>(), h.stride(0), to.data_ptr<float>(), to.stride(0),
                                    active_ptr(active, u, d.B), cur_stream()), "selective_scan_step");
+  changed(out);
   return result;
 }
 

@@ -1,0 +1,77 @@
+"""Calls of the state-space operators (`ops.mamba_ops.causal_conv`, `ops.norm_rotate`, `ops.selective_scan`) that are allowed but
+unusual: states updated in place between a forward and its backward pass, other kinds of derivatives, infinities, growing
+states, inputs that share a buffer. u = 2^-24 is half a unit in the last place of fp32."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from burn_dragon_b200.ops import mamba_ops as MO
+from burn_dragon_b200.ops import norm_rotate as NR
+from burn_dragon_b200.ops import selective_scan as S
+
+U = 2.0 ** -24
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+NAMES = ["conv", "norm_rotate", "scan"]
+
+
+def rand(device, seed):
+    g = torch.Generator().manual_seed(seed)
+    return lambda *s: torch.randn(*s, generator=g).to(device)
+
+
+def calls(device):
+    """{operator: (call of its tensors, those tensors)}; every tensor has a gradient."""
+    r = rand(device, 9)
+    B, T, D, N = 2, 9, 8, 4
+    return {
+        "conv": (lambda x, w, b, st: MO.causal_conv(x, w, b, state=st), [r(B, T, D), r(D, 4), r(D), r(B, 3, D)]),
+        "norm_rotate": (lambda q, k, qw, kw, qb, kb, an: NR.norm_rotate(q, k, qw, kw, qb, kb, angles=an),
+                        [r(B, T, 3, D), r(B, T, 2, D), r(D), r(D), r(D), r(D), r(B, T, 3)]),
+        "scan": (lambda u, dt, A, Bm, Cm, Dk, db, h0: S.selective_scan(u, dt, A, Bm, Cm, Dk, dt_bias=db, dt_softplus=True, h0=h0),
+                 [r(B, T, D), r(B, T, D), -r(D, N).abs(), r(B, T, N), r(B, T, N), r(D), r(D), r(B, D, N)]),
+    }
+
+
+def step_calls(device):
+    """The same of the single-token forms, which take `out`."""
+    r = rand(device, 10)
+    B, D, N = 2, 8, 4
+    return {
+        "conv": (lambda x, st, w, b, out=None: MO.causal_conv_step(x, st, w, b, out=out), [r(B, D), r(B, 3, D), r(D, 4), r(D)], 1),
+        "scan": (lambda u, dt, A, Bm, Cm, h, Dk, db, out=None: S.selective_scan_step(u, dt, A, Bm, Cm, h, Dk, dt_bias=db, dt_softplus=True, out=out),
+                 [r(B, D), r(B, D), -r(D, N).abs(), r(B, N), r(B, N), r(B, D, N), r(D), r(D)], 5),
+    }
+
+
+@pytest.mark.parametrize("name", ["conv", "scan"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_in_place_counts_as_a_change_of_its_state(device, name):
+    fn, tensors, state = step_calls(device)[name]
+    out = torch.empty_like(tensors[state])
+    before, kept = out._version, tensors[state]._version
+    fn(*tensors, out=out)
+    assert out._version > before and tensors[state]._version == kept
+    before = tensors[state]._version
+    fn(*tensors, out=tensors[state])
+    assert tensors[state]._version > before
+    with torch.inference_mode():                                             # (tensors made there count no changes)
+        inner = tensors[state].clone()
+        fn(*tensors, out=inner)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["conv", "scan"])
+def test_a_backward_pass_refuses_a_state_that_changed_since(name):
+    fn, tensors = calls("cuda")[name]
+    step, row, at = step_calls("cuda")[name]
+    leaves = [t.clone().requires_grad_() for t in tensors[:-1]]
+    state = tensors[-1].clone()
+    y, _ = fn(*leaves, state)
+    step(*row[:at], state, *row[at + 1:], out=torch.empty_like(state))       # the state itself stays: no objection
+    want = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+    step(*row[:at], state, *row[at + 1:], out=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), leaves)
+    y, _ = fn(*leaves, tensors[-1])
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y.sum(), leaves)))
