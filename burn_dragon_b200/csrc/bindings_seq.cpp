@@ -118,6 +118,16 @@ bool records(std::initializer_list<const Tensor*> tensors, std::initializer_list
   return false;
 }
 
+// There is no forward mode: a tangent would be lost without a word, since the kernels see values only.
+void no_tangents(std::initializer_list<const Tensor*> tensors, std::initializer_list<const OptTensor*> others, const char* name) {
+  const auto check = [&](const Tensor& t) {
+    TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative, and an input carries a tangent");
+  };
+  for (const Tensor* t : tensors) check(*t);
+  for (const OptTensor* t : others)
+    if (given(*t)) check(**t);
+}
+
 // Gradients are not differentiable again: a second derivative that reaches them ends in an error.
 variable_list first_derivative(variable_list grads, const variable_list& incoming, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -243,6 +253,7 @@ struct CausalConv : Function<CausalConv> {
 
 std::vector<Tensor> causal_conv(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& state, const OptTensor& lengths,
                                 bool silu) {
+  no_tangents({&x, &w}, {&bias, &state}, "causal_conv");
   if (!records({&x, &w}, {&bias, &state})) return causal_conv_fwd(x, w, bias, state, lengths, silu);
   return CausalConv::apply(x, w, bias, state, lengths, silu);
 }
@@ -252,6 +263,7 @@ std::vector<Tensor> causal_conv_step(const Tensor& x, const Tensor& state, const
                                      bool silu, const OptTensor& out) {
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x: [B, C], w: [C, k]");
+  no_tangents({&x, &state, &w}, {&bias, &out}, "causal_conv_step");
   BdhConvDesc d = conv_desc(x, w, bias, state, c10::nullopt, silu);
   std::vector<Tensor> result{new_rows(x, x.sizes())};
   d.y = result[0].data_ptr();
@@ -407,6 +419,7 @@ struct NormRotate : Function<NormRotate> {
 std::vector<Tensor> norm_rotate(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                 const OptTensor& q_bias, const OptTensor& k_bias, const OptTensor& angles, const OptTensor& freqs,
                                 const OptTensor& positions, int64_t pos0, const OptTensor& lengths, double eps) {
+  no_tangents({&q}, {&k, &q_weight, &k_weight, &q_bias, &k_bias, &angles, &freqs}, "norm_rotate");
   if (!records({&q}, {&k, &q_weight, &k_weight, &q_bias, &k_bias, &angles}))
     return norm_rotate_fwd(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
   return NormRotate::apply(q, k, q_weight, k_weight, q_bias, k_bias, angles, freqs, positions, pos0, lengths, eps);
@@ -522,6 +535,7 @@ struct SelectiveScan : Function<SelectiveScan> {
 std::vector<Tensor> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
                                    const OptTensor& skip, const OptTensor& dt_bias, bool softplus, const OptTensor& h0,
                                    const OptTensor& lengths) {
+  no_tangents({&u, &dt, &A, &Bm, &Cm}, {&skip, &dt_bias, &h0}, "selective_scan");
   if (!records({&u, &dt, &A, &Bm, &Cm}, {&skip, &dt_bias, &h0}))
     return selective_scan_fwd(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths, false);
   return SelectiveScan::apply(u, dt, A, Bm, Cm, skip, dt_bias, softplus, h0, lengths);
@@ -533,6 +547,7 @@ std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const
                                         const OptTensor& out) {
   c10::cuda::CUDAGuard guard(u.device());
   TORCH_CHECK(u.dim() == 2 && dt.dim() == 2 && Bm.dim() == 2 && Cm.dim() == 2, "u, dt: [B, D], B, C: [B, N]");
+  no_tangents({&u, &dt, &A, &Bm, &Cm, &h}, {&skip, &dt_bias, &out}, "selective_scan_step");
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, c10::nullopt, c10::nullopt);
   std::vector<Tensor> result{new_rows(u, u.sizes())};
   d.y = result[0].data_ptr();

@@ -102,7 +102,8 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     passed as `state` with the sequence's next rows (None: zeros). Rows are fp32, fp16 or bf16 (y and the states are of
     their type), sums fp32; x and the state may be views whose channels are adjacent. `lengths` [B]: the rows of each sequence that
     count; y is 0 behind them, the state ends there, and whatever x holds there is not read. Differentiable in x, w,
-    bias and both states, once (no second derivative); the sums over rows are made in a fixed order."""
+    bias and both states, once (the kernels refuse second derivatives and forward-mode tangents); the sums over rows are made
+    in a fixed order."""
     silu = _check_conv(x, w, bias, activation, 3)
     B, T, C = x.shape
     A.check_like(state, x, (B, w.shape[1] - 1, C), "state", x.dtype)

@@ -75,3 +75,43 @@ def test_a_backward_pass_refuses_a_state_that_changed_since(name):
         torch.autograd.grad(y.sum(), leaves)
     y, _ = fn(*leaves, tensors[-1])
     assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y.sum(), leaves)))
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_tangents_are_carried_or_refused(device, name):
+    """The torch statements carry a tangent; the kernels have no forward mode and say so, with and without a gradient."""
+    fn, tensors = calls(device)[name]
+    for i, t in enumerate(tensors):
+        for grad in (False, True):
+            with fwAD.dual_level():
+                leaf = t.clone().requires_grad_(grad)
+                args = [fwAD.make_dual(leaf, torch.ones_like(t)) if j == i else v for j, v in enumerate(tensors)]
+                if device == "cuda":
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        fn(*args)
+                else:
+                    assert any(fwAD.unpack_dual(o).tangent is not None for o in fn(*args))
+    if device == "cuda":
+        fn(*tensors)
+
+
+@pytest.mark.parametrize("name", ["conv", "scan"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_tangents_of_single_tokens(device, name):
+    fn, tensors, _ = step_calls(device)[name]
+    for i, t in enumerate(tensors):
+        with fwAD.dual_level():
+            args = [fwAD.make_dual(v, torch.ones_like(v)) if j == i else v for j, v in enumerate(tensors)]
+            if device == "cuda":
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*args)
+            else:
+                assert any(fwAD.unpack_dual(o).tangent is not None for o in fn(*args))
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_of_frequencies():
+    q, f = torch.randn(1, 2, 1, 8, device="cuda"), torch.rand(8, device="cuda")
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        NR.norm_rotate(q, freqs=fwAD.make_dual(f, torch.ones_like(f)))
