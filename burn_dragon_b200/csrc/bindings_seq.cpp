@@ -7,7 +7,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <initializer_list>
@@ -128,20 +128,26 @@ void no_tangents(std::initializer_list<const Tensor*> tensors, std::initializer_
     if (given(*t)) check(**t);
 }
 
-// Gradients are not differentiable again: a second derivative that reaches them ends in an error.
-variable_list first_derivative(variable_list grads, const variable_list& incoming, const char* name) {
+// Gradients are not differentiable again: a second derivative that reaches them ends in an error. A backward pass under
+// grad mode (create_graph) gives them this node, whose edges are those of everything they depend on - the incoming gradients
+// and the inputs, constant as the seed may be - so that no way from a later loss to an input goes around it.
+struct NoSecondDerivative : torch::autograd::Node {
+  std::string operator_name;
+  variable_list apply(variable_list&&) override { TORCH_CHECK(false, operator_name, " has no second derivative"); }
+};
+
+variable_list first_derivative(variable_list grads, variable_list incoming, AutogradContext* ctx, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
-  bool recorded = false;
-  for (const Tensor& t : incoming) recorded = recorded || wants(t);
-  if (!recorded) return grads;
-  variable_list in;
-  for (const Tensor& t : grads)
-    if (t.defined()) in.push_back(t.detach().requires_grad_(true));
-  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", static_cast<int64_t>(in.size()));
-  const variable_list out = (*error)(variable_list(in));
-  size_t i = 0;
+  const variable_list inputs = ctx->get_saved_variables();
+  incoming.insert(incoming.end(), inputs.begin(), inputs.end());
+  const std::shared_ptr<NoSecondDerivative> node(new NoSecondDerivative, torch::autograd::deleteNode);
+  node->operator_name = name;
+  node->set_next_edges(torch::autograd::collect_next_edges(incoming));
   for (Tensor& t : grads)
-    if (t.defined()) t = out[i++];
+    if (t.defined()) {
+      t = t.detach();
+      torch::autograd::set_history(t, node);
+    }
   return grads;
 }
 
@@ -247,7 +253,7 @@ struct CausalConv : Function<CausalConv> {
           if (want >> (i - 1) & 1) out[i] = made[at++];
       }
     }
-    return first_derivative(std::move(out), grads, "causal_conv");
+    return first_derivative(std::move(out), std::move(grads), ctx, "causal_conv");
   }
 };
 
@@ -412,7 +418,7 @@ struct NormRotate : Function<NormRotate> {
           if (i == 0 || (i == 1 && in[1].defined()) || (i > 1 && (want >> (i - 2) & 1))) out[i] = made[at++];
       }
     }
-    return first_derivative(std::move(out), grads, "norm_rotate");
+    return first_derivative(std::move(out), std::move(grads), ctx, "norm_rotate");
   }
 };
 
@@ -528,7 +534,7 @@ struct SelectiveScan : Function<SelectiveScan> {
         if (in[i].defined()) out[i] = made[at++];
       if (want_h0) out[8] = made[at];
     }
-    return first_derivative(std::move(out), grads, "selective_scan");
+    return first_derivative(std::move(out), std::move(grads), ctx, "selective_scan");
   }
 };
 

@@ -115,3 +115,30 @@ def test_forward_mode_tangents_of_frequencies():
     q, f = torch.randn(1, 2, 1, 8, device="cuda"), torch.rand(8, device="cuda")
     with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         NR.norm_rotate(q, freqs=fwAD.make_dual(f, torch.ones_like(f)))
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_gradient_penalty_is_not_dropped(device, name):
+    """The seed of the first derivative is a constant, the gradient depends on the inputs all the same: the torch statements
+    differentiate it, the kernels refuse. Every input in turn, by backward() and by grad()."""
+    fn, tensors = calls(device)[name]
+    for i in range(len(tensors)):
+        leaves = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(tensors)]
+        for whole in (True, False):
+            outs = fn(*leaves)
+            used = [o for o in outs if o.requires_grad]
+            first, = torch.autograd.grad(sum(o.sum() for o in used), leaves[i], create_graph=True)
+            loss = sum(o.square().sum() for o in used) + first.square().sum()
+            if device == "cuda":
+                with pytest.raises(RuntimeError, match="no second derivative"):
+                    loss.backward() if whole else torch.autograd.grad(loss, leaves[i])
+            elif whole:
+                loss.backward()
+            else:
+                torch.autograd.grad(loss, leaves[i])
+    if device == "cuda":                              # asked for once, a gradient is what it was
+        leaves = [t.clone().requires_grad_() for t in tensors]
+        out = fn(*leaves)[0]
+        once = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(once, torch.autograd.grad(out.sum(), leaves, create_graph=True)))
