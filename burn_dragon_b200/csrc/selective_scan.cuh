@@ -651,6 +651,7 @@ struct BwdMem {
     __device__ __forceinline__ RowsOf<T, NP> bc() const { return {B, C}; }
   } warp[BWD_WARPS];
   alignas(16) float bc[BWD_WARPS][LT][2 * NP];     // the warps' sums over their channels
+  alignas(16) float last[BWD_WARPS][NP];           // dC of a sequence's last row, where rows of its tile are behind it
 };
 
 // What a step of the reverse walk reads
@@ -710,6 +711,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
   for (int tile = last - 1; tile >= first; --tile) {
     const int t0 = tile * LT;
     const bool any = t0 < len;                         // (the same for the whole block)
+    const int rows = min(LT, len - t0);                // of the sequence
     Pack<T, S::V> u[S::NV], dt_raw[S::NV], dy[S::NV];
 #pragma unroll
     for (int i = 0; i < S::NV; ++i) {
@@ -748,6 +750,31 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
             h[k][1] = fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]);
           }
         now = next;
+      }
+      if (rows < LT) {
+        // Rows behind the sequence multiply the state, which may be infinite, by their zeros: they get a state of 0. The last
+        // row's dC, which the walk makes of the state behind it, is made here.
+        float gy[CT], cv[4];
+        sh.in.dys(rows - 1, cl, gy);
+        f2 sc0 = mul1(gy[0], h[0][0]), sc1 = mul1(gy[0], h[0][1]);
+#pragma unroll
+        for (int k = 1; k < CT; ++k) {
+          sc0 = fma1(gy[k], h[k][0], sc0);
+          sc1 = fma1(gy[k], h[k][1], sc1);
+        }
+        unpack2(sc0, cv[0], cv[1]);
+        unpack2(sc1, cv[2], cv[3]);
+        int at;
+        bool once;
+        sum_over<4, S::LANES, G>(cv, lane, at, once);
+        constexpr int CLEFT = 4 / S::LANES > 1 ? 4 / S::LANES : 1;
+        if (once)
+#pragma unroll
+          for (int i = 0; i < CLEFT; ++i) all.last[warp][n0 + at + i] = cv[i];
+#pragma unroll 1
+        for (int t = rows; t < LT; ++t)
+#pragma unroll
+          for (int k = 0; k < CT; ++k) sh.h[t][k][lane] = make_ulonglong2(0, 0);
       }
       BwdStep<T, G, CT> at_t, before;
       at_t.load(sh, LT - 1, lane, cl, n0);
@@ -796,6 +823,10 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
 #pragma unroll
           for (int i = 0; i < CLEFT; ++i) all.bc[warp][t][(at + i) / 4 * S::NP + n0 + (at + i) % 4] = cv[i];
         at_t = before;
+      }
+      if (rows < LT) {
+        __syncwarp();
+        for (int i = lane; i < S::NP; i += 32) all.bc[warp][rows - 1][S::NP + i] = all.last[warp][i];
       }
 #pragma unroll
       for (int k = 0; k < CT; ++k) {                   // sums of tiles: a chain of 16, then one of the tiles
@@ -850,7 +881,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
       const int t = i / (S::NP / 2), n = i % (S::NP / 2) * 4;
       if (t0 + t >= d.T) break;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (any)
+      if (t < rows)
 #pragma unroll
         for (int k = 0; k < BWD_WARPS; ++k) {
           const float4 q = *reinterpret_cast<const float4*>(&all.bc[k][t][n]);

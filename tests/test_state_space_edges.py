@@ -142,3 +142,53 @@ def test_a_gradient_penalty_is_not_dropped(device, name):
         out = fn(*leaves)[0]
         once = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
         assert all(torch.equal(a, b) for a, b in zip(once, torch.autograd.grad(out.sum(), leaves, create_graph=True)))
+
+
+INF_STATES = [16, 64]
+
+
+@pytest.mark.parametrize("N", INF_STATES)
+@pytest.mark.parametrize("T,D,ragged", [(20, 16, False), (300, 24, False), (20, 17, False), (37, 16, True)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_infinite_input_reaches_its_own_results_only(device, N, T, D, ragged):
+    """An infinite dt' u makes its own states infinite, and what is made of them: not the sums over the rows behind a
+    sequence, where the state stays and everything is 0. B, C, dy > 0, so no infinity meets another; which results are
+    infinite or NaN is the float64 statement's. A finite one is a sum of at most 64 T terms, each off by (24 + (24 + T) 2) u per
+    step back, of which at most 50 matter (dt' A < -0.1: exp(-5) is left), and the sum by 64 T u more: 50 (24 + 648) u +
+    19200 u = 3.2e-3 of the largest of its kind for T = 300."""
+    g = torch.Generator().manual_seed(N + T)
+    r = lambda *s: (torch.rand(*s, generator=g) + 0.1).to(device)                                        # noqa: E731
+    p = dict(u=r(2, T, D), dt=r(2, T, D), A=-r(D, N) - 0.9, B=r(2, T, N), C=r(2, T, N), D=r(D), dt_bias=r(D), h0=r(2, D, N))
+    p["u"][0, T // 2, 3] = float("inf")
+    p["u"][1, 5, D - 1] = float("-inf")
+    dy, dh = r(2, T, D), r(2, D, N)
+    n = torch.tensor([T, 11], device=device) if ragged else None
+
+    def both(q, dy, dh, fn):
+        leaves = {k: t.detach().requires_grad_() for k, t in q.items()}
+        y, h = fn(leaves["u"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"], leaves["D"], dt_bias=leaves["dt_bias"], h0=leaves["h0"], lengths=n)
+        return dict(y=y.detach(), h=h.detach(), **dict(zip(("d_" + k for k in leaves), torch.autograd.grad([y, h], list(leaves.values()), [dy, dh]))))
+
+    got = both(p, dy, dh, S.selective_scan)
+    want = both({k: t.double() for k, t in p.items()}, dy.double(), dh.double(), S.selective_scan_reference)
+    if ragged:                                        # (the statement's own derivatives have 0 * inf at the rows behind a length)
+        cut = {k: t[1:, :11] if k in ("u", "dt", "B", "C") else t[1:] if k == "h0" else t for k, t in p.items()}
+        n = None
+        one = both({k: t.double() for k, t in cut.items()}, dy[1:, :11].double(), dh[1:].double(), S.selective_scan_reference)
+        first = {k: t[:1] if k in ("u", "dt", "B", "C", "h0") else t for k, t in p.items()}
+        two = both({k: t.double() for k, t in first.items()}, dy[:1].double(), dh[:1].double(), S.selective_scan_reference)
+        for k in want:
+            if k in ("d_A", "d_D", "d_dt_bias"):
+                want[k] = two[k] + one[k]
+            elif k in ("h", "d_h0"):
+                want[k] = torch.cat((two[k], one[k]))
+            else:
+                want[k] = torch.cat((two[k], torch.nn.functional.pad(one[k], (0, 0, 0, T - 11))))
+    for k in got:
+        if device == "cpu" and ragged and k not in ("y", "h"):
+            continue
+        a, e = got[k].double(), want[k]
+        fine = torch.isfinite(e)
+        assert torch.equal(torch.isfinite(a), fine) and torch.equal(torch.isnan(a), torch.isnan(e)), k
+        assert torch.equal(a[~fine].nan_to_num(), e[~fine].nan_to_num()), k
+        assert (a[fine] - e[fine]).abs().max() <= 3.2e-3 * e[fine].abs().max(), k
