@@ -283,7 +283,12 @@ struct alignas(16) WarpMem {
   float dy[DY ? LT : 1][CW + 4];
   float bias[CW], skip[CW];
 
+  static constexpr int ZEROS = CW;                     // the columns behind the channels, which stay 0
   __device__ __forceinline__ void params(const BdhScanDesc& d, int c0) {
+    if (const int t = threadIdx.x & 31; t < LT) {
+      step[t][CW] = step[t][CW + 1] = make_float2(0.f, 0.f);
+      if constexpr (DY) dy[t][CW] = dy[t][CW + 1] = 0.f;
+    }
     for (int i = threadIdx.x & 31; i < CW; i += 32) {
       bias[i] = (d.dt_bias && c0 + i < d.D) ? d.dt_bias[c0 + i] : 0.f;
       skip[i] = (d.skip && c0 + i < d.D) ? d.skip[c0 + i] : 0.f;
@@ -368,6 +373,22 @@ __device__ __forceinline__ void store_state(float* p, int c, int n0, const BdhSc
     if (c < d.D && n0 + j < d.N) p[static_cast<long long>(c) * d.N + n0 + j] = v[j];
 }
 
+// States that N is padded with have to stay 0 whatever their channel's step, which may be infinite, and 0 * inf is not 0.
+// Lanes of padding alone read the step (and dy) of a column of zeros behind the warp's channels; a lane that has both kinds
+// (N not a multiple of 4, so never in packs) clears the others' bits. Where the rows come in packs this costs nothing.
+struct Real {
+  f2 m[2];                             // all bits of this lane's states below N
+  __device__ __forceinline__ Real(int n0, int N) {
+    unsigned v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = n0 + j < N ? 0xffffffffu : 0u;
+    m[0] = static_cast<f2>(v[1]) << 32 | v[0];
+    m[1] = static_cast<f2>(v[3]) << 32 | v[2];
+  }
+  template <bool VEC>
+  __device__ __forceinline__ f2 keep(f2 x, int j) const { return VEC ? x : x & m[j]; }
+};
+
 // A2 = A log2(e); 0 for padding
 template <int CT>
 __device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (&A2)[CT][2]) {
@@ -383,6 +404,7 @@ __device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (
 // through those behind it.
 template <int CT, int NP>
 __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to, int by, int c, int n0, const f2 (&A2)[CT][2], f2 (&h)[CT][2]) {
+  const Real real(n0, a.d.N);
   for (int s = from; s != to; s += by) {
 #pragma unroll
     for (int k = 0; k < CT; ++k) {
@@ -391,8 +413,8 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
       const f2 dt = both(a.seg_dt[at]);
       f2 s0, s1;
       load4(a.seg_state + at * NP + n0, s0, s1);
-      h[k][0] = fma2(ex2x2(mul2(dt, A2[k][0])), h[k][0], s0);
-      h[k][1] = fma2(ex2x2(mul2(dt, A2[k][1])), h[k][1], s1);
+      h[k][0] = real.keep<false>(fma2(ex2x2(mul2(dt, A2[k][0])), h[k][0], s0), 0);
+      h[k][1] = real.keep<false>(fma2(ex2x2(mul2(dt, A2[k][1])), h[k][1], s1), 1);
     }
   }
 }
@@ -469,6 +491,8 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
   const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles), end = min(last, (len + LT - 1) / LT);
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) sh.ring.template load<true, true>(d, first + i, end, w.b, c0, len);
+  const Real real(n0, d.N);
+  const int cs = n0 < d.N ? cl : sh.in.ZEROS;          // where this lane reads its steps
   f2 A2[CT][2], h[CT][2];
   load_a<CT>(d, c, n0, A2);
 #pragma unroll
@@ -494,16 +518,16 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
                 make_ulonglong2(h[k][0], h[k][1]);
       using Group = Steps<G, CT, true>;
       Group now, next;
-      now.make(sh.in, bc, 0, cl, n0, A2);
+      now.make(sh.in, bc, 0, cs, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cs, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
-            h[k][0] = fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]);
-            h[k][1] = fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]);
+            h[k][0] = real.template keep<VEC>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
+            h[k][1] = real.template keep<VEC>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
             sh.part[s0 + s][k * 32 + lane] = sum2(fma2(now.k[s][1], h[k][1], mul2(now.k[s][0], h[k][0])));
           }
         now = next;
@@ -571,6 +595,8 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
   const auto tile_of = [&](int i) { return REV ? end - 1 - i : first + i; };
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) sh.ring.template load<!REV, REV>(d, i < n ? tile_of(i) : -1, end, w.b, c0, len);
+  const Real real(n0, d.N);
+  const int cs = n0 < d.N ? cl : sh.in.ZEROS;
   f2 A2[CT][2], h[CT][2];
   float total[CT];
   load_a<CT>(d, c, n0, A2);
@@ -597,10 +623,10 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
         const int t = REV ? LT - 1 - s0 - s : s0 + s;
         float dt[CT], du[CT];
         f2 b[2];
-        sh.in.steps(t, cl, dt, du);
+        sh.in.steps(t, cs, dt, du);
         if constexpr (REV) {
           bc.C(t, n0, b);
-          sh.in.dys(t, cl, du);
+          sh.in.dys(t, cs, du);
         } else {
           bc.B(t, n0, b);
         }
@@ -619,7 +645,8 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
         for (int k = 0; k < CT; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            h[k][j] = REV ? mul2(e[s][k][j], add2(h[k][j], in[s][k][j])) : fma2(e[s][k][j], h[k][j], in[s][k][j]);
+            h[k][j] = real.template keep<VEC>(
+                REV ? mul2(e[s][k][j], add2(h[k][j], in[s][k][j])) : fma2(e[s][k][j], h[k][j], in[s][k][j]), j);
     }
     __syncwarp();
   }
@@ -681,6 +708,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
   const Where w = where(a, blockIdx.x);
   const int n0 = lane % G * 4, cl = lane / G * CT, c0 = (w.part * BWD_WARPS + warp) * S::CW, c = c0 + cl;
   const int len = a.len.get(w.b, d.T);
+  const Real real(n0, d.N);
+  const int cs = n0 < d.N ? cl : sh.in.ZEROS;
   f2 A2[CT][2], r[CT][2], da[CT][2];
   load_a<CT>(d, c, n0, A2);
 #pragma unroll
@@ -737,17 +766,17 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
       using Group = Steps<G, CT, false>;
       const RowsOf<T, S::NP> bc = sh.bc();
       Group now, next;
-      now.make(sh.in, bc, 0, cl, n0, A2);
+      now.make(sh.in, bc, 0, cs, n0, A2);
 #pragma unroll
       for (int s0 = 0; s0 < LT; s0 += Group::N) {
-        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cl, n0, A2);
+        if (s0 + Group::N < LT) next.make(sh.in, bc, s0 + Group::N, cs, n0, A2);
 #pragma unroll
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
             sh.h[s0 + s][k][lane] = make_ulonglong2(h[k][0], h[k][1]);
-            h[k][0] = fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]);
-            h[k][1] = fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]);
+            h[k][0] = real.template keep<VEC>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
+            h[k][1] = real.template keep<VEC>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
           }
         now = next;
       }
@@ -755,7 +784,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
         // Rows behind the sequence multiply the state, which may be infinite, by their zeros: they get a state of 0. The last
         // row's dC, which the walk makes of the state behind it, is made here.
         float gy[CT], cv[4];
-        sh.in.dys(rows - 1, cl, gy);
+        sh.in.dys(rows - 1, cs, gy);
         f2 sc0 = mul1(gy[0], h[0][0]), sc1 = mul1(gy[0], h[0][1]);
 #pragma unroll
         for (int k = 1; k < CT; ++k) {
@@ -777,16 +806,16 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           for (int k = 0; k < CT; ++k) sh.h[t][k][lane] = make_ulonglong2(0, 0);
       }
       BwdStep<T, G, CT> at_t, before;
-      at_t.load(sh, LT - 1, lane, cl, n0);
+      at_t.load(sh, LT - 1, lane, cs, n0);
 #pragma unroll 4
       for (int t = LT - 1; t >= 0; --t) {
-        before.load(sh, t > 0 ? t - 1 : 0, lane, cl, n0);              // ahead of this step's stores
+        before.load(sh, t > 0 ? t - 1 : 0, lane, cs, n0);              // ahead of this step's stores
         f2 sb0, sb1, sc0, sc1;
         float nv[2 * CT];
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
           const float dt = at_t.dt[k], du = at_t.du[k], gy = at_t.gy[k];
-          const f2 g0 = fma1(gy, at_t.c[0], r[k][0]), g1 = fma1(gy, at_t.c[1], r[k][1]);
+          const f2 g0 = real.template keep<VEC>(fma1(gy, at_t.c[0], r[k][0]), 0), g1 = real.template keep<VEC>(fma1(gy, at_t.c[1], r[k][1]), 1);
           const f2 e0 = ex2x2(mul1(dt, A2[k][0])), e1 = ex2x2(mul1(dt, A2[k][1]));
           if (k == 0) {
             sb0 = mul1(du, g0); sb1 = mul1(du, g1);
@@ -795,8 +824,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
             sb0 = fma1(du, g0, sb0); sb1 = fma1(du, g1, sb1);
             sc0 = fma1(gy, h[k][0], sc0); sc1 = fma1(gy, h[k][1], sc1);
           }
-          r[k][0] = mul2(e0, g0);
-          r[k][1] = mul2(e1, g1);
+          r[k][0] = real.template keep<VEC>(mul2(e0, g0), 0);
+          r[k][1] = real.template keep<VEC>(mul2(e1, g1), 1);
           h[k][0] = at_t.h[k].x;
           h[k][1] = at_t.h[k].y;
           const f2 q0 = mul2(r[k][0], h[k][0]), q1 = mul2(r[k][1], h[k][1]);

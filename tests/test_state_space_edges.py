@@ -144,7 +144,7 @@ def test_a_gradient_penalty_is_not_dropped(device, name):
         assert all(torch.equal(a, b) for a, b in zip(once, torch.autograd.grad(out.sum(), leaves, create_graph=True)))
 
 
-INF_STATES = [16, 64]
+INF_STATES = [3, 5, 12, 16, 20, 33, 64]
 
 
 @pytest.mark.parametrize("N", INF_STATES)
@@ -192,3 +192,19 @@ def test_an_infinite_input_reaches_its_own_results_only(device, N, T, D, ragged)
         assert torch.equal(torch.isfinite(a), fine) and torch.equal(torch.isnan(a), torch.isnan(e)), k
         assert torch.equal(a[~fine].nan_to_num(), e[~fine].nan_to_num()), k
         assert (a[fine] - e[fine]).abs().max() <= 3.2e-3 * e[fine].abs().max(), k
+
+
+@pytest.mark.parametrize("N", [5, 12, 16])
+@pytest.mark.parametrize("T", [20, 300])
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_infinite_step_forgets_the_past(device, N, T):
+    """dt' = inf: the decays are exp(-inf) = 0 and the states infinite; the other channels do not notice."""
+    g = torch.Generator().manual_seed(N)
+    r = lambda *s: (torch.rand(*s, generator=g) + 0.1).to(device)                                        # noqa: E731
+    u, dt, A, Bm, Cm = r(1, T, 16), r(1, T, 16), -r(16, N) - 0.9, r(1, T, N), r(1, T, N)
+    clean, _ = S.selective_scan(u, dt, A, Bm, Cm)
+    dt[0, T // 2, 3] = float("inf")
+    y, h = S.selective_scan(u, dt, A, Bm, Cm)
+    assert torch.isinf(y[0, T // 2:, 3]).all() and torch.isinf(h[0, 3]).all()
+    y[0, T // 2:, 3] = clean[0, T // 2:, 3]
+    assert torch.equal(y, clean)
