@@ -472,6 +472,7 @@ __device__ __forceinline__ Where where(const ScanArgs& a, long long unit) {
 template <typename T, int G, int CT, bool VEC>
 struct FwdMem {
   WarpMem<G, CT, false> in;
+  alignas(16) T zeros[Shape<T, G, CT>::E];             // as wide as a lane's channels
   alignas(16) float part[LT][CT * 32 + 4];
   Ring<T, G, CT, VEC, false> ring;
 };
@@ -500,6 +501,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
     load_state(d.h0 ? d.h0 + static_cast<long long>(w.b) * d.D * d.N : nullptr, c + k, n0, d, h[k]);
   carry<CT, S::NP>(a, w.b, 0, w.seg, 1, c, n0, A2, h);
   sh.in.params(d, c0);
+  for (int i = lane; i < S::E; i += 32) sh.zeros[i] = elem_from_float<T>(0.f);
   __syncwarp();
   const int row = lane / 2, col = (lane & 1) * S::E;
   for (int tile = first; tile < last; ++tile) {
@@ -537,9 +539,11 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
     if (t0 + row < d.T) {
       T* y = static_cast<T*>(d.y) + (static_cast<long long>(w.b) * d.T + t0 + row) * d.D;
       const bool in = t0 + row < len;
+      const T* skip_u = d.skip != nullptr ? sh.ring.at(tile).s.u + lane * S::E : sh.zeros;
 #pragma unroll
       for (int i = 0; i < S::NV; ++i) {
-        Pack<T, S::V> o, u = sh.ring.at(tile).u(i);
+        Pack<T, S::V> o, u;                            // (without a skip u is 0 here: 0 times an infinite u is not)
+        u.load(skip_u + i * S::V);
 #pragma unroll
         for (int j = 0; j < S::V; ++j) {
           const int cc = col + i * S::V + j;
@@ -883,7 +887,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           dd[j] = 0.f;
           if (in) {
             const float2 s = sh.out[row][cc];
-            du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
+            du = sh.in.step[row][cc].x * s.x;
+            if (d.skip != nullptr) du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
             dd[j] = fmaf(u[i][j], s.x, LN2 * s.y);
             sum_skip[i * S::V + j] = fmaf(dy[i][j], u[i][j], sum_skip[i * S::V + j]);
           }
@@ -1034,7 +1039,7 @@ __global__ void __launch_bounds__(STEP_THREADS) selective_scan_step_kernel(const
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    y[r] = on ? fmaf(skip, u, sum) : 0.f;
+    y[r] = !on ? 0.f : d.skip ? fmaf(skip, u, sum) : sum;
     if (!live || b >= d.B) continue;
     float* p = out + b * out_sb + at;
     if (on || p != h + b * h_sb + at) {

@@ -208,3 +208,25 @@ def test_an_infinite_step_forgets_the_past(device, N, T):
     assert torch.isinf(y[0, T // 2:, 3]).all() and torch.isinf(h[0, 3]).all()
     y[0, T // 2:, 3] = clean[0, T // 2:, 3]
     assert torch.equal(y, clean)
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("device", DEVICES)
+def test_without_a_skip_an_infinite_input_is_not_multiplied_by_zero(device, T):
+    g = torch.Generator().manual_seed(T)
+    r = lambda *s: (torch.rand(*s, generator=g) + 0.1).to(device)                                        # noqa: E731
+    u, dt, A, Bm, Cm, h0 = r(2, T, 24), r(2, T, 24), -r(24, 16) - 0.9, r(2, T, 16), r(2, T, 16), r(2, 24, 16)
+    u[1, T // 2, 5] = float("inf")
+    with torch.no_grad():
+        y, _ = S.selective_scan(u, dt, A, Bm, Cm, h0=h0)
+        assert torch.isinf(y[1, T // 2:, 5]).all() and torch.isfinite(y[0]).all()
+        if T == 1:
+            y, h = S.selective_scan_step(u[:, 0], dt[:, 0], A, Bm[:, 0], Cm[:, 0], h0)
+            assert torch.isinf(y[1, 5]) and torch.isinf(h[1, 5]).all() and torch.isfinite(y[0]).all()
+    u[1, T // 2, 5] = 1
+    leaf = u.clone().requires_grad_()
+    dy = r(2, T, 24)
+    dy[0, T // 2, 7] = float("inf")
+    y, _ = S.selective_scan(leaf, dt, A, Bm, Cm, h0=h0)
+    du, = torch.autograd.grad(y, leaf, dy)
+    assert torch.isinf(du[0, :T // 2 + 1, 7]).all() and torch.isfinite(du[1]).all() and torch.isfinite(du[0, T // 2 + 1:]).all()
