@@ -300,7 +300,7 @@ struct alignas(16) WarpMem {
   __device__ __forceinline__ void put(const BdhScanDesc& d, const Source& x, int t0, int len) {
     using S = Shape<T, G, CT>;
     const int lane = threadIdx.x & 31, t = lane / 2, c = (lane & 1) * S::E;
-    const float keep = t0 + t < len ? 1.f : 0.f;
+    const f2 keep = t0 + t < len ? ~f2{0} : f2{0};       // (bits, not a factor: the bias alone may be infinite)
     float dt[S::E + 1], uu[S::E + 1];
     dt[S::E] = uu[S::E] = 0.f;
 #pragma unroll
@@ -316,7 +316,7 @@ struct alignas(16) WarpMem {
     for (int j = 0; j < S::E; j += 2) {
       f2 s = pack2(dt[j], dt[j + 1]);
       if (d.softplus) s = softplus2(s);
-      s = mul2(s, both(keep));
+      s &= keep;
       float s0, s1, v0, v1;
       unpack2(s, s0, s1);
       unpack2(mul2(s, pack2(uu[j], uu[j + 1])), v0, v1);

@@ -230,3 +230,18 @@ def test_without_a_skip_an_infinite_input_is_not_multiplied_by_zero(device, T):
     y, _ = S.selective_scan(leaf, dt, A, Bm, Cm, h0=h0)
     du, = torch.autograd.grad(y, leaf, dy)
     assert torch.isinf(du[0, :T // 2 + 1, 7]).all() and torch.isfinite(du[1]).all() and torch.isfinite(du[0, T // 2 + 1:]).all()
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_infinite_bias_does_not_reach_rows_behind_a_length(device, softplus):
+    r = rand(device, 3)
+    bias = torch.zeros(8, device=device)
+    bias[2] = float("inf")
+    h0 = r(2, 8, 4)
+    y, h = S.selective_scan(r(2, 30, 8).abs(), r(2, 30, 8).abs(), -r(8, 4).abs() - 0.1, r(2, 30, 4).abs() + 0.1, r(2, 30, 4).abs() + 0.1, dt_bias=bias,
+                            dt_softplus=softplus, h0=h0, lengths=torch.tensor([5, 30], device=device))
+    assert torch.isfinite(h[0, :2]).all() and torch.isinf(y[0, 0, 2]) and (y[0, 5:] == 0).all() and not torch.isfinite(y[1, :, 2]).any()
+    one, h1 = S.selective_scan(*(t[:, :1] for t in (r(1, 3, 8).abs(), r(1, 3, 8).abs())), -r(8, 4).abs() - 0.1, r(1, 1, 4).abs() + 0.1,
+                               r(1, 1, 4).abs() + 0.1, dt_bias=bias, dt_softplus=softplus)
+    assert torch.isinf(one[0, 0, 2]) and torch.isinf(h1[0, 2]).all() and torch.isfinite(h1[0, 3:]).all()
