@@ -400,6 +400,19 @@ __device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (
   }
 }
 
+// h exp(x), x in units of ln 2, for a whole segment's x: A and the steps may have any sign, so the factor alone may be past 2^128
+// where the product is not. It is applied in two halves, and a state of 0 (nothing came in yet) stays 0.
+__device__ __forceinline__ float grown(float h, float x) {
+  const float half = ex2(0.5f * x);
+  return h == 0.f ? 0.f : h * half * half;
+}
+__device__ __forceinline__ f2 grown2(f2 h, f2 x) {
+  float h0, h1, x0, x1;
+  unpack2(h, h0, h1);
+  unpack2(x, x0, x1);
+  return pack2(grown(h0, x0), grown(h1, x1));
+}
+
 // The state a segment starts from: `h` (the sequence's own) carried through the segments before it, in order; in reverse
 // through those behind it.
 template <int CT, int NP>
@@ -413,8 +426,8 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
       const f2 dt = both(a.seg_dt[at]);
       f2 s0, s1;
       load4(a.seg_state + at * NP + n0, s0, s1);
-      h[k][0] = real.keep<false>(fma2(ex2x2(mul2(dt, A2[k][0])), h[k][0], s0), 0);
-      h[k][1] = real.keep<false>(fma2(ex2x2(mul2(dt, A2[k][1])), h[k][1], s1), 1);
+      h[k][0] = real.keep<false>(add2(grown2(h[k][0], mul2(dt, A2[k][0])), s0), 0);
+      h[k][1] = real.keep<false>(add2(grown2(h[k][1], mul2(dt, A2[k][1])), s1), 1);
     }
   }
 }

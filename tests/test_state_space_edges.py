@@ -1,6 +1,7 @@
 """Calls of the state-space operators (`ops.mamba_ops.causal_conv`, `ops.norm_rotate`, `ops.selective_scan`) that are allowed but
 unusual: states updated in place between a forward and its backward pass, other kinds of derivatives, infinities, growing
 states, inputs that share a buffer. u = 2^-24 is half a unit in the last place of fp32."""
+import math
 
 import pytest
 import torch
@@ -245,3 +246,43 @@ def test_an_infinite_bias_does_not_reach_rows_behind_a_length(device, softplus):
     one, h1 = S.selective_scan(*(t[:, :1] for t in (r(1, 3, 8).abs(), r(1, 3, 8).abs())), -r(8, 4).abs() - 0.1, r(1, 1, 4).abs() + 0.1,
                                r(1, 1, 4).abs() + 0.1, dt_bias=bias, dt_softplus=softplus)
     assert torch.isinf(one[0, 0, 2]) and torch.isinf(h1[0, 2]).all() and torch.isfinite(h1[0, 3:]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_that_grow_while_they_are_zero(device):
+    """A > 0 and inputs that start late: the growth over what came before is past 2^128, of a state of zero. Then the gradients
+    where nothing of the outputs that are used reaches back over the growth. At most 20 steps of growth up to exp(3) hold
+    something: a result is off by 20 (24 + 44 * 3) u and 2^4 u for its sums, 2e-4 of the largest of its kind."""
+    T, D, N = 3000, 24, 16
+    r = rand(device, 12)
+    A = 0.4 + 0.1 * torch.rand(D, N, generator=torch.Generator().manual_seed(1)).to(device)
+    u, dt, Bm, Cm, dy = r(1, T, D), torch.full((1, T, D), 6.0, device=device), r(1, T, N), r(1, T, N), r(1, T, D)
+    u[:, :T - 10] = 0
+    y, h = S.selective_scan(u, dt, A, Bm, Cm)
+    y0, h0 = S.selective_scan_reference(*(t.double() for t in (u, dt, A, Bm, Cm)))
+    for a, e in ((y, y0), (h, h0)):
+        assert torch.isfinite(e).all() and (a.double() - e).abs().max() <= 2e-4 * e.abs().max()
+    dy[:, 10:] = 0
+    dt[:, :20], dt[:, T - 20:] = 0.01, 0.01
+    leaves = [t.clone().requires_grad_() for t in (u, dt, A, Bm, Cm)]
+    exact = [t.double().requires_grad_() for t in (u, dt, A, Bm, Cm)]
+    got = torch.autograd.grad(S.selective_scan(*leaves)[0], leaves, dy)
+    want = torch.autograd.grad(S.selective_scan_reference(*exact)[0], exact, dy.double())
+    for a, e in zip(got, want):
+        assert torch.isfinite(e).all() and (a.double() - e).abs().max() <= 2e-4 * e.abs().max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_small_state_that_grows_within_a_few_steps(device):
+    """h0 = 1e-30 and a growth of exp(115) = 9e49 in five steps: the result, 9e19, is a number of fp32, the growth is not. The
+    sum of the steps' x = 115 is off by (24 + 5) u |x| = 2e-4."""
+    T, D = 3000, 24
+    z = lambda *s: torch.zeros(*s, device=device)                                                        # noqa: E731
+    dt = z(1, T, D)
+    dt[:, 1008:1013] = 23
+    y, h = S.selective_scan(z(1, T, D), dt, torch.ones(D, 16, device=device), z(1, T, 16), z(1, T, 16), h0=torch.full((1, D, 16), 1e-30, device=device))
+    assert (torch.log(h.double()) - (115 + math.log(1e-30))).abs().max() <= 2e-4 and (y == 0).all()
+    dy, leaf = z(1, T, D), torch.full((1, D, 16), 1e-30, device=device).requires_grad_()
+    _, h = S.selective_scan(z(1, T, D), dt, torch.ones(D, 16, device=device), z(1, T, 16), z(1, T, 16), h0=leaf)
+    back, = torch.autograd.grad(h, leaf, torch.full_like(h, 1e-30))
+    assert (torch.log(back.double()) - (115 + math.log(1e-30))).abs().max() <= 2e-4
