@@ -91,8 +91,10 @@ def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None
     check_like(out, src, src.shape, name, src.dtype)
     if torch.is_grad_enabled() and out.requires_grad:
         raise ValueError(f"{name} requires a gradient; a step form has none")
-    strides = out.stride()
-    same = out.data_ptr() == src.data_ptr() and strides == src.stride()
+    sizes = out.shape
+    strides = [st if n > 1 else 0 for st, n in zip(out.stride(), sizes)]             # (a stride that is never taken means nothing)
+    from_strides = [st if n > 1 else 0 for st, n in zip(src.stride(), sizes)]
+    same = out.data_ptr() == src.data_ptr() and strides == from_strides
     dims = sorted((st, n) for st, n in zip(strides, out.shape) if n > 1)
     reach = 1                                            # elements that the dimensions of smaller stride span
     for st, n in dims:
@@ -101,7 +103,7 @@ def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None
         reach = st * (n - 1) + reach
     if same or not out.numel() or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr():
         return
-    if strides == src.stride():                          # slices of one buffer, which may interleave
+    if strides == from_strides:                          # slices of one buffer, which may interleave
         delta, odd = divmod(out.data_ptr() - src.data_ptr(), out.element_size())
         meet = odd or _meet(delta, dims[::-1])
     else:

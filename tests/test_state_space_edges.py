@@ -286,3 +286,15 @@ def test_a_small_state_that_grows_within_a_few_steps(device):
     _, h = S.selective_scan(z(1, T, D), dt, torch.ones(D, 16, device=device), z(1, T, 16), z(1, T, 16), h0=leaf)
     back, = torch.autograd.grad(h, leaf, torch.full_like(h, 1e-30))
     assert (torch.log(back.double()) - (115 + math.log(1e-30))).abs().max() <= 2e-4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_stream_in_place_under_another_batch_stride(device):
+    """The batch stride of a single stream means nothing."""
+    r = rand(device, 16)
+    w, pool, x = r(8, 4), r(2, 5, 3, 8), r(1, 8)
+    one, same = pool[:1, 2], pool[0, 2].unsqueeze(0)
+    assert one.stride(0) != same.stride(0)
+    y, new = MO.causal_conv_step(x, one.clone(), w)
+    y2, _ = MO.causal_conv_step(x, one, w, out=same)
+    assert torch.equal(y, y2) and torch.equal(one, new)
