@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <memory>
 #include <string>
@@ -76,17 +77,30 @@ const unsigned char* active_ptr(const OptTensor& t, const Tensor& on, int64_t B)
   return reinterpret_cast<const unsigned char*>(t->const_data_ptr());
 }
 
+// Bytes from the first element of a tensor's dimensions from `dim` on to behind their last
+int64_t reach(const Tensor& t, int64_t dim) {
+  int64_t n = 1;
+  for (int64_t i = dim; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+  return n * static_cast<int64_t>(t.element_size());
+}
+
+// Do two tensors share memory? Where they repeat at the same distance (streams of one buffer, which may interleave) part by
+// part, else by all that lies between their ends.
+bool meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t delta = static_cast<const char*>(b.const_data_ptr()) - static_cast<const char*>(a.const_data_ptr());
+  const int64_t step = a.dim() > 1 && a.size(0) > 1 ? a.stride(0) * static_cast<int64_t>(a.element_size()) : 0;
+  if (step > 0 && b.dim() > 1 && b.size(0) > 1 && b.stride(0) * static_cast<int64_t>(b.element_size()) == step) {
+    const int64_t from = -reach(b, 1) - delta, below = from / step - (from % step < 0);
+    const int64_t k = std::max(below + 1, 1 - a.size(0));      // the first part of b, counted from a's, that ends behind its start
+    return k < b.size(0) && delta + k * step < reach(a, 1);
+  }
+  return delta < reach(a, 0) && -delta < reach(b, 0);
+}
+
 // A step writes its states while other threads still read their inputs.
 void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs) {
-  const auto end = [](const Tensor& t) {
-    int64_t reach = 1;
-    for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
-    return static_cast<const char*>(t.const_data_ptr()) + reach * static_cast<int64_t>(t.element_size());
-  };
-  if (out.numel() == 0) return;
-  for (const Tensor* t : inputs)
-    TORCH_CHECK(t->numel() == 0 || end(*t) <= static_cast<const char*>(out.const_data_ptr()) ||
-                end(out) <= static_cast<const char*>(t->const_data_ptr()), "out overlaps an input other than the state");
+  for (const Tensor* t : inputs) TORCH_CHECK(!meet(out, *t), "out overlaps an input other than the state");
 }
 
 // What a kernel wrote through a pointer counts as a change of the tensor for autograd too: a backward pass that kept `out`

@@ -298,3 +298,25 @@ def test_one_stream_in_place_under_another_batch_stride(device):
     y, new = MO.causal_conv_step(x, one.clone(), w)
     y2, _ = MO.causal_conv_step(x, one, w, out=same)
     assert torch.equal(y, y2) and torch.equal(one, new)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_and_rows_of_one_buffer_that_share_no_memory(device):
+    """A stream's row beside its state in one buffer: no byte of one is a byte of the other."""
+    r = rand(device, 14)
+    B, D, N = 3, 8, 4
+    w = r(D, 4)
+    for lo, at in ((0, 3), (1, 0)):
+        buf = r(B, 4, D)
+        x, st = buf[:, at], buf[:, lo:lo + 3]
+        y, new = MO.causal_conv_step(x.clone(), st.clone(), w)
+        y2, _ = MO.causal_conv_step(x, st, w, out=st)
+        assert torch.equal(y, y2) and torch.equal(st, new)
+    buf = r(B, 2 * D + 2 * N + D * N)
+    u, dt, Bm, Cm, h = buf.split([D, D, N, N, D * N], -1)
+    h = h.unflatten(-1, (D, N))
+    row = [u, dt, -r(D, N).abs(), Bm, Cm]
+    y, new = S.selective_scan_step(*[t.clone() for t in row], h.clone())
+    rest = buf[:, :-D * N].clone()
+    y2, _ = S.selective_scan_step(*row, h, out=h)
+    assert torch.equal(y, y2) and torch.equal(h, new) and torch.equal(buf[:, :-D * N], rest)
