@@ -99,8 +99,9 @@ bool meet(const Tensor& a, const Tensor& b) {
 }
 
 // A step writes its states while other threads still read their inputs.
-void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs) {
+void check_apart(const Tensor& out, std::initializer_list<const Tensor*> inputs, std::initializer_list<const OptTensor*> others) {
   for (const Tensor* t : inputs) TORCH_CHECK(!meet(out, *t), "out overlaps an input other than the state");
+  for (const OptTensor* t : others) TORCH_CHECK(!given(*t) || !meet(out, **t), "out overlaps an input other than the state");
 }
 
 // What a kernel wrote through a pointer counts as a change of the tensor for autograd too: a backward pass that kept `out`
@@ -287,7 +288,7 @@ std::vector<Tensor> causal_conv_step(const Tensor& x, const Tensor& state, const
   BdhConvDesc d = conv_desc(x, w, bias, state, c10::nullopt, silu);
   std::vector<Tensor> result{new_rows(x, x.sizes())};
   d.y = result[0].data_ptr();
-  if (given(out)) check_apart(*out, {&x, &w});
+  if (given(out)) check_apart(*out, {&x, &w}, {&bias, &active});
   set_state_out(d, x, given(out) ? *out : result.emplace_back(new_rows(x, state.sizes())));
   check_rc(bdh_causal_conv_step(&d, active_ptr(active, x, x.size(0)), cur_stream()), "causal_conv_step");
   changed(out);
@@ -571,7 +572,7 @@ std::vector<Tensor> selective_scan_step(const Tensor& u, const Tensor& dt, const
   BdhScanDesc d = scan_desc(u, dt, A, Bm, Cm, skip, dt_bias, softplus, c10::nullopt, c10::nullopt);
   std::vector<Tensor> result{new_rows(u, u.sizes())};
   d.y = result[0].data_ptr();
-  if (given(out)) check_apart(*out, {&u, &dt, &A, &Bm, &Cm});
+  if (given(out)) check_apart(*out, {&u, &dt, &A, &Bm, &Cm}, {&skip, &dt_bias, &active});
   const Tensor to = given(out) ? *out : result.emplace_back(new_f32(u, {d.B, d.D, d.N}));
   for (const Tensor* t : {&h, &to}) {
     check_rows(*t, u, at::kFloat, {d.B, d.D, d.N}, "h");

@@ -320,3 +320,17 @@ def test_states_and_rows_of_one_buffer_that_share_no_memory(device):
     rest = buf[:, :-D * N].clone()
     y2, _ = S.selective_scan_step(*row, h, out=h)
     assert torch.equal(y, y2) and torch.equal(h, new) and torch.equal(buf[:, :-D * N], rest)
+
+
+@pytest.mark.gpu
+def test_states_that_overlap_a_parameter_are_refused():
+    """Bias, skip and the marks of active streams are read while other threads write states."""
+    z = lambda *s: torch.zeros(*s, device="cuda")                                                        # noqa: E731
+    st = z(2, 3, 8)
+    for more in (dict(bias=st[0, 0]), dict(active=st.view(torch.bool)[0, 0, :2])):
+        with pytest.raises(RuntimeError, match="overlaps an input"):
+            MO.causal_conv_step(z(2, 8), z(2, 3, 8), z(8, 4), out=st, **more)
+    h = z(2, 8, 4)
+    for more in (dict(D=h[0, :2].view(-1)), dict(dt_bias=h[1, 6:].view(-1)), dict(active=h.view(torch.bool)[0, 0, :2])):
+        with pytest.raises(RuntimeError, match="overlaps an input"):
+            S.selective_scan_step(z(2, 8), z(2, 8), z(8, 4), z(2, 4), z(2, 4), z(2, 8, 4), out=h, **more)
