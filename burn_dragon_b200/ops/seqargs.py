@@ -101,14 +101,15 @@ def check_out(out: Optional[torch.Tensor], src: torch.Tensor, name: str) -> None
         if st < reach:
             raise ValueError(f"{name}: its rows overlap one another")
         reach = st * (n - 1) + reach
-    if same or not out.numel() or out.untyped_storage().data_ptr() != src.untyped_storage().data_ptr():
+    if same or not out.numel():
+        return
+    # by their addresses: two storages may be made over the same memory
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
+    (a0, a1), (b0, b1) = span(out), span(src)
+    if a1 <= b0 or b1 <= a0:
         return
     if strides == from_strides:                          # slices of one buffer, which may interleave
         delta, odd = divmod(out.data_ptr() - src.data_ptr(), out.element_size())
-        meet = odd or _meet(delta, dims[::-1])
-    else:
-        span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))  # noqa: E731
-        (a0, a1), (b0, b1) = span(out), span(src)
-        meet = a0 < b1 and b0 < a1
-    if meet:
-        raise ValueError(f"{name} overlaps the state without being it")
+        if not (odd or _meet(delta, dims[::-1])):
+            return
+    raise ValueError(f"{name} overlaps the state without being it")

@@ -334,3 +334,15 @@ def test_states_that_overlap_a_parameter_are_refused():
     for more in (dict(D=h[0, :2].view(-1)), dict(dt_bias=h[1, 6:].view(-1)), dict(active=h.view(torch.bool)[0, 0, :2])):
         with pytest.raises(RuntimeError, match="overlaps an input"):
             S.selective_scan_step(z(2, 8), z(2, 8), z(8, 4), z(2, 4), z(2, 4), z(2, 8, 4), out=h, **more)
+
+
+def test_states_that_overlap_through_another_storage_are_refused():
+    """Two tensors made over the same memory have storages of their own."""
+    memory = bytearray(4 * 72)
+    old = torch.frombuffer(memory, dtype=torch.float32, count=48).view(2, 3, 8)
+    new = torch.frombuffer(memory, dtype=torch.float32, count=48, offset=96).view(2, 3, 8)
+    assert old.untyped_storage().data_ptr() != new.untyped_storage().data_ptr()
+    with pytest.raises(ValueError, match="overlaps"):
+        MO.causal_conv_step(torch.zeros(2, 8), old, torch.zeros(8, 4), out=new)
+    again = torch.frombuffer(memory, dtype=torch.float32, count=48).view(2, 3, 8)
+    MO.causal_conv_step(torch.zeros(2, 8), old, torch.zeros(8, 4), out=again)
