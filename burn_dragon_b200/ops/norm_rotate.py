@@ -46,7 +46,8 @@ def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, 
         v = v * w.to(ct) if w is not None else v
         v = v + b.to(ct) if b is not None else v
         if angles is not None:
-            an = angles if keep is None else torch.where(keep[..., 0], angles, 0.0)
+            an = angles.to(torch.promote_types(angles.dtype, torch.float32))
+            an = an if keep is None else torch.where(keep[..., 0], an, 0.0)
             v = _turn(v, an.cos().to(ct)[:, :, None], an.sin().to(ct)[:, :, None])
         outs.append((v if keep is None else torch.where(keep, v, 0.0)).to(x.dtype))
     return tuple(outs)
@@ -60,7 +61,7 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     """RMS norm and rotation of q [B, T, Hq, Dh] and k [B, T, Hk, Dh] (or None): -> (q', k'), contiguous, in their type.
     Rows are fp32, fp16 or bf16 and may be views into a wider projection (channels adjacent); Dh is even and at most
     512. Weights and biases: [Dh] for all heads or [heads, Dh], all of them alike (None: 1 and 0).
-    Rotation, if any: `angles` [B, T, pairs] in radians, or `freqs` [2 * pairs] in cycles per position with `positions`
+    Rotation, if any: `angles` [B, T, pairs] in radians (of any floating type, as exact as that type has them), or `freqs` [2 * pairs] in cycles per position with `positions`
     - the first token's (an int), or [T] or [B, T] integers (the single-token form has T = 1 and one position a stream).
     `lengths` [B]: rows behind a sequence's length give 0 and take no part in any gradient. The kernels
     refuse second derivatives and forward-mode tangents."""
@@ -113,6 +114,8 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     if not (B * T <= 1 << 30):
         raise ValueError("more than 2^30 tokens")
     pos = None
+    if angles is not None and angles.dtype is torch.float64:
+        angles = torch.remainder(angles, 2 * math.pi)    # before the kernel's 32 bits, which leave little of a large angle
     if isinstance(positions, torch.Tensor):
         pos = positions if positions.dim() == 2 else positions.expand(B, T)
     out = native.ops.norm_rotate(

@@ -346,3 +346,25 @@ def test_states_that_overlap_through_another_storage_are_refused():
         MO.causal_conv_step(torch.zeros(2, 8), old, torch.zeros(8, 4), out=new)
     again = torch.frombuffer(memory, dtype=torch.float32, count=48).view(2, 3, 8)
     MO.causal_conv_step(torch.zeros(2, 8), old, torch.zeros(8, 4), out=again)
+
+
+@pytest.mark.parametrize("kind", ["far", "half"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_angles_of_other_types(device, kind):
+    """Angles keep the value they have in their own type: 10^7 radians in float64 (32 bits leave whole radians), bf16 angles
+    whose sine is not one of bf16. A row's norm is off by (Dh / 2 + 8) u, its turn by 2^-21 |v|: 2^-19 of the pair holds them."""
+    r = rand(device, 17)
+    q, do = r(2, 5, 3, 16), r(2, 5, 3, 16)
+    angle = 1e7 * r(2, 5, 8).double() if kind == "far" else (3 * r(2, 5, 8)).bfloat16()
+    leaf = angle.clone().requires_grad_()
+    out, _ = NR.norm_rotate(q, angles=leaf)
+    da, = torch.autograd.grad(out, leaf, do)
+    v = q.double() / (q.double().square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    turned = torch.view_as_complex(v.unflatten(-1, (8, 2))) * torch.polar(torch.ones(2, 5, 1, 8, device=device).double(), angle.double()[:, :, None])
+    want = torch.view_as_real(turned).flatten(-2)
+    size = turned.abs()[..., None].expand(*turned.shape, 2).flatten(-2)
+    assert ((out.double() - want).abs() <= 2.0 ** -19 * size).all()
+    cross = want[..., 0::2] * do.double()[..., 1::2] - want[..., 1::2] * do.double()[..., 0::2]
+    scale = (turned.abs() * do.double().unflatten(-1, (8, 2)).abs().sum(-1)).sum(2)
+    assert da.dtype == angle.dtype
+    assert ((da.double() - cross.sum(2)).abs() <= 2.0 ** -18 * scale + torch.finfo(da.dtype).eps / 2 * cross.sum(2).abs()).all()
