@@ -24,16 +24,20 @@ def _turn(v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return torch.cat((torch.stack((a * cos - b * sin, b * cos + a * sin), -1).flatten(-2), v[..., n:]), -1)
 
 
+def _angles_at(positions, freqs: torch.Tensor, B: int, T: int) -> torch.Tensor:
+    """[B, T, pairs] in float64: 2 pi frac(position * freq)"""
+    pos = positions if isinstance(positions, torch.Tensor) else positions + torch.arange(T, device=freqs.device)
+    turns = pos.double()[..., None] * freqs[0::2].double()
+    return ((turns - turns.floor()) * (2 * math.pi)).expand(B, T, -1)
+
+
 def norm_rotate_reference(q, k=None, q_weight=None, k_weight=None, q_bias=None, k_bias=None, *, angles=None, freqs=None, positions=0,
                           lengths=None, eps: float = 1e-5):
     """Torch statement of `norm_rotate` (any device and floating type, differentiable)."""
     B, T = q.shape[:2]
     ct = torch.promote_types(q.dtype, torch.float32)
     if angles is None and freqs is not None:
-        pos = positions if isinstance(positions, torch.Tensor) else positions + torch.arange(T, device=q.device)
-        turns = pos.double()[..., None] * freqs[0::2].double()
-        angles = (turns - turns.floor()) * (2 * math.pi)
-        angles = angles.expand(B, T, -1)
+        angles = _angles_at(positions, freqs, B, T)
     keep = A.valid_rows(lengths, B, T, q.device)
     keep = keep[..., None, None] if keep is not None else None
     outs = []
@@ -114,6 +118,8 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     if not (B * T <= 1 << 30):
         raise ValueError("more than 2^30 tokens")
     pos = None
+    if freqs is not None and freqs.dtype is torch.float64:      # (the kernel has them in 32 bits)
+        angles, freqs, positions, pos0 = _angles_at(positions, freqs, B, T), None, 0, 0
     if angles is not None and angles.dtype is torch.float64:
         angles = torch.remainder(angles, 2 * math.pi)    # before the kernel's 32 bits, which leave little of a large angle
     if isinstance(positions, torch.Tensor):

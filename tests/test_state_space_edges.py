@@ -368,3 +368,20 @@ def test_angles_of_other_types(device, kind):
     scale = (turned.abs() * do.double().unflatten(-1, (8, 2)).abs().sum(-1)).sum(2)
     assert da.dtype == angle.dtype
     assert ((da.double() - cross.sum(2)).abs() <= 2.0 ** -18 * scale + torch.finfo(da.dtype).eps / 2 * cross.sum(2).abs()).all()
+
+
+@pytest.mark.parametrize("form", ["int", "tensor"])
+@pytest.mark.parametrize("device", DEVICES)
+def test_frequencies_in_64_bits(device, form):
+    """At position 3 10^9 a frequency rounded to 32 bits is off by 3 10^9 f 2^-25 turns, 90 f: in 64 bits nothing of that is left."""
+    r = rand(device, 19)
+    q, start = r(2, 5, 3, 16), 3_000_000_000
+    freqs = (torch.rand(8, generator=torch.Generator().manual_seed(2), dtype=torch.float64) / 3).repeat_interleave(2).to(device)
+    pos = start + torch.arange(5, device=device)
+    out, _ = NR.norm_rotate(q, freqs=freqs, positions=start if form == "int" else pos)
+    turns = pos.double()[:, None] * freqs[0::2]
+    angle = 2 * math.pi * (turns - turns.floor())
+    v = q.double() / (q.double().square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    turned = torch.view_as_complex(v.unflatten(-1, (8, 2))) * torch.polar(torch.ones_like(angle), angle)[None, :, None]
+    size = turned.abs()[..., None].expand(*turned.shape, 2).flatten(-2)
+    assert ((out.double() - torch.view_as_real(turned).flatten(-2)).abs() <= 2.0 ** -19 * size).all()
