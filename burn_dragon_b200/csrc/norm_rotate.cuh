@@ -19,6 +19,7 @@
 #include "bdh_kernels.h"
 #include "pair_math.cuh"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace bdh {
@@ -134,7 +135,10 @@ __device__ __forceinline__ float group_sum(float v, int G) {
     if (o < G) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// 1 / sqrt(x). The quick root takes a subnormal x for 0. With a normal eps there is none; SUB: there may be (2 % of a pass).
+template <bool SUB>
 __device__ __forceinline__ float rsqrt_of(float x) {
+  if constexpr (SUB) return rsqrtf(x);
   float r;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
@@ -212,7 +216,7 @@ __device__ __forceinline__ f2 turn(f2 v, float2 e) {
   return pack2(x * e.x - y * e.y, fmaf(y, e.x, x * e.y));
 }
 
-template <typename T, int V, bool VEC, int NV, int U>
+template <typename T, int V, bool VEC, int NV, int U, bool SUB>
 __global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_kernel(const NormArgs a, int w_rows) {
   using P = Place<T, V, VEC, NV>;
   using Raw = typename P::Raw;
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_
         for (int i = 0; i < N; ++i) ss = fma2(x[n][i], x[n][i], ss);
       }
       load(next, next_rows, u);
-      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
+      const float rs = rsqrt_of<SUB>(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
       if (!now.live || !me.has(a, u)) continue;
       const bool key = me.key(a, u);
       T* o = static_cast<T*>(key ? d.k_out : d.q_out) + rows.dense(a, me, u);
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? FWD_BLOCKS : 2) norm_rotate_fwd_
 // Shared memory: weights; two sets of angles; then (dang) the rows' cross products, or (at the end) the rows' sums for the
 // weights. PER_HEAD: a sum for each of the thread's heads; else one for q and one for k. partial: [2 (weight, bias)]
 // [lines][width], see norm_rotate_params_kernel.
-template <typename T, int V, bool VEC, int NV, int U, bool PER_HEAD, bool BIAS>
+template <typename T, int V, bool VEC, int NV, int U, bool PER_HEAD, bool BIAS, bool SUB>
 __global__ void __launch_bounds__(NT, NV == 1 ? BWD_BLOCKS : 2) norm_rotate_bwd_kernel(const NormArgs a, int w_rows, float* partial, float* dang) {
   using P = Place<T, V, VEC, NV>;
   using Raw = typename P::Raw;
@@ -369,7 +373,7 @@ __global__ void __launch_bounds__(NT, NV == 1 ? BWD_BLOCKS : 2) norm_rotate_bwd_
         }
       }
       load(next, next_at, u);
-      const float rs = rsqrt_of(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
+      const float rs = rsqrt_of<SUB>(fmaf(group_sum(sum2(ss), a.G), a.per_column, eps));
       const float m = group_sum(sum2(dot), a.G) * a.per_column * rs * rs;            // mean(w dv x r) r, per element of x
       if (!now.live || !me.has(a, u)) continue;
       T* o = static_cast<T*>(key ? d.dk : d.dq) + at.dense(a, me, u);
@@ -550,6 +554,8 @@ NormArgs args_for(const BdhNormRotateDesc& d, int v, int nv, int groups_a_block)
   return a;
 }
 
+bool subnormal(const BdhNormRotateDesc& d) { return !(d.eps >= FLT_MIN); }      // may mean x^2 + eps be?
+
 int launched() { return cudaGetLastError() == cudaSuccess ? BDH_OK : BDH_ERR_LAUNCH; }
 
 // Blocks along the tokens: as many as run at once, so that the weights are read (and their gradients written) once per
@@ -575,7 +581,7 @@ int fwd_launch(const BdhNormRotateDesc& d, cudaStream_t s) {
   const NormArgs a = args_for(d, V, NV, U);
   const int w_rows = weight_rows(a);
   const size_t smem = sizeof(float) * 2 * w_rows * a.G * V * NV + sizeof(float2) * 2 * a.TS * d.P;
-  auto kernel = norm_rotate_fwd_kernel<T, V, VEC, NV, U>;
+  auto kernel = subnormal(d) ? norm_rotate_fwd_kernel<T, V, VEC, NV, U, true> : norm_rotate_fwd_kernel<T, V, VEC, NV, U, false>;
   if (const int rc = allow_smem(kernel, smem)) return rc;
   kernel<<<dim3(token_blocks(a, FWD_BLOCKS), a.slices), NT, smem, s>>>(a, w_rows);
   return launched();
@@ -619,7 +625,8 @@ int bwd_launch(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
   const BwdPlan p = bwd_plan(a, V * NV, want_w, want_b, o.dang != nullptr);
   float* partial = want_w ? o.scratch : nullptr;        // (with BIAS the bias' sums lie behind the weights')
   float* ang = o.dang ? (p.angles ? o.scratch + p.partial : o.dang) : nullptr;
-  auto kernel = norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD, BIAS>;
+  auto kernel = subnormal(d) ? norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD, BIAS, true>
+                             : norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD, BIAS, false>;
   if (const int rc = allow_smem(kernel, p.smem)) return rc;
   kernel<<<dim3(p.blocks, a.slices), NT, p.smem, s>>>(a, weight_rows(a), partial, ang);
   if (launched() != BDH_OK) return BDH_ERR_LAUNCH;

@@ -385,3 +385,22 @@ def test_frequencies_in_64_bits(device, form):
     turned = torch.view_as_complex(v.unflatten(-1, (8, 2))) * torch.polar(torch.ones_like(angle), angle)[None, :, None]
     size = turned.abs()[..., None].expand(*turned.shape, 2).flatten(-2)
     assert ((out.double() - torch.view_as_real(turned).flatten(-2)).abs() <= 2.0 ** -19 * size).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_whose_squares_are_subnormal(device, dtype):
+    """eps = 0 and elements of about 1e-20, whose squares (1e-40) are subnormal numbers of fp32, in steps of 1.4e-45: each is
+    off by at most 7e-46, the mean by 1e-5 of itself with the elements drawn here, the result by half of that and its rounding."""
+    r = rand(device, 18)
+    x = (1e-20 * (1 + r(2, 3, 2, 16).abs())).to(dtype)
+    leaf = x.clone().requires_grad_()
+    out, _ = NR.norm_rotate(leaf, eps=0.0)
+    dx, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    v = x.double().requires_grad_()
+    want = v / v.square().mean(-1, keepdim=True).sqrt()
+    dw, = torch.autograd.grad(want, v, torch.ones_like(want))
+    half = torch.finfo(dtype).eps / 2
+    assert ((out.double() - want).abs() <= (1e-5 + half) * want.abs()).all()
+    if device == "cuda":                              # (torch's own derivative of the root takes its third power: inf)
+        assert (dx.double() - dw).abs().max() <= (1e-4 + half) * (1 / x.double().square().mean(-1).sqrt()).max()
