@@ -41,7 +41,7 @@ def selective_scan_reference(u, dt, A, Bm, Cm, D=None, *, dt_bias=None, dt_softp
         y = y + D.to(ct) * us
     if keep is not None:
         y = torch.where(keep[..., None], y, 0.0)
-    return y.to(u.dtype), h
+    return y.to(u.dtype), (h if T else h.clone())               # (a state of its own, also behind no rows)
 
 
 def _check(u, dt, A, Bm, Cm, D, dt_bias, dims: int) -> Tuple[int, int, int]:

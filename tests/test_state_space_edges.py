@@ -404,3 +404,18 @@ def test_rows_whose_squares_are_subnormal(device, dtype):
     assert ((out.double() - want).abs() <= (1e-5 + half) * want.abs()).all()
     if device == "cuda":                              # (torch's own derivative of the root takes its third power: inf)
         assert (dx.double() - dw).abs().max() <= (1e-4 + half) * (1 / x.double().square().mean(-1).sqrt()).max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_state_behind_an_empty_prompt_is_its_own(device):
+    """A prompt of no rows returns the state it was given, in memory of its own: a step in place on the one leaves the other."""
+    z = lambda *s: torch.zeros(*s, device=device)                                                        # noqa: E731
+    h0 = torch.randn(2, 8, 4, device=device)
+    kept = h0.clone()
+    _, h = S.selective_scan(z(2, 0, 8), z(2, 0, 8), z(8, 4), z(2, 0, 4), z(2, 0, 4), h0=h0)
+    assert torch.equal(h, h0) and h.data_ptr() != h0.data_ptr()
+    S.selective_scan_step(z(2, 8), z(2, 8) + 1, z(8, 4) - 1, z(2, 4), z(2, 4), h, out=h)
+    assert torch.equal(h0, kept) and not torch.equal(h, h0)
+    st = torch.randn(2, 3, 8, device=device)
+    _, end = MO.causal_conv(z(2, 0, 8), z(8, 4), state=st)
+    assert torch.equal(end, st) and end.data_ptr() != st.data_ptr()
