@@ -419,3 +419,48 @@ def test_the_state_behind_an_empty_prompt_is_its_own(device):
     st = torch.randn(2, 3, 8, device=device)
     _, end = MO.causal_conv(z(2, 0, 8), z(8, 4), state=st)
     assert torch.equal(end, st) and end.data_ptr() != st.data_ptr()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,B,T,C,k,ragged", [
+    (torch.bfloat16, 4, 20_000, 8, 4, False),         # 5000 tiles of 16 rows: a thread walks a second one
+    (torch.float32, 3, 30_011, 6, 3, True),
+    (torch.float16, 4, 20_000, 7, 2, True),           # element by element
+    (torch.float32, 2, 2500, 4160, 4, False),         # tiles of 64 rows
+    (torch.bfloat16, 2, 3000, 3968, 2, True),         # of 32
+    (torch.bfloat16, 4, 20_100, 16, 5, True),         # a width known at run time
+])
+def test_convolutions_of_many_tiles(dtype, B, T, C, k, ragged):
+    """Against the definition in 64 bits. A gradient row is a sum of k terms, each off by 16 u and the quick SiLU's 2^-19 (1 + m) for
+    inputs of magnitude m; a parameter's is a sum of n = B T of them in an order whose longest chain is below n / 64 + 256 terms."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")                                           # noqa: E731
+    x, dy, w, b, st = r(B, T, C).to(dtype), r(B, T, C).to(dtype), r(C, k) / k ** 0.5, 0.1 * r(C), r(B, k - 1, C).to(dtype)
+    n = torch.randint(T // 2, T + 1, (B,), generator=g, device="cuda") if ragged else None
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, st)]
+    y, _ = MO.causal_conv(leaves[0], leaves[1], leaves[2], state=leaves[3], lengths=n)
+    dx, dw, db, dst = torch.autograd.grad(y, leaves, dy)
+    keep = torch.ones(B, T, 1, device="cuda", dtype=torch.bool) if n is None else (torch.arange(T, device="cuda") < n[:, None])[..., None]
+    eps = torch.finfo(dtype).eps / 2
+    floor = 2.0 ** -25 if dtype == torch.float16 else 1e-30
+    for c in range(0, C, 1024):                       # channels are independent
+        at = slice(c, c + 1024)
+        seq = torch.cat((st[..., at].double(), torch.where(keep, x[..., at].double(), 0.0)), 1)
+        pre = sum((seq[:, j:j + T] * w[at, j].double() for j in range(k)), b[at].double())
+        mag = sum((seq[:, j:j + T].abs() * w[at, j].double().abs() for j in range(k)), b[at].double().abs())
+        sig = torch.sigmoid(pre)
+        off = 2.0 ** -19 * (1 + mag)
+        want = torch.where(keep, pre * sig, 0.0)
+        assert ((y[..., at].double() - want).abs() <= eps * want.abs() + off * mag + floor).all()
+        gr = torch.where(keep, dy[..., at].double() * sig * (1 + pre * (1 - sig)), 0.0)
+        bound = torch.where(keep, dy[..., at].double().abs() * off * (1 + mag), 0.0)
+        ds, es = torch.zeros_like(seq), torch.zeros_like(seq)
+        chain = (B * T / 64 + 256) * U
+        for j in range(k):
+            ds[:, j:j + T] += gr * w[at, j].double()
+            es[:, j:j + T] += (bound + 16 * U * gr.abs()) * w[at, j].double().abs()
+            want, lim = (gr * seq[:, j:j + T]).sum((0, 1)), ((bound + chain * gr.abs()) * seq[:, j:j + T].abs()).sum((0, 1))
+            assert ((dw[at, j].double() - want).abs() <= lim + eps * want.abs()).all(), j
+        assert ((db[at].double() - gr.sum((0, 1))).abs() <= (bound + chain * gr.abs()).sum((0, 1))).all()
+        assert ((dx[..., at].double() - ds[:, k - 1:]).abs() <= eps * ds[:, k - 1:].abs() + es[:, k - 1:] + floor).all()
+        assert ((dst[..., at].double() - ds[:, :k - 1]).abs() <= eps * ds[:, :k - 1].abs() + es[:, :k - 1] + floor).all()
