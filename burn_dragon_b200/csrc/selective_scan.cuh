@@ -759,6 +759,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
   for (int j = 0; j < S::E; ++j) sum_skip[j] = sum_bias[j] = 0.f;
   const int first = w.seg * a.per_seg, last = min(first + a.per_seg, a.tiles);
   const int row = lane / 2, col = (lane & 1) * S::E;
+  const unsigned skip_bits = d.skip != nullptr ? ~0u : 0u;     // (without a skip dy, which may be infinite, has no part in du)
   Tile<T, G, CT, VEC, true> x;
   x.load(d, w.b, c0, (last - 1) * LT, len);
   f2 mark[CT][2];                                      // the next tile's first state, fetched with its rows
@@ -918,8 +919,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
           dd[j] = 0.f;
           if (in) {
             const float2 s = sh.out[row][cc];
-            du = sh.in.step[row][cc].x * s.x;
-            if (d.skip != nullptr) du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * dy[i][j]);
+            du = fmaf(sh.in.step[row][cc].x, s.x, sh.in.skip[cc] * __uint_as_float(__float_as_uint(dy[i][j]) & skip_bits));
             dd[j] = fmaf(u[i][j], s.x, LN2 * s.y);
             sum_skip[i * S::V + j] = fmaf(dy[i][j], u[i][j], sum_skip[i * S::V + j]);
           }
