@@ -11,8 +11,9 @@
 // atomics: two runs give the same bits). Channels go in pairs (one instruction for two), rows in sets that change
 // places instead of moving, and the next set is on its way while one is worked on.
 //
-// Measured, 8 x 2048 x 4096 bf16: forward 57 us (0.73 of the copy rate), backward 110 us (0.57: about 30 instructions an
-// element pair and row, at three warps a scheduler) and 7 us for the parameters' sums; one token of 64 streams 4.6 us.
+// Measured, 8 x 2048 x 4096 bf16: forward 57 us (0.73 of the copy rate), backward 110 us (0.57) and 7 us for the parameters' sums;
+// one token of 64 streams 4.5 us. The backward pass issues about 30 instructions an element pair and row, but a scheduler is busy
+// only 43 % of the time: its three warps wait for the results of their own arithmetic.
 #include "bdh_kernels.h"
 #include "pair_math.cuh"
 
@@ -543,8 +544,8 @@ int step_launch(const BdhConvDesc& d, const unsigned char* active, cudaStream_t 
   return launched();
 }
 
-// Channels a thread. Forward two: the most threads that still store a pair (8 x 2048 x 4096 bf16: 55 us; four 57,
-// eight 78 us, at 4096 x 2048 10.5, 18 and 26 us). Backward 8 bytes: rows come through shared memory there, and a
+// Channels a thread. Forward two: the most threads that still store a pair (8 x 2048 x 4096 bf16, in one run: 55 us; four 57,
+// eight 78 us; at 4096 x 2048 10.5, 18 and 26 us). Backward 8 bytes: rows come through shared memory there, and a
 // thread's overhead is shared by more elements.
 template <typename T>
 int fwd_type(const BdhConvDesc& d, cudaStream_t s) {

@@ -13,8 +13,9 @@
 // groups of hr rows, each of q or of k alone, so that a weight's gradient stays in registers over all rows that share
 // it. Sums are fp32, in a fixed order.
 //
-// Measured, 4 x 4096 tokens, 32 + 8 heads of 128, bf16: forward 89 us (0.60 of the copy rate), backward 158 us (0.50): the
-// pairs' turns and conversions issue about 20 instructions a pair of elements. 64 tokens alone: 5 us.
+// Measured, 4 x 4096 tokens, 32 + 8 heads of 128, bf16: forward 89 us (0.58 of the copy rate), backward 158 us (0.49). The pairs' turns
+// and conversions issue about 20 instructions a pair of elements, with a scheduler busy 60 and 49 % of the time: at five and
+// three warps each they wait for the results of their own arithmetic and of shared memory. 64 tokens alone: 5 us.
 #pragma once
 #include "bdh_kernels.h"
 #include "pair_math.cuh"
@@ -26,8 +27,8 @@ namespace bdh {
 namespace {
 
 constexpr int NT = 128;
-// Blocks an SM: as many as run at once, in one round over the tokens. Registers for five and three (forward 87 us, backward
-// 156 us at 4 x 4096 tokens, 32 + 8 heads of 128, bf16; for four and two 90 and 191 us, for six and four, which spill, 125 and
+// Blocks an SM: as many as run at once, in one round over the tokens. Registers for five and three (4 x 4096 tokens, 32 + 8 heads
+// of 128, bf16, in one run: forward 87 us, backward 156 us; for four and two 90 and 191 us, for six and four, which spill, 125 and
 // 203 us; two rounds of blocks 89 and 171 us). Rows of several packs a lane need more.
 constexpr int FWD_BLOCKS = 5, BWD_BLOCKS = 3;
 

@@ -24,9 +24,9 @@
 // Exponentials are the hardware's (2 units in the last place) with their mean error taken out (`decay`): the gradient of A over 2048
 // steps is off by 0.95e-6 of its norm, as with exact ones in fp32 (0.9e-6), which would take a third more time.
 //
-// Measured (bf16 rows, 16 states): a prompt of 8192 x 4096 361 us, of 6 x 777 x 1000 with 64 states (fp16, lengths drawn) 107 to 134 us; forward
-// 4 x 2048 x 2048 160 us, backward 450 us. At full occupancy a pass runs at 0.7 of the exponentials' rate; the backward
-// kernel issues ~190 instructions for 8 states of a lane and step, at two warps a scheduler.
+// Measured (bf16 rows, 16 states): a prompt of 8192 x 4096 362 us, of 6 x 777 x 1000 with 64 states (fp16, lengths drawn) 107 to 134 us; forward
+// 4 x 2048 x 2048 159 us, backward 470 us. With enough warps a pass runs at 0.64 to 0.78 of the exponentials' rate; the backward
+// kernel issues ~190 instructions for 8 states of a lane and step, and at two warps a scheduler is busy 54 % of the time.
 #pragma once
 #include "bdh_kernels.h"
 #include "device_once.h"
