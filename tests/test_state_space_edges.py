@@ -489,3 +489,84 @@ def test_slow_states_do_not_drift(device, form, n):
     for t in range(T):
         want = torch.exp(dt[:, t, :, None].double() * A.double()) * want + dt[:, t, :, None].double()
     assert (h.double() / want - 1).mean().abs() <= n * 1.6e-8 + 4e-8
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_lengths_in_32_bits(device):
+    """The same bits whatever the type of the lengths, which may be a view; negative ones are 0, large ones all rows."""
+    r = rand(device, 21)
+    long = torch.tensor([[5, 0], [-1, 0], [40, 0], [17, 0]], device=device)[:, 0]
+    x, w = r(4, 21, 16), r(16, 4)
+    q, qw = r(4, 21, 2, 16), r(16)
+    u, dt, A, Bm, Cm = r(4, 21, 16), r(4, 21, 16).abs(), -r(16, 8).abs(), r(4, 21, 8), r(4, 21, 8)
+    for n in (long.int(), long.clamp(0, 21), long.clamp(0, 21).int()):
+        assert all(torch.equal(a, b) for a, b in zip(MO.causal_conv(x, w, lengths=long), MO.causal_conv(x, w, lengths=n)))
+        assert torch.equal(NR.norm_rotate(q, q_weight=qw, lengths=long)[0], NR.norm_rotate(q, q_weight=qw, lengths=n)[0])
+        assert all(torch.equal(a, b) for a, b in zip(S.selective_scan(u, dt, A, Bm, Cm, lengths=long), S.selective_scan(u, dt, A, Bm, Cm, lengths=n)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_convolution_of_one_tap(device):
+    """Width 1 has a state of no rows: given or not, carried or stepped, it is act(bias + w x)."""
+    r = rand(device, 22)
+    x, w, b, st = r(3, 9, 24), r(24, 1), r(24), torch.zeros(3, 0, 24, device=device)
+    n = torch.tensor([9, 0, 4], device=device)
+    keep = (torch.arange(9, device=device) < n[:, None])[..., None]
+    pre = x.double() * w[:, 0].double() + b.double()
+    want = torch.where(keep, pre * torch.sigmoid(pre), 0.0)
+    for state in (None, st):
+        y, end = MO.causal_conv(x, w, b, state=state, lengths=n)
+        assert end.shape == (3, 0, 24) and (y.double() - want).abs().max() <= 2.0 ** -19 * (1 + pre.abs().max()) * pre.abs().max()
+    y1, end = MO.causal_conv_step(x[:, 0], st, w, b, active=n > 0)
+    assert end.shape == (3, 0, 24) and (y1 - y[:, 0]).abs().max() <= 2.0 ** -20 * (1 + pre.abs().max()) * pre.abs().max()
+    MO.causal_conv_step(x[:, 0], st, w, b, out=st)
+
+
+@pytest.mark.gpu
+def test_offsets_past_31_bits():
+    """Views whose last sequence starts more than 2^31 elements in; only what is read of them exists in full."""
+    B, T, step = 3, 20, 2 ** 30 + 64
+    wide = torch.empty(B * step, device="cuda", dtype=torch.bfloat16)
+    tail = wide.as_strided((B, 2 ** 14), (step, 1), step - 2 ** 14)
+    tail.copy_(torch.randn(B, 2 ** 14, device="cuda"))
+    view = lambda at, *s: wide.as_strided((B, T, *s), (step, 400, *torch.empty(*s).stride()), step - 2 ** 14 + at)   # noqa: E731
+    u, dt, Bm, Cm, q = view(0, 64), view(64, 64), view(128, 16), view(144, 16), view(160, 3, 64)
+    A = -torch.rand(64, 16, device="cuda")
+    assert (B - 1) * step > 2 ** 31
+    for fn, tensors in ((lambda *t: S.selective_scan(*t[:2], A, *t[2:], dt_softplus=True), [u, dt, Bm, Cm]), (lambda t: NR.norm_rotate(t, t[:, :, :2])[:2], [q])):
+        leaves, dense = [t.detach().requires_grad_() for t in tensors], [t.detach().clone().requires_grad_() for t in tensors]
+        got, want = fn(*leaves), fn(*dense)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        seeds = [torch.ones_like(o) for o in got]
+        grads = [torch.autograd.grad(got, leaves, seeds), torch.autograd.grad(want, dense, seeds)]
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """The same inputs through forward and backward passes that run beside each other, each with scratch of its own."""
+    fns = {k: v for k, v in calls("cuda").items()}
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    big = {"conv": [torch.randn(4, 2000, 256, device="cuda"), torch.randn(256, 4, device="cuda"), torch.randn(256, device="cuda"),
+                    torch.randn(4, 3, 256, device="cuda")],
+           "norm_rotate": [torch.randn(4, 500, 8, 64, device="cuda"), torch.randn(4, 500, 2, 64, device="cuda")] +
+                          [torch.randn(64, device="cuda") for _ in range(4)] + [torch.randn(4, 500, 32, device="cuda")],
+           "scan": [torch.randn(2, 1500, 64, device="cuda"), torch.randn(2, 1500, 64, device="cuda"), -torch.rand(64, 16, device="cuda"),
+                    torch.randn(2, 1500, 16, device="cuda"), torch.randn(2, 1500, 16, device="cuda"), torch.randn(64, device="cuda"),
+                    torch.randn(64, device="cuda"), torch.randn(2, 64, 16, device="cuda")]}
+
+    def run(name):
+        leaves = [t.detach().requires_grad_() for t in big[name]]
+        outs = fns[name][0](*leaves)
+        return [*(o.detach() for o in outs), *torch.autograd.grad([o.square().sum() for o in outs], leaves)]
+
+    want = {name: run(name) for name in NAMES}
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append({name: run(name) for name in NAMES})
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for name in NAMES for a, b in zip(want[name], g[name]))
