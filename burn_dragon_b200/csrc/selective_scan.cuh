@@ -380,8 +380,9 @@ __device__ __forceinline__ void store_state(float* p, int c, int n0, const BdhSc
 }
 
 // States that N is padded with have to stay 0 whatever their channel's step, which may be infinite, and 0 * inf is not 0.
-// Lanes of padding alone read the step (and dy) of a column of zeros behind the warp's channels; a lane that has both kinds
-// (N not a multiple of 4, so never in packs) clears the others' bits. Where the rows come in packs this costs nothing.
+// Lanes of padding alone read the step (and dy) of a column of zeros behind the warp's channels, which costs nothing; a lane that has
+// both kinds (N not a multiple of 4) clears the others' bits (3 % of a pass).
+enum { PACKS, ELEMENTS, MIXED };                       // rows in packs of 16 bytes; element by element; so, with such lanes
 struct Real {
   f2 m[2];                             // all bits of this lane's states below N
   __device__ __forceinline__ Real(int n0, int N) {
@@ -391,8 +392,8 @@ struct Real {
     m[0] = static_cast<f2>(v[1]) << 32 | v[0];
     m[1] = static_cast<f2>(v[3]) << 32 | v[2];
   }
-  template <bool VEC>
-  __device__ __forceinline__ f2 keep(f2 x, int j) const { return VEC ? x : x & m[j]; }
+  template <int FIT>
+  __device__ __forceinline__ f2 keep(f2 x, int j) const { return FIT == MIXED ? x & m[j] : x; }
 };
 
 // A2 = A log2(e); 0 for padding
@@ -446,7 +447,7 @@ __device__ __forceinline__ void carry(const ScanArgs& a, int b, int from, int to
       for (int k = 0; k < CT; ++k)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          h[k][j] = real.keep<false>(add2(grown2(h[k][j], mul2(both(dt[i][k]), A2[k][j])), in[i][k][j]), j);
+          h[k][j] = real.keep<MIXED>(add2(grown2(h[k][j], mul2(both(dt[i][k]), A2[k][j])), in[i][k][j]), j);
   }
 }
 
@@ -508,8 +509,9 @@ struct FwdMem {
   Ring<T, G, CT, VEC, false> ring;
 };
 
-template <typename T, int G, int CT, bool VEC>
+template <typename T, int G, int CT, int FIT>
 __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd_kernel(const ScanArgs a, long long units, float* marks) {
+  constexpr bool VEC = FIT == PACKS;
   using S = Shape<T, G, CT>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31;
@@ -559,8 +561,8 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_fwd
         for (int s = 0; s < Group::N; ++s)
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
-            h[k][0] = real.template keep<VEC>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
-            h[k][1] = real.template keep<VEC>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
+            h[k][0] = real.template keep<FIT>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
+            h[k][1] = real.template keep<FIT>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
             sh.part[s0 + s][k * 32 + lane] = sum2(fma2(now.k[s][1], h[k][1], mul2(now.k[s][0], h[k][0])));
           }
         now = next;
@@ -612,8 +614,9 @@ struct SweepMem {
   Ring<T, G, CT, VEC, REV> ring;
 };
 
-template <typename T, int G, int CT, bool VEC, bool REV>
+template <typename T, int G, int CT, int FIT, bool REV>
 __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_sweep_kernel(const ScanArgs a, long long units, float* seg_state, float* seg_dt) {
+  constexpr bool VEC = FIT == PACKS;
   using S = Shape<T, G, CT>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31;
@@ -680,7 +683,7 @@ __global__ void __launch_bounds__(32 * FWD_WARPS, FWD_BLOCKS) selective_scan_swe
         for (int k = 0; k < CT; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            h[k][j] = real.template keep<VEC>(
+            h[k][j] = real.template keep<FIT>(
                 REV ? mul2(e[s][k][j], add2(h[k][j], in[s][k][j])) : fma2(e[s][k][j], h[k][j], in[s][k][j]), j);
     }
     __syncwarp();
@@ -732,8 +735,9 @@ struct BwdStep {
   }
 };
 
-template <typename T, int G, int CT, bool VEC>
+template <typename T, int G, int CT, int FIT>
 __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd_kernel(const ScanArgs a, const ScanGrads o) {
+  constexpr bool VEC = FIT == PACKS;
   using S = Shape<T, G, CT>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   BwdMem<T, G, CT>& all = *reinterpret_cast<BwdMem<T, G, CT>*>(smem_raw);
@@ -811,8 +815,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
 #pragma unroll
           for (int k = 0; k < CT; ++k) {
             sh.h[s0 + s][k][lane] = make_ulonglong2(h[k][0], h[k][1]);
-            h[k][0] = real.template keep<VEC>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
-            h[k][1] = real.template keep<VEC>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
+            h[k][0] = real.template keep<FIT>(fma2(now.e[s][k][0], h[k][0], now.in[s][k][0]), 0);
+            h[k][1] = real.template keep<FIT>(fma2(now.e[s][k][1], h[k][1], now.in[s][k][1]), 1);
           }
         now = next;
       }
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
 #pragma unroll
         for (int k = 0; k < CT; ++k) {
           const float dt = at_t.dt[k], du = at_t.du[k], gy = at_t.gy[k];
-          const f2 g0 = real.template keep<VEC>(fma1(gy, at_t.c[0], r[k][0]), 0), g1 = real.template keep<VEC>(fma1(gy, at_t.c[1], r[k][1]), 1);
+          const f2 g0 = real.template keep<FIT>(fma1(gy, at_t.c[0], r[k][0]), 0), g1 = real.template keep<FIT>(fma1(gy, at_t.c[1], r[k][1]), 1);
           const f2 e0 = decay(dt, A2[k][0]), e1 = decay(dt, A2[k][1]);
           if (k == 0) {
             sb0 = mul1(du, g0); sb1 = mul1(du, g1);
@@ -860,8 +864,8 @@ __global__ void __launch_bounds__(32 * BWD_WARPS, BWD_BLOCKS) selective_scan_bwd
             sb0 = fma1(du, g0, sb0); sb1 = fma1(du, g1, sb1);
             sc0 = fma1(gy, h[k][0], sc0); sc1 = fma1(gy, h[k][1], sc1);
           }
-          r[k][0] = real.template keep<VEC>(mul2(e0, g0), 0);
-          r[k][1] = real.template keep<VEC>(mul2(e1, g1), 1);
+          r[k][0] = real.template keep<FIT>(mul2(e0, g0), 0);
+          r[k][1] = real.template keep<FIT>(mul2(e1, g1), 1);
           h[k][0] = at_t.h[k].x;
           h[k][1] = at_t.h[k].y;
           const f2 q0 = mul2(r[k][0], h[k][0]), q1 = mul2(r[k][1], h[k][1]);
@@ -1199,30 +1203,30 @@ int allow_smem(PerDeviceOnce& once, K kernel, int bytes) {
   });
 }
 
-template <typename T, int G, int CT, bool VEC, bool REV>
+template <typename T, int G, int CT, int FIT, bool REV>
 int sweep_launch(const ScanArgs& a, const Plan& p, float* seg, cudaStream_t s) {
   // (a sweep's warps: those of the pass that it serves, whose segments it shares)
   ScanArgs sw = a;
   sw.parts = (a.d.D + Shape<T, G, CT>::CW - 1) / Shape<T, G, CT>::CW;
   const long long units = static_cast<long long>(a.d.B) * p.segs * sw.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
-  auto kernel = selective_scan_sweep_kernel<T, G, CT, VEC, REV>;
-  constexpr int smem = FWD_WARPS * sizeof(SweepMem<T, G, CT, VEC, REV>);
+  auto kernel = selective_scan_sweep_kernel<T, G, CT, FIT, REV>;
+  constexpr int smem = FWD_WARPS * sizeof(SweepMem<T, G, CT, FIT == PACKS, REV>);
   static PerDeviceOnce once;
   if (const int rc = allow_smem(once, kernel, smem)) return rc;
   kernel<<<static_cast<unsigned>(grid), 32 * FWD_WARPS, smem, s>>>(sw, units, seg, const_cast<float*>(a.seg_dt));
   return launched();
 }
 
-template <typename T, int G, int CT, bool VEC>
+template <typename T, int G, int CT, int FIT>
 int fwd_launch(const BdhScanDesc& d, const Plan& p, float* marks, float* seg, cudaStream_t s) {
   const ScanArgs a = args_for(d, p, p.segs > 1 ? seg : nullptr);
   if (p.segs > 1)
-    if (const int rc = sweep_launch<T, G, CT, VEC, false>(a, p, seg, s)) return rc;
+    if (const int rc = sweep_launch<T, G, CT, FIT, false>(a, p, seg, s)) return rc;
   const long long units = static_cast<long long>(d.B) * p.segs * p.parts, grid = (units + FWD_WARPS - 1) / FWD_WARPS;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
-  auto kernel = selective_scan_fwd_kernel<T, G, CT, VEC>;
-  constexpr int smem = FWD_WARPS * sizeof(FwdMem<T, G, CT, VEC>);
+  auto kernel = selective_scan_fwd_kernel<T, G, CT, FIT>;
+  constexpr int smem = FWD_WARPS * sizeof(FwdMem<T, G, CT, FIT == PACKS>);
   static PerDeviceOnce once;
   if (const int rc = allow_smem(once, kernel, smem)) return rc;
   kernel<<<static_cast<unsigned>(grid), 32 * FWD_WARPS, smem, s>>>(a, units, marks);
@@ -1234,15 +1238,15 @@ struct BwdOut {
   void *dB, *dC;
 };
 
-template <typename T, int G, bool VEC>
+template <typename T, int G, int FIT>
 int bwd_launch(const BdhScanDesc& d, const Plan& p, const ScanGrads& o, float* seg, const BwdOut& out, cudaStream_t s) {
   constexpr int CT = 2;
   const ScanArgs a = args_for(d, p, p.segs > 1 ? seg : nullptr);
   if (p.segs > 1)
-    if (const int rc = sweep_launch<T, G, CT, VEC, true>(a, p, seg, s)) return rc;
+    if (const int rc = sweep_launch<T, G, CT, FIT, true>(a, p, seg, s)) return rc;
   const long long grid = static_cast<long long>(d.B) * p.segs * p.parts;
   if (grid > 0x7fffffffLL) return BDH_ERR_TOO_LARGE;
-  auto kernel = selective_scan_bwd_kernel<T, G, CT, VEC>;
+  auto kernel = selective_scan_bwd_kernel<T, G, CT, FIT>;
   constexpr int smem = sizeof(BwdMem<T, G, CT>);
   static PerDeviceOnce once;
   if (const int rc = allow_smem(once, kernel, smem)) return rc;
@@ -1261,6 +1265,12 @@ int bwd_launch(const BdhScanDesc& d, const Plan& p, const ScanGrads& o, float* s
 }
 
 template <typename F>
+int by_fit(const BdhScanDesc& d, int size, const F& f) {
+  if (packs_fit(d, size)) return f(std::integral_constant<int, PACKS>{});
+  return d.N % 4 ? f(std::integral_constant<int, MIXED>{}) : f(std::integral_constant<int, ELEMENTS>{});
+}
+
+template <typename F>
 int by_lanes(int G, const F& f) {
   switch (G) {
     case 2: return f(std::integral_constant<int, 2>{});
@@ -1276,11 +1286,11 @@ template <typename T>
 int selective_scan_fwd_of(const BdhScanDesc& d, float* marks, float* scratch, cudaStream_t s) {
   const Plan p = fwd_plan(d);
   if (p.segs > 1 && scratch == nullptr) return BDH_ERR_ARGUMENT;
-  const bool vec = packs_fit(d, sizeof(T));
   return by_lanes(p.G, [&](auto g) {
-    constexpr int G = decltype(g)::value;
-    if (vec) return p.CT == 2 ? fwd_launch<T, G, 2, true>(d, p, marks, scratch, s) : fwd_launch<T, G, 1, true>(d, p, marks, scratch, s);
-    return p.CT == 2 ? fwd_launch<T, G, 2, false>(d, p, marks, scratch, s) : fwd_launch<T, G, 1, false>(d, p, marks, scratch, s);
+    return by_fit(d, sizeof(T), [&](auto fit) {
+      constexpr int G = decltype(g)::value, FIT = decltype(fit)::value;
+      return p.CT == 2 ? fwd_launch<T, G, 2, FIT>(d, p, marks, scratch, s) : fwd_launch<T, G, 1, FIT>(d, p, marks, scratch, s);
+    });
   });
 }
 
@@ -1295,10 +1305,8 @@ int selective_scan_bwd_of(const BdhScanDesc& d, const float* marks, float* scrat
   o.da = o.bc + bc_floats(d, p);
   o.per_channel = o.da + da_floats(d, p);
   const BwdOut out{dA, dD, dbias, dB, dC};
-  const bool vec = packs_fit(d, sizeof(T));
   return by_lanes(p.G, [&](auto g) {
-    constexpr int G = decltype(g)::value;
-    return vec ? bwd_launch<T, G, true>(d, p, o, seg, out, s) : bwd_launch<T, G, false>(d, p, o, seg, out, s);
+    return by_fit(d, sizeof(T), [&](auto fit) { return bwd_launch<T, decltype(g)::value, decltype(fit)::value>(d, p, o, seg, out, s); });
   });
 }
 
