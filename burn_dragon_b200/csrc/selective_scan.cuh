@@ -408,10 +408,11 @@ __device__ __forceinline__ void load_a(const BdhScanDesc& d, int c, int n0, f2 (
 }
 
 // h exp(x), x in units of ln 2, for a whole segment's x: A and the steps may have any sign, so the factor alone may be past 2^128
-// where the product is not. It is applied in two halves, and a state of 0 (nothing came in yet) stays 0.
+// where the product is not. It is applied in two halves, and a state of 0 (nothing came in yet) or an infinite one stays what it
+// is, as it does step by step.
 __device__ __forceinline__ float grown(float h, float x) {
   const float half = ex2(0.5f * x);
-  return h == 0.f ? 0.f : h * half * half;
+  return h + h == h ? h : h * half * half;             // (0 and the infinities are their own doubles)
 }
 __device__ __forceinline__ f2 grown2(f2 h, f2 x) {
   float h0, h1, x0, x1;

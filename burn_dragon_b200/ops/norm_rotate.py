@@ -65,10 +65,10 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Opt
     """RMS norm and rotation of q [B, T, Hq, Dh] and k [B, T, Hk, Dh] (or None): -> (q', k'), contiguous, in their type.
     Rows are fp32, fp16 or bf16 and may be views into a wider projection (channels adjacent); Dh is even and at most
     512. Weights and biases: [Dh] for all heads or [heads, Dh], all of them alike (None: 1 and 0).
-    Rotation, if any: `angles` [B, T, pairs] in radians (of any floating type, as exact as that type has them), or `freqs` [2 * pairs] in cycles per position with `positions`
-    - the first token's (an int), or [T] or [B, T] integers (the single-token form has T = 1 and one position a stream).
-    `lengths` [B]: rows behind a sequence's length give 0 and take no part in any gradient. The kernels
-    refuse second derivatives and forward-mode tangents."""
+    Rotation, if any: `angles` [B, T, pairs] in radians (of any floating type, as exact as that type has them), or `freqs`
+    [2 * pairs] in cycles per position with `positions` - the first token's (an int), or [T] or [B, T] integers (the single-token form has T = 1 and one position a stream).
+    `lengths` [B]: rows behind a sequence's length give 0 and take no part in any gradient. The kernels refuse second
+    derivatives and forward-mode tangents."""
     if not (q.dim() == 4 and q.is_floating_point()):
         raise ValueError(f"q: expected a floating [B, T, heads, Dh] tensor, got {q.dtype} {tuple(q.shape)}")
     B, T, Hq, Dh = q.shape

@@ -73,8 +73,9 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
     -> (y [B, T, D] in the rows' type, hT [B, D, N] fp32). Rows are fp32, fp16 or bf16, all alike, and may be views into a
     wider projection (elements of a row adjacent). `lengths` [B]: behind a sequence's length the state stays as it
     is, y is 0, and the inputs are not read. Differentiable once in everything but `lengths`, the carried states included (the
-    kernels refuse second derivatives and forward-mode tangents); a forward pass under autograd keeps the fp32 states of every 16th step (B T D N / 4 bytes, N rounded up to 8, 16, 32
-    or 64). All states and sums are fp32, sums over rows and channels in a fixed order."""
+    kernels refuse second derivatives and forward-mode tangents); a forward pass under autograd keeps the fp32 states of
+    every 16th step (B T D N / 4 bytes, N rounded up to 8, 16, 32 or 64). All states and sums are fp32, sums over rows and
+    channels in a fixed order."""
     B, Dn, N = _check(u, dt, A, Bm, Cm, D, dt_bias, 3)
     A_.check_like(h0, u, (B, Dn, N), "h0", _state_type(u))
     lengths = A_.check_lengths(lengths, u, B)

@@ -288,6 +288,29 @@ def test_a_small_state_that_grows_within_a_few_steps(device):
     assert (torch.log(back.double()) - (115 + math.log(1e-30))).abs().max() <= 2e-4
 
 
+@pytest.mark.parametrize("N", [12, 16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_infinite_state_outlives_a_long_decay(device, N):
+    """The decay over a segment of many steps is below the numbers of fp32; each step's is not, so that an infinite state (B, C, u > 0) or
+    gradient (C, B, dy > 0) stays infinite as far as it reaches, and nothing else is touched."""
+    T, D = 3000, 24
+    g = torch.Generator().manual_seed(N)
+    r = lambda *s: (torch.rand(*s, generator=g) + 0.5).to(device)                                        # noqa: E731
+    u, dt, A, Bm, Cm, dy = r(1, T, D), r(1, T, D), -4 - r(D, N), r(1, T, N), r(1, T, N), r(1, T, D)
+    clean, h0 = S.selective_scan(u, dt, A, Bm, Cm)
+    bad = u.clone()
+    bad[0, 100, 3] = float("inf")
+    y, h = S.selective_scan(bad, dt, A, Bm, Cm)
+    assert torch.isinf(y[0, 100:, 3]).all() and torch.isinf(h[0, 3]).all()
+    rest = torch.ones(T, D, dtype=torch.bool, device=device)
+    rest[100:, 3] = False
+    assert torch.equal(y[0][rest], clean[0][rest]) and torch.equal(h[0, torch.arange(D) != 3], h0[0, torch.arange(D) != 3])
+    dy[0, 2900, 3] = float("inf")
+    leaf = u.clone().requires_grad_()
+    du, = torch.autograd.grad(S.selective_scan(leaf, dt, A, Bm, Cm)[0], leaf, dy)
+    assert torch.isinf(du[0, :2901, 3]).all() and torch.isfinite(du[0, 2901:]).all() and torch.isfinite(du[0, :, torch.arange(D) != 3]).all()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_one_stream_in_place_under_another_batch_stride(device):
     """The batch stride of a single stream means nothing."""
